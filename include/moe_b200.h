@@ -486,6 +486,96 @@ moe_status moe_gguf_layer_desc(moe_gguf* file, int layer, moe_layer_desc* desc);
  * MOE_DTYPE_Q2_0 (the decode GEMV streams it: 0.28 B per weight). */
 moe_status moe_requantize_q2_0(int src_dtype, const void* src, int E, int N, int K, void* dst, void* stream);
 
+/* ---- attention over a paged key/value cache -------------------------------------------------
+ * The other half of a decoder layer next to the routed experts: the operators that a stack of MoE
+ * layers needs to serve its GQA attention. No counterpart in the reference, whose attention belongs
+ * to the model it links against. One moe_attn per layer holds the attention's configuration and its
+ * workspace; the pools are the caller's memory and stay the caller's.
+ *
+ * Pools: k_pool and v_pool [num_pages, num_kv_heads, page_size, head_dim] in `dtype`, consecutive
+ * pages page_stride elements apart (0: contiguous), 16-byte aligned. A slot number is
+ * page * page_size + offset. A page table row lists a sequence's pages in order; entries past its
+ * length are not read. Rows of q, k and v are given by a pointer and two strides in elements (between
+ * tokens and between heads); the head_dim values of one head are consecutive, pointers are 16-byte
+ * aligned and strides are multiples of 8. Query head h reads key/value head
+ * h / (num_heads / num_kv_heads). Sums, softmax statistics and norms are held in f32.
+ *
+ * Slots past a sequence's length and pages past its last are never used and may hold anything. Device-
+ * side errors (a slot, page or position out of range, a length past the page table) never read or write
+ * out of bounds; they are latched and reported by moe_attn_check. One moe_attn's calls must not overlap
+ * on the GPU (one stream, or streams ordered by events): they share its workspace. Every call enqueues
+ * its work on `stream` without a host synchronisation and can be captured in a CUDA graph. */
+typedef struct moe_attn moe_attn;
+typedef enum { MOE_ATTN_BF16 = 0, MOE_ATTN_F16 = 1 } moe_attn_dtype;
+typedef enum {
+  MOE_ROPE_HALVES = 0,  /* pair i is (x[i], x[i + rope_dim / 2]) */
+  MOE_ROPE_ADJACENT = 1 /* pair i is (x[2 i], x[2 i + 1]) */
+} moe_rope_pairs;
+typedef struct {
+  int dtype;            /* moe_attn_dtype of q, k, v, the pools and the outputs */
+  int num_heads;        /* query heads, a multiple of num_kv_heads, at most 128 per key/value head */
+  int num_kv_heads;
+  int head_dim;         /* 64 or 128 */
+  float scale;          /* multiplier on q . k; 0: 1 / sqrt(head_dim) */
+  float softcap;        /* > 0: scores become softcap * tanh(score / softcap); 0: none */
+  int window;           /* > 0: a query sees only the last `window` positions, its own included; 0: all */
+  void* k_pool;
+  void* v_pool;
+  int64_t num_pages;    /* num_pages * page_size below 2^31 */
+  int page_size;        /* 16, 32, 64 or 128 tokens */
+  int64_t page_stride;  /* elements between pages; 0: num_kv_heads * page_size * head_dim */
+  /* Rotary positions (moe_attn_append): the first rope_dim values of a head turn pair by pair, pair i by
+   * the {cos, sin} at rope_table[position][i]. rope_dim 0: no rotation; else a multiple of 16 up to
+   * head_dim. rope_axes is 1, or 3 for positions with three axes (time, height, width): the first
+   * rope_sections[0] pairs follow axis 0, the next rope_sections[1] axis 1, the rest axis 2. */
+  const float* rope_table; /* [rope_positions, rope_dim / 2, 2] f32, device */
+  int rope_positions;
+  int rope_dim;
+  int rope_pairs;          /* moe_rope_pairs */
+  int rope_axes;
+  int rope_sections[3];    /* pairs per axis, summing to rope_dim / 2; not read with one axis */
+  /* RMS norm of each q / k head before the rotation: x / sqrt(mean(x^2) + norm_eps) * weight; NULL: none. */
+  const void* q_norm;      /* [head_dim] in dtype, device, 16-byte aligned */
+  const void* k_norm;
+  float norm_eps;
+  int device;              /* CUDA ordinal */
+  int max_seqs;            /* most sequences of one moe_attn_decode; sizes the workspace */
+} moe_attn_desc;
+moe_status moe_attn_create(const moe_attn_desc* desc, moe_attn** out);
+void moe_attn_destroy(moe_attn* attn);
+/* Device bytes the handle holds (its workspace; the pools are the caller's). */
+int64_t moe_attn_device_bytes(const moe_attn* attn);
+/* T new tokens into the cache: q [T, num_heads], k and v [T, num_kv_heads] rows; positions
+ * [rope_axes, T] int32 (not read with rope_dim 0); slots [T] int64. Writes norm(k) rotated and v to
+ * their slots and norm(q) rotated to q_out, each rounded once from f32. A slot of -1 marks a padding
+ * token: nothing is stored for it and its q_out rows are zero; so are those of a token whose slot or
+ * position is out of range (latched as MOE_ERR_BAD_IDS). Slots of one call are distinct. q_out may be q
+ * (the same strides). */
+moe_status moe_attn_append(moe_attn* attn, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                           const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                           int64_t v_token_stride, int64_t v_head_stride, int T, const int32_t* positions,
+                           const int64_t* slots, void* q_out, int64_t out_token_stride, int64_t out_head_stride,
+                           void* stream);
+/* One new token per sequence: q [B, num_heads] rows, seq_lens [B] int32 (cached tokens, the new one
+ * included), page_table [B, max_pages] int32. y [B, num_heads, head_dim] contiguous =
+ * softmax(scores) v over the sequence's last `window` (or all) positions; lse [B, num_heads] f32 or NULL =
+ * log sum exp of its scores. A sequence of length <= 0 gives y = 0 and lse = -inf. */
+moe_status moe_attn_decode(moe_attn* attn, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                           const int32_t* seq_lens, const int32_t* page_table, int max_pages, int B, void* y,
+                           float* lse, void* stream);
+/* Causal attention of a ragged batch of prompt chunks already appended: sequence b's query rows are
+ * cu_q[b] .. cu_q[b + 1] - 1 (cu_q [B + 1] int32, ascending from 0 to T), the last of its seq_lens[b]
+ * cached positions; row i sees positions up to its own. y [T, num_heads, head_dim] contiguous; lse
+ * [T, num_heads] f32 or NULL. Cached values are read in tiles: an infinite or NaN value at a position below
+ * seq_lens[b] may reach rows of that sequence that do not see the position. A chunk longer than its seq_lens
+ * is latched as MOE_ERR_BAD_IDS; its rows that have no position give y = 0 and lse = -inf. */
+moe_status moe_attn_prefill(moe_attn* attn, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                            const int32_t* cu_q, const int32_t* seq_lens, const int32_t* page_table, int max_pages,
+                            int B, int T, void* y, float* lse, void* stream);
+/* Synchronises `stream`, then reads and clears the handle's error word: MOE_OK, MOE_ERR_BAD_IDS or
+ * MOE_ERR_TIMEOUT. */
+moe_status moe_attn_check(moe_attn* attn, void* stream);
+
 /* Library version string. */
 const char* moe_version(void);
 

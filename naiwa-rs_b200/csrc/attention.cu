@@ -1,0 +1,419 @@
+// attention.cu — the moe_attn handle, its C ABI, and the append kernel of the paged key/value cache.
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <string>
+
+#include "attention_internal.cuh"
+
+namespace moe {
+namespace attn {
+
+// ---- append ----------------------------------------------------------------------------------------
+//
+// Per token and head: u = x / sqrt(mean(x^2) + eps) * w (optional), then pair i of the first rope_dim
+// values (a, b) -> (a c - b s, b c + a s) with (c, s) = rope_table[position of the pair's axis][i].
+// Bound by bytes: (heads + 2 kv_heads) * head_dim * 2 read and as many written per token. Each row
+// (one head of one token) is held by head_dim / 8 lanes with 16 bytes each, so every load and store is a
+// full 16-byte access, the norm is a shuffle reduction within the lane group, and a half-pair partner is
+// rope_dim / 16 lanes away. A lane group takes ROWS rows of one token: their loads are in flight together
+// and the lane's table values are read once for all of them.
+constexpr int APPEND_THREADS = 256;
+constexpr int ROWS = 4;
+
+struct AppendParams {
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;
+  const int32_t* positions;
+  const int64_t* slots;
+  int T, heads, kv_heads;
+  Pools pools;
+  const float* rope_table;
+  int rope_positions, rope_dim, rope_axes, adjacent;
+  int axis1, axis2;  // first pair of axis 1 and of axis 2
+  const void *q_norm, *k_norm;
+  float eps;
+  int32_t* err;
+};
+
+template <class T, int D>
+__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) {
+  constexpr int LPR = D / 8;  // lanes of a row
+  pdl_wait();
+  pdl_trigger();
+  const int rows = p.heads + 2 * p.kv_heads;
+  const int groups = (rows + ROWS - 1) / ROWS;  // lane groups per token
+  const int64_t gidx = ((int64_t)blockIdx.x * APPEND_THREADS + threadIdx.x) / LPR;
+  const int64_t t64 = gidx / groups;
+  const bool live = t64 < p.T;
+  const int t = live ? (int)t64 : 0;
+  const int r0 = (int)(gidx % groups) * ROWS;
+  const int l = threadIdx.x % LPR;
+
+  uint4 x[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = r0 + i;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (live && r < rows) {
+      const T* src;
+      if (r < p.heads) src = static_cast<const T*>(p.q) + t * p.q_ts + r * p.q_hs;
+      else if (r < p.heads + p.kv_heads) src = static_cast<const T*>(p.k) + t * p.k_ts + (r - p.heads) * p.k_hs;
+      else src = static_cast<const T*>(p.v) + t * p.v_ts + (r - p.heads - p.kv_heads) * p.v_hs;
+      x[i] = *reinterpret_cast<const uint4*>(src + l * 8);
+    }
+  }
+
+  // slot and positions: a token that fails a check is stored nowhere
+  bool ok = live;
+  int64_t slot = -1;
+  if (live) {
+    slot = p.slots[t];
+    if (slot < 0 || slot >= ((int64_t)p.pools.num_pages << p.pools.page_shift)) {
+      ok = false;
+      if (slot != -1) latch(p.err, MOE_ERR_BAD_IDS);
+    }
+  }
+  // this lane's pairs: 8 pairs j0 .. j0 + 7 (halves: value l * 8 + i pairs up at half distance), or the 4
+  // pairs l * 4 .. of its own values (adjacent)
+  const int half = p.rope_dim / 2;
+  const bool turns = l * 8 < p.rope_dim;
+  float c[8], s[8];
+  if (p.rope_dim > 0) {
+    int pos[3] = {0, 0, 0};
+    if (ok) {
+#pragma unroll
+      for (int a = 0; a < 3; ++a) {
+        if (a < p.rope_axes) pos[a] = p.positions[(int64_t)a * p.T + t];
+        if (pos[a] < 0 || pos[a] >= p.rope_positions) ok = false;
+      }
+      if (!ok) latch(p.err, MOE_ERR_BAD_IDS);
+    }
+    if (ok && turns) {
+      const int np = p.adjacent ? 4 : 8;
+      const int j0 = p.adjacent ? l * 4 : (l * 8 >= half ? l * 8 - half : l * 8);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i < np) {
+          const int j = j0 + i;
+          const int at = j >= p.axis2 ? pos[2] : j >= p.axis1 ? pos[1] : pos[0];
+          const float2 cs = __ldg(reinterpret_cast<const float2*>(p.rope_table) + (int64_t)at * half + j);
+          c[i] = cs.x;
+          s[i] = cs.y;
+        }
+      }
+    }
+  }
+  const int64_t page = slot >> p.pools.page_shift;
+  const int off = (int)(slot & ((1 << p.pools.page_shift) - 1));
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = r0 + i;
+    const bool is_v = r >= p.heads + p.kv_heads;
+    uint4 out = x[i];
+    // Every lane runs the shuffles of its row (the branch on is_v differs between lane groups of a warp, so
+    // the value rows take part with values that are then dropped).
+    float f[8];
+    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 u = Elem<T>::unpack(w[j]);
+      f[2 * j] = u.x;
+      f[2 * j + 1] = u.y;
+    }
+    const T* nw = static_cast<const T*>(r < p.heads ? p.q_norm : p.k_norm);
+    if (p.q_norm || p.k_norm) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
+#pragma unroll
+      for (int o = LPR / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
+      if (nw) {
+        const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
+        const uint4 nv = __ldg(reinterpret_cast<const uint4*>(nw + l * 8));
+        const uint32_t n4[4] = {nv.x, nv.y, nv.z, nv.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 u = Elem<T>::unpack(n4[j]);
+          f[2 * j] = f[2 * j] * inv * u.x;
+          f[2 * j + 1] = f[2 * j + 1] * inv * u.y;
+        }
+      }
+    }
+    if (p.rope_dim > 0) {
+      if (p.adjacent) {
+        if (turns && ok) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float a = f[2 * j], b = f[2 * j + 1];
+            f[2 * j] = a * c[j] - b * s[j];
+            f[2 * j + 1] = b * c[j] + a * s[j];
+          }
+        }
+      } else {
+        const int hl = half / 8;  // lanes between the two halves of a pair
+        const bool upper = l >= hl;
+        const int from = (threadIdx.x & 31) + (turns ? (upper ? -hl : hl) : 0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float other = __shfl_sync(FULL, f[j], from);
+          if (turns && ok) f[j] = upper ? f[j] * c[j] + other * s[j] : f[j] * c[j] - other * s[j];
+        }
+      }
+    }
+    if (!live || r >= rows) continue;
+    if (!is_v) out = make_uint4(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]), Elem<T>::pack(f[4], f[5]),
+                                Elem<T>::pack(f[6], f[7]));
+    if (r < p.heads) {
+      if (!ok) out = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + t * p.o_ts + r * p.o_hs + l * 8) = out;
+    } else if (ok) {
+      const int h = is_v ? r - p.heads - p.kv_heads : r - p.heads;
+      T* dst = static_cast<T*>(is_v ? p.pools.v : p.pools.k) + page * p.pools.page_stride +
+               (((int64_t)h << p.pools.page_shift) + off) * D;
+      *reinterpret_cast<uint4*>(dst + l * 8) = out;
+    }
+  }
+}
+
+template <class T>
+static cudaError_t launch_append(const AppendParams& p, int D, cudaStream_t st) {
+  const int rows = p.heads + 2 * p.kv_heads;
+  const int64_t threads = (int64_t)p.T * ceil_div(rows, ROWS) * (D / 8);
+  const dim3 grid((unsigned)((threads + APPEND_THREADS - 1) / APPEND_THREADS));
+  return D == 64 ? launch_pdl(append_kernel<T, 64>, grid, dim3(APPEND_THREADS), 0, st, p)
+                 : launch_pdl(append_kernel<T, 128>, grid, dim3(APPEND_THREADS), 0, st, p);
+}
+
+// No C++ exception crosses the C ABI.
+template <class F>
+static moe_status guarded(F&& f) noexcept {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return MOE_ERR_OOM;
+  } catch (...) {
+    return MOE_ERR_INVALID;
+  }
+}
+
+static moe_status bad(const char* call, const char* what) {
+  return fail(MOE_ERR_INVALID, std::string(call) + ": " + what);
+}
+
+static bool rows_ok(const void* p, int64_t ts, int64_t hs) { return !((uintptr_t)p & 15) && ts % 8 == 0 && hs % 8 == 0; }
+
+static Pools pools_of(const moe_attn& a) {
+  int shift = 0;
+  while ((1 << shift) < a.d.page_size) ++shift;
+  return Pools{a.d.k_pool, a.d.v_pool, a.page_stride, (int)a.d.num_pages, shift};
+}
+
+static moe_status validate(const moe_attn_desc& d) {
+  const char* me = "moe_attn_create";
+  if (d.dtype != MOE_ATTN_BF16 && d.dtype != MOE_ATTN_F16)
+    return fail(MOE_ERR_UNSUPPORTED, "moe_attn_create: dtype must be bf16 or f16");
+  if (d.head_dim != 64 && d.head_dim != 128)
+    return fail(MOE_ERR_UNSUPPORTED, "moe_attn_create: head_dim must be 64 or 128");
+  if (d.num_kv_heads <= 0 || d.num_heads <= 0 || d.num_heads % d.num_kv_heads || d.num_heads / d.num_kv_heads > 128 ||
+      d.num_heads > 65536)
+    return bad(me, "num_heads must be a multiple of num_kv_heads, at most 128 times it");
+  if (d.page_size != 16 && d.page_size != 32 && d.page_size != 64 && d.page_size != 128)
+    return bad(me, "page_size must be 16, 32, 64 or 128");
+  if (d.num_pages <= 0 || d.num_pages * d.page_size > 0x7fffffffll || d.num_pages > 0x7fffffffll)
+    return bad(me, "num_pages * page_size must be in 1 .. 2^31 - 1");
+  const int64_t packed = (int64_t)d.num_kv_heads * d.page_size * d.head_dim;
+  if (d.page_stride && (d.page_stride < packed || d.page_stride % 8))
+    return bad(me, "page_stride must be a multiple of 8 that holds a page");
+  if (!d.k_pool || !d.v_pool || ((uintptr_t)d.k_pool & 15) || ((uintptr_t)d.v_pool & 15))
+    return bad(me, "the pools must be 16-byte aligned device memory");
+  if (!(d.scale >= 0.0f) || !std::isfinite(d.scale) || !(d.softcap >= 0.0f) || !std::isfinite(d.softcap) || d.window < 0)
+    return bad(me, "scale, softcap and window must be finite and not negative");
+  if (d.rope_dim < 0 || d.rope_dim % 16 || d.rope_dim > d.head_dim)
+    return bad(me, "rope_dim must be a multiple of 16 up to head_dim");
+  if (d.rope_dim) {
+    if (!d.rope_table || ((uintptr_t)d.rope_table & 15) || d.rope_positions <= 0)
+      return bad(me, "rope_dim needs a 16-byte aligned rope_table with rope_positions rows");
+    if (d.rope_pairs != MOE_ROPE_HALVES && d.rope_pairs != MOE_ROPE_ADJACENT) return bad(me, "unknown rope_pairs");
+    if (d.rope_axes != 1 && d.rope_axes != 3) return bad(me, "rope_axes must be 1 or 3");
+    if (d.rope_axes == 3) {
+      int64_t sum = 0;
+      for (int a = 0; a < 3; ++a) {
+        if (d.rope_sections[a] < 0) return bad(me, "negative rope section");
+        sum += d.rope_sections[a];
+      }
+      if (sum != d.rope_dim / 2) return bad(me, "rope_sections must sum to rope_dim / 2");
+    }
+  }
+  if (((uintptr_t)d.q_norm & 15) || ((uintptr_t)d.k_norm & 15)) return bad(me, "norm weights must be 16-byte aligned");
+  if ((d.q_norm || d.k_norm) && !(d.norm_eps >= 0.0f)) return bad(me, "norm_eps must not be negative");
+  if (d.max_seqs <= 0 || (int64_t)d.max_seqs * d.num_heads > (1 << 28)) return bad(me, "max_seqs out of range");
+  return MOE_OK;
+}
+
+}  // namespace attn
+}  // namespace moe
+
+using namespace moe;
+using namespace moe::attn;
+
+extern "C" moe_status moe_attn_create(const moe_attn_desc* desc, moe_attn** out) {
+  return guarded([&]() -> moe_status {
+    if (!desc || !out) return bad("moe_attn_create", "null desc or out");
+    *out = nullptr;
+    MOE_TRY(validate(*desc));
+    DeviceGuard guard(desc->device);
+    if (!guard.ok) return bad("moe_attn_create", "no such device");
+    moe_attn* a = new (std::nothrow) moe_attn();
+    if (!a) return fail(MOE_ERR_OOM, "moe_attn_create: host allocation failed");
+    a->d = *desc;
+    a->group = desc->num_heads / desc->num_kv_heads;
+    a->scale = desc->scale > 0.0f ? desc->scale : 1.0f / std::sqrt((float)desc->head_dim);
+    a->page_stride =
+        desc->page_stride ? desc->page_stride : (int64_t)desc->num_kv_heads * desc->page_size * desc->head_dim;
+    const moe_status st = [&]() -> moe_status {
+      MOE_CUDA_TRY(cudaDeviceGetAttribute(&a->sms, cudaDevAttrMultiProcessorCount, desc->device));
+      const int rows = decode_rows(a->group);
+      const size_t slots = (size_t)decode_max_ctas(a->sms) * 2;  // a CTA leaves at most two partial results
+      const size_t acc = slots * rows * desc->head_dim * sizeof(float), ml = slots * rows * sizeof(float2);
+      const size_t cnt = (size_t)desc->max_seqs * desc->num_kv_heads * decode_row_blocks(a->group) * sizeof(int32_t);
+      MOE_CUDA_TRY(cudaMalloc(&a->partial, acc));
+      MOE_CUDA_TRY(cudaMalloc(&a->partial_ml, ml));
+      MOE_CUDA_TRY(cudaMalloc(&a->counters, cnt));
+      MOE_CUDA_TRY(cudaMalloc(&a->err, sizeof(int32_t)));
+      MOE_CUDA_TRY(cudaMemset(a->counters, 0, cnt));
+      MOE_CUDA_TRY(cudaMemset(a->err, 0, sizeof(int32_t)));
+      MOE_CUDA_TRY(cudaDeviceSynchronize());  // the zeros are in place for a first call on any stream
+      a->bytes = (int64_t)(acc + ml + cnt + sizeof(int32_t));
+      MOE_TRY(prepare_decode(*a));
+      MOE_TRY(prepare_prefill(*a));
+      for (int i = 0; i < 2; ++i)
+        MOE_TRY(make_page_tmap(i ? &a->v_map : &a->k_map, desc->dtype, i ? desc->v_pool : desc->k_pool, desc->head_dim,
+                               desc->page_size, desc->num_kv_heads, desc->num_pages, a->page_stride));
+      return MOE_OK;
+    }();
+    if (st != MOE_OK) {
+      const std::string msg = last_error_message();
+      moe_attn_destroy(a);
+      return fail(st, msg);
+    }
+    *out = a;
+    return MOE_OK;
+  });
+}
+
+extern "C" void moe_attn_destroy(moe_attn* a) {
+  if (!a) return;
+  DeviceGuard guard(a->d.device);
+  cudaFree(a->partial);
+  cudaFree(a->partial_ml);
+  cudaFree(a->counters);
+  cudaFree(a->err);
+  delete a;
+}
+
+extern "C" int64_t moe_attn_device_bytes(const moe_attn* a) { return a ? a->bytes : 0; }
+
+extern "C" moe_status moe_attn_append(moe_attn* a, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                      const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                      int64_t v_token_stride, int64_t v_head_stride, int T, const int32_t* positions,
+                                      const int64_t* slots, void* q_out, int64_t out_token_stride,
+                                      int64_t out_head_stride, void* stream) {
+  return guarded([&]() -> moe_status {
+    const char* me = "moe_attn_append";
+    if (!a) return bad(me, "null handle");
+    if (T < 0) return bad(me, "T must not be negative");
+    if (T == 0) return MOE_OK;
+    if (!q || !k || !v || !slots || !q_out || (a->d.rope_dim && !positions)) return bad(me, "null pointer");
+    if (!rows_ok(q, q_token_stride, q_head_stride) || !rows_ok(k, k_token_stride, k_head_stride) ||
+        !rows_ok(v, v_token_stride, v_head_stride) || !rows_ok(q_out, out_token_stride, out_head_stride))
+      return bad(me, "rows must be 16-byte aligned with strides that are multiples of 8");
+    AppendParams p{};
+    p.q = q, p.k = k, p.v = v, p.q_out = q_out;
+    p.q_ts = q_token_stride, p.q_hs = q_head_stride, p.k_ts = k_token_stride, p.k_hs = k_head_stride;
+    p.v_ts = v_token_stride, p.v_hs = v_head_stride, p.o_ts = out_token_stride, p.o_hs = out_head_stride;
+    p.positions = positions, p.slots = slots, p.T = T;
+    p.heads = a->d.num_heads, p.kv_heads = a->d.num_kv_heads;
+    p.pools = pools_of(*a);
+    p.rope_table = a->d.rope_table, p.rope_positions = a->d.rope_positions, p.rope_dim = a->d.rope_dim;
+    p.rope_axes = a->d.rope_axes, p.adjacent = a->d.rope_pairs == MOE_ROPE_ADJACENT;
+    const bool axes = a->d.rope_axes == 3;
+    p.axis1 = axes ? a->d.rope_sections[0] : a->d.rope_dim;
+    p.axis2 = axes ? a->d.rope_sections[0] + a->d.rope_sections[1] : a->d.rope_dim;
+    p.q_norm = a->d.q_norm, p.k_norm = a->d.k_norm, p.eps = a->d.norm_eps;
+    p.err = a->err;
+    DeviceGuard guard(a->d.device);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    MOE_CUDA_TRY(a->d.dtype == MOE_ATTN_BF16 ? launch_append<__nv_bfloat16>(p, a->d.head_dim, st)
+                                             : launch_append<__half>(p, a->d.head_dim, st));
+    return MOE_OK;
+  });
+}
+
+extern "C" moe_status moe_attn_decode(moe_attn* a, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                      const int32_t* seq_lens, const int32_t* page_table, int max_pages, int B,
+                                      void* y, float* lse, void* stream) {
+  return guarded([&]() -> moe_status {
+    const char* me = "moe_attn_decode";
+    if (!a) return bad(me, "null handle");
+    if (B < 0 || B > a->d.max_seqs) return bad(me, "B must be in 0 .. max_seqs");
+    if (B == 0) return MOE_OK;
+    if (!q || !seq_lens || !page_table || !y || max_pages <= 0) return bad(me, "null pointer or no pages");
+    if (!rows_ok(q, q_token_stride, q_head_stride) || ((uintptr_t)y & 15))
+      return bad(me, "rows must be 16-byte aligned with strides that are multiples of 8");
+    if ((int64_t)max_pages * a->d.page_size > 0x7fffffffll) return bad(me, "max_pages * page_size above 2^31 - 1");
+    DecodeParams p{};
+    p.q = q, p.q_token_stride = q_token_stride, p.q_head_stride = q_head_stride;
+    p.seq_lens = seq_lens, p.page_table = page_table, p.max_pages = max_pages, p.B = B;
+    p.heads = a->d.num_heads, p.kv_heads = a->d.num_kv_heads, p.group = a->group;
+    p.row_blocks = decode_row_blocks(a->group);
+    p.pools = pools_of(*a);
+    p.scale = a->scale, p.softcap = a->d.softcap, p.window = a->d.window;
+    p.y = y, p.lse = lse;
+    p.partial = a->partial, p.partial_ml = a->partial_ml, p.counters = a->counters, p.err = a->err;
+    DeviceGuard guard(a->d.device);
+    return launch_decode(*a, p, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" moe_status moe_attn_prefill(moe_attn* a, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                       const int32_t* cu_q, const int32_t* seq_lens, const int32_t* page_table,
+                                       int max_pages, int B, int T, void* y, float* lse, void* stream) {
+  return guarded([&]() -> moe_status {
+    const char* me = "moe_attn_prefill";
+    if (!a) return bad(me, "null handle");
+    if (B < 0 || T < 0) return bad(me, "B and T must not be negative");
+    if (B == 0 || T == 0) return MOE_OK;
+    if (!q || !cu_q || !seq_lens || !page_table || !y || max_pages <= 0) return bad(me, "null pointer or no pages");
+    if (!rows_ok(q, q_token_stride, q_head_stride) || ((uintptr_t)y & 15))
+      return bad(me, "rows must be 16-byte aligned with strides that are multiples of 8");
+    if ((int64_t)max_pages * a->d.page_size > 0x7fffffffll) return bad(me, "max_pages * page_size above 2^31 - 1");
+    PrefillParams p{};
+    p.q = q, p.q_token_stride = q_token_stride, p.q_head_stride = q_head_stride;
+    p.cu_q = cu_q, p.seq_lens = seq_lens, p.page_table = page_table, p.max_pages = max_pages, p.B = B, p.T = T;
+    p.heads = a->d.num_heads, p.kv_heads = a->d.num_kv_heads, p.group = a->group;
+    const Pools pools = pools_of(*a);
+    p.num_pages = pools.num_pages, p.page_shift = pools.page_shift;
+    p.scale = a->scale, p.softcap = a->d.softcap, p.window = a->d.window;
+    p.y = y, p.lse = lse, p.err = a->err;
+    DeviceGuard guard(a->d.device);
+    return launch_prefill(*a, p, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" moe_status moe_attn_check(moe_attn* a, void* stream) {
+  return guarded([&]() -> moe_status {
+    if (!a) return bad("moe_attn_check", "null handle");
+    DeviceGuard guard(a->d.device);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int32_t word = 0;
+    MOE_CUDA_TRY(cudaMemcpyAsync(&word, a->err, sizeof(word), cudaMemcpyDeviceToHost, st));
+    MOE_CUDA_TRY(cudaStreamSynchronize(st));
+    if (!word) return MOE_OK;
+    MOE_CUDA_TRY(cudaMemsetAsync(a->err, 0, sizeof(word), st));
+    MOE_CUDA_TRY(cudaStreamSynchronize(st));
+    return fail((moe_status)word, word == MOE_ERR_TIMEOUT ? "attention: a bounded device-side wait gave up"
+                                                          : "attention: a slot, page, position or length out of range");
+  });
+}

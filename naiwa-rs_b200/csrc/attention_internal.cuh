@@ -1,0 +1,120 @@
+// attention_internal.cuh — the moe_attn handle, the kernels' parameter blocks and the helpers that the
+// paged-attention kernels share.
+#pragma once
+#include <cuda.h>
+
+#include <exception>
+
+#include "moe_internal.cuh"
+#include "tensor_map.cuh"
+
+struct moe_attn {
+  moe_attn_desc d;
+  int group;            // query heads per key/value head
+  int sms;
+  int64_t page_stride;  // elements
+  float scale;
+  // decode workspace: see attention_decode.cu
+  float* partial = nullptr;
+  float2* partial_ml = nullptr;
+  int32_t* counters = nullptr;
+  int32_t* err = nullptr;
+  int64_t bytes = 0;
+  CUtensorMap k_map, v_map;  // prefill's page boxes
+};
+
+namespace moe {
+namespace attn {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+struct Pools {
+  void* k;
+  void* v;
+  int64_t page_stride;  // elements
+  int num_pages, page_shift;
+};
+
+struct DecodeParams {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  const int32_t* seq_lens;
+  const int32_t* page_table;
+  int max_pages, B, heads, kv_heads, group;
+  int row_blocks;  // blocks of query heads per key/value head
+  Pools pools;
+  float scale, softcap;
+  int window;
+  void* y;
+  float* lse;
+  float* partial;
+  float2* partial_ml;
+  int32_t* counters;
+  int32_t* err;
+};
+
+struct PrefillParams {
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  const int32_t* cu_q;
+  const int32_t* seq_lens;
+  const int32_t* page_table;
+  int max_pages, B, T, heads, kv_heads, group;
+  int num_pages, page_shift;
+  float scale, softcap;
+  int window;
+  void* y;
+  float* lse;
+  int32_t* err;
+};
+
+// Rows of query heads that one decode work unit holds, and the sizes that follow from them.
+inline int decode_rows(int group) { return group <= 8 ? 8 : 16; }
+inline int decode_row_blocks(int group) { return ceil_div(group, decode_rows(group)); }
+int decode_max_ctas(int sms);
+
+// Per-device kernel attributes of the handle's variant; called with its device current.
+moe_status prepare_decode(const moe_attn& a);
+moe_status prepare_prefill(const moe_attn& a);
+moe_status launch_decode(const moe_attn& a, const DecodeParams& p, cudaStream_t st);
+moe_status launch_prefill(const moe_attn& a, const PrefillParams& p, cudaStream_t st);
+// 4-D map over a pool: box of 64 values x min(page_size, 128) tokens of one head of one page, SWIZZLE_128B.
+moe_status make_page_tmap(CUtensorMap* map, int dtype, const void* pool, int head_dim, int page_size, int kv_heads,
+                          int64_t num_pages, int64_t page_stride);
+
+// ---- element types ------------------------------------------------------------------------------
+
+template <class T>
+struct Elem;
+template <>
+struct Elem<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma_bf16(d, a, b0, b1);
+  }
+};
+template <>
+struct Elem<__half> {
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    mma_f16(d, a, b0, b1);
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void latch(int32_t* err, moe_status st) { atomicCAS(err, 0, (int32_t)st); }
+
+}  // namespace attn
+}  // namespace moe

@@ -42,6 +42,7 @@
 #include <string>
 
 #include "moe_internal.cuh"
+#include "tensor_map.cuh"
 
 namespace moe {
 namespace tc {
@@ -1039,21 +1040,26 @@ static PFN_encodeTiled get_encode() {
   return fn;
 }
 
-// 2-D map over an f16 [rows, cols] row-major buffer, box 64 columns x 32 rows, SWIZZLE_128B.
-moe_status make_row_tmap(void* map_out, const void* base, int64_t rows, int cols) {
+moe_status encode_tmap_sw128(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                             const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
   PFN_encodeTiled enc = get_encode();
   if (!enc) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
-  if (((uintptr_t)base & 15) || (cols * 2) % 16) return fail(MOE_ERR_INVALID, "tensor map: misaligned rows");
-  CUtensorMap* m = static_cast<CUtensorMap*>(map_out);
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
-  cuuint32_t box[2] = {64, (cuuint32_t)tc::TMA_ROWS};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = enc(map, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
   return MOE_OK;
+}
+
+// 2-D map over an f16 [rows, cols] row-major buffer, box 64 columns x 32 rows, SWIZZLE_128B.
+moe_status make_row_tmap(void* map_out, const void* base, int64_t rows, int cols) {
+  if (((uintptr_t)base & 15) || (cols * 2) % 16) return fail(MOE_ERR_INVALID, "tensor map: misaligned rows");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)cols * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)tc::TMA_ROWS};
+  return encode_tmap_sw128(static_cast<CUtensorMap*>(map_out), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides,
+                           box);
 }
 
 size_t tensor_map_bytes() { return sizeof(CUtensorMap); }

@@ -18,3 +18,4 @@ from .doorbell import Ring  # noqa: F401,E402
 from .cpu import CpuExperts, Executor, add_f32_into_bf16, cpu_isa  # noqa: F401,E402
 from .paged import PagedMoE  # noqa: F401,E402
 from .gguf import GGUFFile  # noqa: F401,E402
+from .attention import AttentionConfig, PagedAttention, kv_pools, page_slots, rope_table  # noqa: F401,E402

@@ -25,6 +25,8 @@ STATUS_NAMES = {
 }
 
 DTYPE_BF16, DTYPE_Q8_0, DTYPE_Q4_K, DTYPE_FP8_E4M3_B128, DTYPE_Q2_0 = 0, 1, 2, 3, 4
+ATTN_BF16, ATTN_F16 = 0, 1
+ROPE_HALVES, ROPE_ADJACENT = 0, 1
 ROUTER_SOFTMAX, ROUTER_SOFTMAX_RENORM, ROUTER_SIGMOID_GROUP = 0, 1, 2
 
 
@@ -60,6 +62,34 @@ class LayerDesc(ctypes.Structure):
     ]
 
 
+class AttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int),
+        ("num_heads", ctypes.c_int),
+        ("num_kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("window", ctypes.c_int),
+        ("k_pool", ctypes.c_void_p),
+        ("v_pool", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int),
+        ("page_stride", ctypes.c_int64),
+        ("rope_table", ctypes.c_void_p),
+        ("rope_positions", ctypes.c_int),
+        ("rope_dim", ctypes.c_int),
+        ("rope_pairs", ctypes.c_int),
+        ("rope_axes", ctypes.c_int),
+        ("rope_sections", ctypes.c_int * 3),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("norm_eps", ctypes.c_float),
+        ("device", ctypes.c_int),
+        ("max_seqs", ctypes.c_int),
+    ]
+
+
 MOE_ID_NONE = 0xFFFFFFFF  # empty top-k slot: skipped by the plan (include/moe_b200.h)
 
 LIB_PATH = _build.LIB
@@ -75,7 +105,7 @@ def lib():
         if not alt and (not os.path.exists(LIB_PATH) or os.environ.get("MOE_B200_REBUILD") == "1"):
             _build.build()
         L = ctypes.CDLL(alt or LIB_PATH)
-        P, i, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+        P, i, f, L64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
         sigs = {
             "moe_layer_create": (i, [ctypes.POINTER(LayerDesc), ctypes.POINTER(ctypes.c_void_p)]),
             "moe_layer_warmup": (i, [P, i]),
@@ -161,6 +191,13 @@ def lib():
             "moe_gguf_get_int": (i, [P, ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64)]),
             "moe_gguf_get_str": (ctypes.c_size_t, [P, ctypes.c_char_p, ctypes.c_char_p, ctypes.c_size_t]),
             "moe_gguf_layer_desc": (i, [P, i, ctypes.POINTER(LayerDesc)]),
+            "moe_attn_create": (i, [ctypes.POINTER(AttnDesc), ctypes.POINTER(ctypes.c_void_p)]),
+            "moe_attn_destroy": (None, [P]),
+            "moe_attn_device_bytes": (ctypes.c_int64, [P]),
+            "moe_attn_append": (i, [P, P, L64, L64, P, L64, L64, P, L64, L64, i, P, P, P, L64, L64, P]),
+            "moe_attn_decode": (i, [P, P, L64, L64, P, P, i, i, P, P, P]),
+            "moe_attn_prefill": (i, [P, P, L64, L64, P, P, P, i, i, i, P, P, P]),
+            "moe_attn_check": (i, [P, P]),
             "moe_version": (ctypes.c_char_p, []),
         }
         for name, (res, args) in sigs.items():
