@@ -1,4 +1,5 @@
 // attention.cu — the moe_attn handle, its C ABI, and the append kernel of the paged key/value cache.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -17,7 +18,8 @@ namespace attn {
 // (one head of one token) is held by head_dim / 8 lanes with 16 bytes each, so every load and store is a
 // full 16-byte access, the norm is a shuffle reduction within the lane group, and a half-pair partner is
 // rope_dim / 16 lanes away. A lane group takes ROWS rows of one token: their loads are in flight together
-// and the lane's table values are read once for all of them.
+// and the lane's table values are read once for all of them. Blocks are (lanes of a row, lane groups, tokens), so a
+// thread finds its work without a division.
 constexpr int APPEND_THREADS = 256;
 constexpr int ROWS = 4;
 
@@ -43,13 +45,12 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
   pdl_wait();
   pdl_trigger();
   const int rows = p.heads + 2 * p.kv_heads;
-  const int groups = (rows + ROWS - 1) / ROWS;  // lane groups per token
-  const int64_t gidx = ((int64_t)blockIdx.x * APPEND_THREADS + threadIdx.x) / LPR;
-  const int64_t t64 = gidx / groups;
+  const int l = threadIdx.x;                                            // this lane's 8 values of a row
+  const int r0 = (blockIdx.y * blockDim.y + threadIdx.y) * ROWS;        // first row
+  const int64_t t64 = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
   const bool live = t64 < p.T;
-  const int t = live ? (int)t64 : 0;
-  const int r0 = (int)(gidx % groups) * ROWS;
-  const int l = threadIdx.x % LPR;
+  const int64_t t = live ? t64 : 0;
+  const int lane = (threadIdx.x + blockDim.x * (threadIdx.y + blockDim.y * threadIdx.z)) & 31;
 
   uint4 x[ROWS];
 #pragma unroll
@@ -67,9 +68,14 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
 
   // slot and positions: a token that fails a check is stored nowhere
   bool ok = live;
-  int64_t slot = -1;
+  const int64_t slot = live ? p.slots[t] : -1;
+  int pos[3] = {0, 0, 0};
+  if (live && p.rope_dim > 0) {
+#pragma unroll
+    for (int a = 0; a < 3; ++a)
+      if (a < p.rope_axes) pos[a] = p.positions[(int64_t)a * p.T + t];
+  }
   if (live) {
-    slot = p.slots[t];
     if (slot < 0 || slot >= ((int64_t)p.pools.num_pages << p.pools.page_shift)) {
       ok = false;
       if (slot != -1) latch(p.err, MOE_ERR_BAD_IDS);
@@ -81,16 +87,23 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
   const bool turns = l * 8 < p.rope_dim;
   float c[8], s[8];
   if (p.rope_dim > 0) {
-    int pos[3] = {0, 0, 0};
     if (ok) {
 #pragma unroll
-      for (int a = 0; a < 3; ++a) {
-        if (a < p.rope_axes) pos[a] = p.positions[(int64_t)a * p.T + t];
+      for (int a = 0; a < 3; ++a)
         if (pos[a] < 0 || pos[a] >= p.rope_positions) ok = false;
-      }
       if (!ok) latch(p.err, MOE_ERR_BAD_IDS);
     }
-    if (ok && turns) {
+    if (ok && turns && p.rope_axes == 1) {  // one table row: two pairs per 16-byte load
+      const int j0 = p.adjacent ? l * 4 : (l * 8 >= half ? l * 8 - half : l * 8);
+      const float4* row = reinterpret_cast<const float4*>(p.rope_table + ((int64_t)pos[0] * half + j0) * 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < 2 || !p.adjacent) {
+          const float4 cs = __ldg(row + i);
+          c[2 * i] = cs.x, s[2 * i] = cs.y, c[2 * i + 1] = cs.z, s[2 * i + 1] = cs.w;
+        }
+      }
+    } else if (ok && turns) {
       const int np = p.adjacent ? 4 : 8;
       const int j0 = p.adjacent ? l * 4 : (l * 8 >= half ? l * 8 - half : l * 8);
 #pragma unroll
@@ -154,7 +167,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
       } else {
         const int hl = half / 8;  // lanes between the two halves of a pair
         const bool upper = l >= hl;
-        const int from = (threadIdx.x & 31) + (turns ? (upper ? -hl : hl) : 0);
+        const int from = lane + (turns ? (upper ? -hl : hl) : 0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float other = __shfl_sync(FULL, f[j], from);
@@ -180,10 +193,12 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
 template <class T>
 static cudaError_t launch_append(const AppendParams& p, int D, cudaStream_t st) {
   const int rows = p.heads + 2 * p.kv_heads;
-  const int64_t threads = (int64_t)p.T * ceil_div(rows, ROWS) * (D / 8);
-  const dim3 grid((unsigned)((threads + APPEND_THREADS - 1) / APPEND_THREADS));
-  return D == 64 ? launch_pdl(append_kernel<T, 64>, grid, dim3(APPEND_THREADS), 0, st, p)
-                 : launch_pdl(append_kernel<T, 128>, grid, dim3(APPEND_THREADS), 0, st, p);
+  const int lanes = D / 8, groups = ceil_div(rows, ROWS);
+  const int by = std::min(groups, APPEND_THREADS / lanes);
+  const int bz = std::max(1, std::min(p.T, APPEND_THREADS / (lanes * by)));
+  const dim3 block(lanes, by, bz), grid((unsigned)ceil_div(p.T, bz), (unsigned)ceil_div(groups, by));
+  return D == 64 ? launch_pdl(append_kernel<T, 64>, grid, block, 0, st, p)
+                 : launch_pdl(append_kernel<T, 128>, grid, block, 0, st, p);
 }
 
 // No C++ exception crosses the C ABI.
@@ -276,11 +291,14 @@ extern "C" moe_status moe_attn_create(const moe_attn_desc* desc, moe_attn** out)
       MOE_CUDA_TRY(cudaDeviceGetAttribute(&a->sms, cudaDevAttrMultiProcessorCount, desc->device));
       const int rows = decode_rows(a->group);
       const size_t slots = (size_t)decode_max_ctas(a->sms) * 2;  // a CTA leaves at most two partial results
-      const size_t acc = slots * rows * desc->head_dim * sizeof(float), ml = slots * rows * sizeof(float2);
-      const size_t cnt = (size_t)desc->max_seqs * desc->num_kv_heads * decode_row_blocks(a->group) * sizeof(int32_t);
+      const size_t acc = slots * rows * desc->head_dim * sizeof(float), ml = 2 * slots * rows * sizeof(float2);
+      const size_t units = (size_t)desc->max_seqs * desc->num_kv_heads * decode_row_blocks(a->group);
+      const size_t cnt = (units + slots) * sizeof(int32_t);
       MOE_CUDA_TRY(cudaMalloc(&a->partial, acc));
       MOE_CUDA_TRY(cudaMalloc(&a->partial_ml, ml));
+      a->group_ml = a->partial_ml + slots * rows;
       MOE_CUDA_TRY(cudaMalloc(&a->counters, cnt));
+      a->group_counters = a->counters + units;
       MOE_CUDA_TRY(cudaMalloc(&a->err, sizeof(int32_t)));
       MOE_CUDA_TRY(cudaMemset(a->counters, 0, cnt));
       MOE_CUDA_TRY(cudaMemset(a->err, 0, sizeof(int32_t)));
@@ -371,7 +389,8 @@ extern "C" moe_status moe_attn_decode(moe_attn* a, const void* q, int64_t q_toke
     p.pools = pools_of(*a);
     p.scale = a->scale, p.softcap = a->d.softcap, p.window = a->d.window;
     p.y = y, p.lse = lse;
-    p.partial = a->partial, p.partial_ml = a->partial_ml, p.counters = a->counters, p.err = a->err;
+    p.partial = a->partial, p.partial_ml = a->partial_ml, p.group_ml = a->group_ml;
+    p.counters = a->counters, p.group_counters = a->group_counters, p.err = a->err;
     DeviceGuard guard(a->d.device);
     return launch_decode(*a, p, static_cast<cudaStream_t>(stream));
   });

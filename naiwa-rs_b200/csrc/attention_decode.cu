@@ -32,6 +32,9 @@ constexpr int THREADS = WARPS * 32;
 constexpr int BLK = 16;      // tokens of a block
 constexpr int CTAS_PER_SM = 2;
 constexpr int MIN_SLICE = 2 * WARPS;  // blocks
+constexpr int JOIN = 8;               // parts joined at once
+constexpr int ONE_JOIN = 2 * JOIN;    // more parts than these are joined in two steps, in groups of JOIN
+constexpr int SHORT = 4 * WARPS;      // blocks up to which a (sequence, head) is never split
 
 int decode_max_ctas(int sms) { return sms * CTAS_PER_SM; }
 
@@ -79,13 +82,15 @@ struct Seq {
   int len, lo, first, nb;
 };
 
-__device__ __forceinline__ Seq seq_of(const DecodeParams& p, int b) {
+// pad > 0: every sequence with a token counts that many blocks (the ones past its last token are empty).
+__device__ __forceinline__ Seq seq_of(const DecodeParams& p, int b, int pad) {
   Seq s;
   const int cap = p.max_pages << p.pools.page_shift;
   s.len = max(0, min(__ldg(p.seq_lens + b), cap));
   s.lo = p.window > 0 ? max(0, s.len - p.window) : 0;
   s.first = s.lo / BLK;
   s.nb = (s.len + BLK - 1) / BLK - s.first;
+  if (pad > 0 && s.nb > 0) s.nb = pad;
   return s;
 }
 
@@ -95,7 +100,7 @@ struct Cursor {
   Seq s;
 };
 
-__device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c, int n, int vheads) {
+__device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c, int n, int vheads, int pad) {
   c.j += n;
   while (c.j >= c.s.nb && c.b < p.B) {
     c.j -= c.s.nb;
@@ -104,16 +109,10 @@ __device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c, int n,
       do {
         ++c.b;
         if (c.b >= p.B) return;
-        c.s = seq_of(p, c.b);
+        c.s = seq_of(p, c.b, pad);
       } while (c.s.nb == 0);
     }
   }
-}
-
-// The page of cursor c's block (one out of range is latched, and its tokens read as zeros).
-__device__ __forceinline__ int page_of(const DecodeParams& p, const Cursor& c) {
-  const int tok = (c.s.first + c.j) * BLK;
-  return __ldg(p.page_table + (int64_t)c.b * p.max_pages + (tok >> p.pools.page_shift));
 }
 
 // Four values of an output row from the joined sums (maximum M in units of log2, sum of weights L), and its lse.
@@ -125,6 +124,77 @@ __device__ __forceinline__ void store_row(const DecodeParams& p, int64_t row, in
   if (p.lse && d == 0) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
 }
 
+// Workspace slot of part k of a (sequence, head) whose first CTA is c0: a CTA's part that began in an earlier
+// CTA's slice goes to its slot 0, one that begins in its own slice to slot 1.
+__device__ __forceinline__ int part_slot(int c0, int k) { return (c0 + k) * 2 + (k == 0 ? 1 : 0); }
+
+// A (sequence, head) that several CTAs share: their number, the first one, its counter, its first output row.
+struct Split {
+  int parts, c0, unit;
+  int64_t out_row;
+  int rows;
+};
+
+// Counts an arrival; true for the last of `need`, which leaves the counter at zero for the next call.
+__device__ __forceinline__ bool arrive(int32_t* counter, int need) {
+  const bool last = atomicAdd(counter, 1) == need - 1;
+  if (last) *counter = 0;
+  return last;
+}
+
+__device__ __forceinline__ bool arrive_first(const DecodeParams& p, const Split& sp, int k) {
+  if (sp.parts <= ONE_JOIN) return arrive(p.counters + sp.unit, sp.parts);
+  const int g0 = k / JOIN * JOIN;
+  return arrive(p.group_counters + part_slot(sp.c0, g0), min(JOIN, sp.parts - g0));
+}
+
+// Joins parts k0, k0 + step, .. (n of them, in this order; ml: their maxima and sums) into the output, or, with to_ml,
+// into part k0's slot of the workspace. A chunk's loads are all in flight together.
+template <class T, int D, int ROWS>
+__device__ __forceinline__ void join(const DecodeParams& p, const Split& sp, int k0, int step, int n, const float2* ml,
+                                     float2* to_ml) {
+  for (int e = threadIdx.x; e < sp.rows * (D / 4); e += THREADS) {
+    const int row = e / (D / 4), d = (e % (D / 4)) * 4;
+    float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int k = 0; k < n; k += JOIN) {
+      float2 s[JOIN];
+      float4 v[JOIN];
+#pragma unroll
+      for (int i = 0; i < JOIN; ++i) {
+        s[i] = make_float2(-INFINITY, 0.0f);
+        v[i] = make_float4(0, 0, 0, 0);
+        if (k + i < n) {
+          const int64_t at = (int64_t)part_slot(sp.c0, k0 + (k + i) * step) * ROWS + row;
+          s[i] = __ldcg(ml + at);
+          v[i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
+        }
+      }
+      float mx = M;
+#pragma unroll
+      for (int i = 0; i < JOIN; ++i) mx = fmaxf(mx, s[i].x);
+      const float ref = mx == -INFINITY ? 0.0f : mx;
+      const float f = ex2(M - ref);
+      M = mx;
+      L *= f;
+      o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+      for (int i = 0; i < JOIN; ++i) {
+        const float w = ex2(s[i].x - ref);
+        L = fmaf(s[i].y, w, L);
+        o.x = fmaf(v[i].x, w, o.x), o.y = fmaf(v[i].y, w, o.y), o.z = fmaf(v[i].z, w, o.z), o.w = fmaf(v[i].w, w, o.w);
+      }
+    }
+    if (!to_ml) {
+      store_row<T, D>(p, sp.out_row + row, d, o, M, L);
+    } else {  // the slot's own values are read by this thread alone, its ml by others: that goes elsewhere
+      const int64_t at = (int64_t)part_slot(sp.c0, k0) * ROWS + row;
+      __stcg(reinterpret_cast<float4*>(p.partial + at * D + d), o);
+      if (d == 0) __stcg(to_ml + at, make_float2(M, L));
+    }
+  }
+}
+
 template <class T, int D, int NT>
 __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodeParams p) {
   using S = Shape<D>;
@@ -133,10 +203,11 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
   extern __shared__ __align__(128) unsigned char smem[];
   float* red = reinterpret_cast<float*>(smem + WARPS * S::STAGES * 2 * S::HALF);
   float2* red_ml = reinterpret_cast<float2*>(red + WARPS * 8 * RED);
-  __shared__ long long s_scan[WARPS];
+  __shared__ int s_scan[WARPS];
+  __shared__ int s_most[WARPS];
   __shared__ int s_b;
-  __shared__ long long s_base;
-  __shared__ int s_last;
+  __shared__ int s_base;
+  __shared__ int s_last[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int vheads = p.kv_heads * p.row_blocks;
   pdl_wait();
@@ -144,21 +215,34 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
 
   // ---- this CTA's slice [start, end) of the line, and the sequence it starts in ----
   const int per = (p.B + THREADS - 1) / THREADS;
-  long long mine = 0;
-  for (int b = tid * per; b < min(p.B, (tid + 1) * per); ++b) {
-    const Seq s = seq_of(p, b);
-    mine += s.nb;
+  const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  int mine = 0;  // blocks of this thread's sequences; their number and the longest one ride along
+  int most = 0, some = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int nb = seq_of(p, b, 0).nb;
+    mine += nb;
+    most = max(most, nb);
+    some += nb > 0;
     if (blockIdx.x == 0 && __ldg(p.seq_lens + b) > (p.max_pages << p.pools.page_shift)) latch(p.err, MOE_ERR_BAD_IDS);
   }
-  long long incl = mine;
+  most = __reduce_max_sync(FULL, most);
+  if (lane == 0) s_most[warp] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) most = max(most, s_most[w]);
+  // Short sequences are not split: each counts as many blocks as the longest, and slices hold whole (sequence, head)s.
+  // The join of a split costs about as much as the blocks it would spread out.
+  const int pad = most <= SHORT ? most : 0;
+  if (pad) mine = some * pad;
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(FULL, incl, o);
+    const int v = __shfl_up_sync(FULL, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) s_scan[warp] = incl;
   __syncthreads();
-  long long total = 0, before = incl - mine;
+  int total = 0, before = incl - mine;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     if (w < warp) before += s_scan[w];
@@ -167,12 +251,14 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
   total *= vheads;
   before *= vheads;
   mine *= vheads;
-  const long long slice = max((total + gridDim.x - 1) / gridDim.x, (long long)MIN_SLICE);
-  const long long start = slice * blockIdx.x, end = min(total, start + slice);
+  int slice = max(total / (int)gridDim.x + (total % (int)gridDim.x ? 1 : 0), MIN_SLICE);
+  if (pad) slice = (slice + pad - 1) / pad * pad;
+  const bool slice_past = (int64_t)slice * blockIdx.x >= total;
+  const int start = slice_past ? total : slice * blockIdx.x, end = slice_past ? total : total - start > slice ? start + slice : total;
 
   // sequences without a token: zeros
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    if (seq_of(p, b).nb > 0) continue;
+    if (seq_of(p, b, 0).nb > 0) continue;
     for (int i = tid; i < p.heads * (D / 8); i += THREADS)
       reinterpret_cast<uint4*>(static_cast<T*>(p.y) + (int64_t)b * p.heads * D)[i] = make_uint4(0, 0, 0, 0);
     if (p.lse)
@@ -180,10 +266,10 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
   }
   if (start >= total) return;  // uniform over the CTA
   if (start >= before && start < before + mine) {
-    int b = tid * per;
-    long long base = before;
+    int b = b0;
+    int base = before;
     for (;; ++b) {
-      const long long n = (long long)seq_of(p, b).nb * vheads;
+      const int n = seq_of(p, b, pad).nb * vheads;
       if (start < base + n) break;
       base += n;
     }
@@ -192,32 +278,52 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
   }
   __syncthreads();
 
-  Cursor pre;  // the next block this warp loads
+  Cursor pre;  // the next block this warp looks up
   pre.b = s_b;
-  pre.s = seq_of(p, pre.b);
-  const long long rem = start - s_base;
-  pre.h = (int)(rem / pre.s.nb);
-  pre.j = (int)(rem % pre.s.nb);
+  pre.s = seq_of(p, pre.b, pad);
+  pre.h = (start - s_base) / pre.s.nb;
+  pre.j = (start - s_base) % pre.s.nb;
   Cursor cur = pre;  // the piece being computed (j: its first block in this slice)
-  long long pre_idx = start + warp;
-  advance(p, pre, warp, vheads);
-  int next_page = pre_idx < end ? page_of(p, pre) : 0;
+  int pre_idx = start + warp;
+  advance(p, pre, warp, vheads, pad);
 
   unsigned char* ring = smem + warp * S::STAGES * 2 * S::HALF;
   const uint32_t ring_a = smem_u32(ring);
-  int fill = 0;
-  // Loads the block at `pre` into ring stage `fill` (one cp.async group, empty past the slice's end) and moves
-  // `pre` on; the page of the block after it is fetched now, so its latency passes behind the loads.
+  int fill = 0, batch = 32;
+  int issued = start + warp;  // the block that the next load fetches
+  int64_t my_at = 0;  // lane i: where the warp's i-th block of the batch lies in the pools, and its rows [lo, hi)
+  int my_rows = 0;
+  // Loads the warp's next block into ring stage `fill` (one cp.async group, empty past the slice's end). The places of
+  // 32 blocks are looked up at once, one per lane, so that the page table's latency is paid once for them.
   auto load_next = [&]() {
-    if (pre_idx < end) {
-      const int page = next_page;
-      const bool page_ok = (unsigned)page < (unsigned)p.pools.num_pages;
-      if (!page_ok && lane == 0) latch(p.err, MOE_ERR_BAD_IDS);
-      const int tok = (pre.s.first + pre.j) * BLK;
-      const int lo = pre.s.lo - tok, hi = page_ok ? pre.s.len - tok : 0;  // rows lo <= r < hi are loaded
-      const int off = tok & ((1 << p.pools.page_shift) - 1);
-      const int64_t at = (int64_t)(page_ok ? page : 0) * p.pools.page_stride +
-                         ((((int64_t)(pre.h / p.row_blocks)) << p.pools.page_shift) + off) * D;
+    if (batch == 32) {
+      batch = 0;
+      my_rows = 0;
+      const int idx = pre_idx + lane * WARPS;
+      if (idx < end) {
+        Cursor c = pre;
+        advance(p, c, lane * WARPS, vheads, pad);
+        const int tok = (c.s.first + c.j) * BLK;
+        if (tok < c.s.len) {  // not a padding block
+          const int page = __ldg(p.page_table + (int64_t)c.b * p.max_pages + (tok >> p.pools.page_shift));
+          if ((unsigned)page < (unsigned)p.pools.num_pages) {
+            my_rows = max(0, c.s.lo - tok) | min(BLK, c.s.len - tok) << 16;
+            my_at = (int64_t)page * p.pools.page_stride +
+                    ((((int64_t)(c.h / p.row_blocks)) << p.pools.page_shift) + (tok & ((1 << p.pools.page_shift) - 1))) * D;
+          } else {
+            latch(p.err, MOE_ERR_BAD_IDS);  // its tokens read as zeros
+          }
+        }
+      }
+      __syncwarp();
+      pre_idx += 32 * WARPS;
+      if (pre_idx < end) advance(p, pre, 32 * WARPS, vheads, pad);
+    }
+    const int64_t at = __shfl_sync(FULL, my_at, batch);
+    const int rows = __shfl_sync(FULL, my_rows, batch);
+    ++batch;
+    if (issued < end) {
+      const int lo = rows & 0xffff, hi = rows >> 16;
       const T* ks = static_cast<const T*>(p.pools.k) + at;
       const T* vs = static_cast<const T*>(p.pools.v) + at;
       const uint32_t dst = ring_a + fill * 2 * S::HALF;
@@ -229,10 +335,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
         cp_async16(to, ks + r * D + c * 8, in);
         cp_async16(to + S::HALF, vs + r * D + c * 8, in);
       }
-      pre_idx += WARPS;
-      advance(p, pre, WARPS, vheads);
-      if (pre_idx < end) next_page = page_of(p, pre);
     }
+    issued += WARPS;
     asm volatile("cp.async.commit_group;" ::: "memory");
     fill = fill + 1 == S::STAGES ? 0 : fill + 1;
   };
@@ -240,11 +344,14 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
   for (int i = 0; i < S::STAGES - 1; ++i) load_next();
 
   const float c_log2 = p.scale * LOG2E;
+  const bool capped = p.softcap > 0.0f;
+  const float cap_in = capped ? 2.0f * c_log2 / p.softcap : 0.0f, cap_out = p.softcap * LOG2E;
   const int g8 = lane >> 2, t4 = lane & 3;
   int use = 0;
-  long long idx = start;  // first block of the piece
+  int idx = start;  // first block of the piece
+  Split ahead{}, behind{};  // the pieces shared with the CTAs before and behind this one
   while (idx < end) {
-    const long long piece_end = min(end, idx + (cur.s.nb - cur.j));
+    const int piece_end = end - idx > cur.s.nb - cur.j ? idx + (cur.s.nb - cur.j) : end;
     const int kvh = cur.h / p.row_blocks, row0 = (cur.h % p.row_blocks) * ROWS;
     const int live_rows = min(ROWS, p.group - row0);
     // q as the B operand: head n = g8, values 2 t4, +1 and + 8
@@ -272,7 +379,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
         for (int i = 0; i < 4; ++i) acc[dt][nt][i] = 0.0f;
     }
     // first block of this warp at or after idx
-    long long w_idx = idx + ((warp - (int)((idx - start) % WARPS) + WARPS) % WARPS);
+    int w_idx = idx + ((warp - (idx - start) % WARPS + WARPS) % WARPS);
     for (; w_idx < piece_end; w_idx += WARPS) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
       __syncwarp();
@@ -304,7 +411,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v = s[nt][i] + s2[nt][i];
-          v = p.softcap > 0.0f ? p.softcap * LOG2E * tanhf(v * p.scale / p.softcap) : v * c_log2;
+          // capped: tanh(x) = 1 - 2 / (e^2x + 1), absolute error about 1e-7 of the cap
+          v = capped ? cap_out - __fdividef(2.0f * cap_out, ex2(v * cap_in) + 1.0f) : v * c_log2;
           s[nt][i] = (i < 2 ? in0 : in1) ? v : -INFINITY;  // in units of log2
         }
         float corr[2];
@@ -352,9 +460,9 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
     }
 
     // ---- end of the piece: join the warps, 8 heads at a time ----
-    const long long u0 = idx - cur.j, u1 = u0 + cur.s.nb;  // the whole (sequence, head) on the line
-    const int c0 = (int)(u0 / slice), n_parts = (int)((u1 - 1) / slice) - c0 + 1;
-    const int my_slot = blockIdx.x * 2 + (blockIdx.x == c0 ? 1 : 0);
+    const int u0 = idx - cur.j;  // the whole (sequence, head) starts here on the line
+    const int c0 = u0 / slice, n_parts = (u0 + (cur.s.nb - 1)) / slice - c0 + 1;
+    const int my_slot = part_slot(c0, blockIdx.x - c0);
     const int64_t out_row = (int64_t)cur.b * p.heads + kvh * p.group + row0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -399,52 +507,54 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
       }
       __syncthreads();  // red is free again
     }
-    if (n_parts > 1) {
-      // the last of the piece's CTAs to arrive joins them
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        int32_t* cnt = p.counters + (int64_t)cur.b * vheads + cur.h;
-        s_last = atomicAdd(cnt, 1) == n_parts - 1;
-        if (s_last) *cnt = 0;  // ready for the next call
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        for (int e = tid; e < live_rows * (D / 4); e += THREADS) {
-          const int n = e / (D / 4), d = (e % (D / 4)) * 4;
-          float M = -INFINITY, L = 0.0f;
-          float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-          for (int k = 0; k < n_parts; ++k) {
-            const int64_t at = (int64_t)((c0 + k) * 2 + (k == 0 ? 1 : 0)) * ROWS + n;
-            const float2 ml = __ldcg(p.partial_ml + at);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
-            const float mn = fmaxf(M, ml.x);
-            const float ref = mn == -INFINITY ? 0.0f : mn;
-            const float f0 = ex2(M - ref), f1 = ex2(ml.x - ref);
-            M = mn;
-            L = L * f0 + ml.y * f1;
-            o.x = o.x * f0 + v.x * f1, o.y = o.y * f0 + v.y * f1;
-            o.z = o.z * f0 + v.z * f1, o.w = o.w * f0 + v.w * f1;
-          }
-          store_row<T, D>(p, out_row + n, d, o, M, L);
-        }
-      }
+    if (n_parts > 1) {  // at most two pieces of a slice: the one it begins in and the one it ends in
+      const Split sp = {n_parts, c0, cur.b * vheads + cur.h, out_row, live_rows};
+      if (blockIdx.x == c0) behind = sp;
+      else ahead = sp;
     }
-    const int step = (int)(piece_end - idx);
+    const int step = piece_end - idx;
     idx = piece_end;
-    if (idx < end) advance(p, cur, step, vheads);
+    if (idx < end) advance(p, cur, step, vheads, pad);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+  // ---- arrivals: the last CTA of a (sequence, head) joins its parts, or of a group of parts when there are many ----
+  if (ahead.parts == 0 && behind.parts == 0) return;
+  __threadfence();
+  __syncthreads();
+  if (lane == 0 && warp < 2) {
+    const Split& sp = warp ? behind : ahead;
+    s_last[warp] = sp.parts > 0 && arrive_first(p, sp, blockIdx.x - sp.c0);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    if (!s_last[i]) continue;  // uniform over the CTA
+    const Split sp = i ? behind : ahead;
+    __threadfence();
+    if (sp.parts <= ONE_JOIN) {
+      join<T, D, ROWS>(p, sp, 0, 1, sp.parts, p.partial_ml, nullptr);
+      continue;
+    }
+    const int g0 = (blockIdx.x - sp.c0) / JOIN * JOIN;
+    join<T, D, ROWS>(p, sp, g0, 1, min(JOIN, sp.parts - g0), p.partial_ml, p.group_ml);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_last[i] = arrive(p.counters + sp.unit, (sp.parts + JOIN - 1) / JOIN);
+    __syncthreads();
+    if (s_last[i]) {
+      __threadfence();
+      join<T, D, ROWS>(p, sp, 0, JOIN, (sp.parts + JOIN - 1) / JOIN, p.group_ml, nullptr);
+    }
+  }
 }
 
 // f(kernel, dynamic shared memory) for the handle's types and sizes.
 template <class F>
 static moe_status with_kernel(const moe_attn& a, F&& f) {
   const bool wide = decode_rows(a.group) == 16;
-  static_assert(decode_smem<128>() <= 233472 / CTAS_PER_SM - 1024 - 128 && decode_smem<64>() <= decode_smem<128>(),
-                "two CTAs per SM");
+  static_assert(decode_smem<128>() <= 233472 / CTAS_PER_SM - 1024 - 256 && decode_smem<64>() <= decode_smem<128>(),
+                "shared memory of an SM");
   auto by_type = [&](auto zero) -> moe_status {
     using T = decltype(zero);
     if (a.d.head_dim == 64)
@@ -465,6 +575,8 @@ moe_status launch_decode(const moe_attn& a, const DecodeParams& p, cudaStream_t 
   // no more CTAs than the widest table's blocks give work to
   const int64_t widest = ((int64_t)p.max_pages << p.pools.page_shift) / BLK;
   const int64_t bound = (widest * p.B * p.kv_heads * p.row_blocks + MIN_SLICE - 1) / MIN_SLICE;
+  if (widest * p.B * p.kv_heads * p.row_blocks > 0x3fffffffll)
+    return fail(MOE_ERR_INVALID, "moe_attn_decode: B * num_kv_heads * max_pages * page_size / 16 must be below 2^30");
   const int grid = (int)std::min<int64_t>(decode_max_ctas(a.sms), bound);
   return with_kernel(a, [&](auto kernel, int smem) -> moe_status {
     MOE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(THREADS), smem, st, p));

@@ -16,8 +16,8 @@ struct moe_attn {
   float scale;
   // decode workspace: see attention_decode.cu
   float* partial = nullptr;
-  float2* partial_ml = nullptr;
-  int32_t* counters = nullptr;
+  float2 *partial_ml = nullptr, *group_ml = nullptr;
+  int32_t *counters = nullptr, *group_counters = nullptr;  // one allocation
   int32_t* err = nullptr;
   int64_t bytes = 0;
   CUtensorMap k_map, v_map;  // prefill's page boxes
@@ -49,8 +49,8 @@ struct DecodeParams {
   void* y;
   float* lse;
   float* partial;
-  float2* partial_ml;
-  int32_t* counters;
+  float2 *partial_ml, *group_ml;
+  int32_t *counters, *group_counters;
   int32_t* err;
 };
 

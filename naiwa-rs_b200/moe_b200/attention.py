@@ -14,7 +14,7 @@ from dataclasses import dataclass
 
 from . import _lib
 from ._lib import AttnDesc, MoeError, check, lib
-from .layer import _stream, _torch
+from .layer import _torch
 
 _PAIRS = {"halves": _lib.ROPE_HALVES, "adjacent": _lib.ROPE_ADJACENT}
 
@@ -60,6 +60,16 @@ def page_slots(page_table, seqs, positions, page_size: int):
     """The cache slots ([T] int64) of tokens at `positions` of sequences `seqs` (CUDA int tensors), for append."""
     pos = positions.long()
     return page_table[seqs.long(), pos // page_size].long() * page_size + pos % page_size
+
+
+def _current_stream(device, stream):
+    """The raw handle of `stream`, or of the device's current stream (the direct lookup where torch has one: a
+    Stream object costs microseconds, a tenth of a small call)."""
+    if stream is not None:
+        return stream.cuda_stream
+    torch = _torch()
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return torch.cuda.current_stream(device).cuda_stream if raw is None else raw(device.index)
 
 
 def _invalid(msg: str):
@@ -145,7 +155,7 @@ class PagedAttention:
     def check(self, stream=None):
         """Raise MoeError when a previous call latched a device-side error (a slot, page, position or length out of
         range)."""
-        check(lib().moe_attn_check(self._h, _stream(stream)))
+        check(lib().moe_attn_check(self._h, _current_stream(self.device, stream)))
 
     # -- argument checks ---------------------------------------------------------------------------------
     def _rows(self, x, heads: int, what: str):
@@ -186,7 +196,7 @@ class PagedAttention:
             positions = self._ints(positions, (self.axes, T), "append: positions", torch.int32)
         slots = self._ints(slots, (T,), "append: slots", torch.int64)
         if out is None:
-            out = torch.empty((T, cfg.num_heads, cfg.head_dim), dtype=self._dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif self._rows(out, cfg.num_heads, "append: out") is not out or out.shape[0] != T:
             raise _invalid("append: out must be [T, num_heads, head_dim] with consecutive, 16-byte aligned heads")
         qt, qh, _ = q.stride()
@@ -195,14 +205,14 @@ class PagedAttention:
         ot, oh, _ = out.stride()
         check(self._append(self._h, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, T,
                            positions.data_ptr() if cfg.rope_dim else None, slots.data_ptr(), out.data_ptr(), ot, oh,
-                           _stream(stream)))
+                           _current_stream(self.device, stream)))
         return out
 
     def _outputs(self, q, out, lse, return_lse, what):
         torch = _torch()
         T, H, D = q.shape
         if out is None:
-            out = torch.empty((T, H, D), dtype=self._dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != self._dtype or out.device != self.device or \
                 not out.is_contiguous() or out.data_ptr() % 16:
             raise _invalid(f"{what}: out must be a contiguous, 16-byte aligned tensor of q's shape and type")
@@ -233,7 +243,7 @@ class PagedAttention:
         qt, qh, _ = q.stride()
         check(self._decode(self._h, q.data_ptr(), qt, qh, seq_lens.data_ptr(), page_table.data_ptr(),
                            page_table.shape[1], B, out.data_ptr(), None if lse is None else lse.data_ptr(),
-                           _stream(stream)))
+                           _current_stream(self.device, stream)))
         return out if lse is None else (out, lse)
 
     def prefill(self, q, cu_q, seq_lens, page_table, out=None, lse=None, return_lse=False, stream=None):
@@ -250,5 +260,5 @@ class PagedAttention:
         qt, qh, _ = q.stride()
         check(self._prefill(self._h, q.data_ptr(), qt, qh, cu_q.data_ptr(), seq_lens.data_ptr(),
                             page_table.data_ptr(), page_table.shape[1], B, q.shape[0], out.data_ptr(),
-                            None if lse is None else lse.data_ptr(), _stream(stream)))
+                            None if lse is None else lse.data_ptr(), _current_stream(self.device, stream)))
         return out if lse is None else (out, lse)
