@@ -299,11 +299,19 @@ extern "C" moe_status moe_attn_create(const moe_attn_desc* desc, moe_attn** out)
       a->group_ml = a->partial_ml + slots * rows;
       MOE_CUDA_TRY(cudaMalloc(&a->counters, cnt));
       a->group_counters = a->counters + units;
+      const size_t pf_acc = prefill_partial_bytes(*a), pf_ml = prefill_ml_bytes(*a);
+      const size_t pf_cnt = (prefill_counters(*a) + 2) * sizeof(int32_t);
+      MOE_CUDA_TRY(cudaMalloc(&a->pf_partial, pf_acc));
+      MOE_CUDA_TRY(cudaMalloc(&a->pf_ml, pf_ml));
+      MOE_CUDA_TRY(cudaMalloc(&a->pf_counters, pf_cnt));
+      MOE_CUDA_TRY(cudaMemset(a->pf_counters, 0, pf_cnt));
       MOE_CUDA_TRY(cudaMalloc(&a->err, sizeof(int32_t)));
       MOE_CUDA_TRY(cudaMemset(a->counters, 0, cnt));
+      a->counter_bytes = cnt;
+      a->pf_counter_bytes = pf_cnt;
       MOE_CUDA_TRY(cudaMemset(a->err, 0, sizeof(int32_t)));
       MOE_CUDA_TRY(cudaDeviceSynchronize());  // the zeros are in place for a first call on any stream
-      a->bytes = (int64_t)(acc + ml + cnt + sizeof(int32_t));
+      a->bytes = (int64_t)(acc + ml + cnt + pf_acc + pf_ml + pf_cnt + sizeof(int32_t));
       MOE_TRY(prepare_decode(*a));
       MOE_TRY(prepare_prefill(*a));
       for (int i = 0; i < 2; ++i)
@@ -327,6 +335,9 @@ extern "C" void moe_attn_destroy(moe_attn* a) {
   cudaFree(a->partial);
   cudaFree(a->partial_ml);
   cudaFree(a->counters);
+  cudaFree(a->pf_partial);
+  cudaFree(a->pf_ml);
+  cudaFree(a->pf_counters);
   cudaFree(a->err);
   delete a;
 }
@@ -416,6 +427,8 @@ extern "C" moe_status moe_attn_prefill(moe_attn* a, const void* q, int64_t q_tok
     p.num_pages = pools.num_pages, p.page_shift = pools.page_shift;
     p.scale = a->scale, p.softcap = a->d.softcap, p.window = a->d.window;
     p.y = y, p.lse = lse, p.err = a->err;
+    p.partial = a->pf_partial, p.partial_ml = a->pf_ml, p.counters = a->pf_counters;
+    p.work = a->pf_counters + prefill_counters(*a);
     DeviceGuard guard(a->d.device);
     return launch_prefill(*a, p, static_cast<cudaStream_t>(stream));
   });
@@ -431,6 +444,9 @@ extern "C" moe_status moe_attn_check(moe_attn* a, void* stream) {
     MOE_CUDA_TRY(cudaStreamSynchronize(st));
     if (!word) return MOE_OK;
     MOE_CUDA_TRY(cudaMemsetAsync(a->err, 0, sizeof(word), st));
+    // a call that gave up may have left its counters half way
+    MOE_CUDA_TRY(cudaMemsetAsync(a->counters, 0, a->counter_bytes, st));
+    MOE_CUDA_TRY(cudaMemsetAsync(a->pf_counters, 0, a->pf_counter_bytes, st));
     MOE_CUDA_TRY(cudaStreamSynchronize(st));
     return fail((moe_status)word, word == MOE_ERR_TIMEOUT ? "attention: a bounded device-side wait gave up"
                                                           : "attention: a slot, page, position or length out of range");

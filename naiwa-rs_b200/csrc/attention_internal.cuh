@@ -18,7 +18,12 @@ struct moe_attn {
   float* partial = nullptr;
   float2 *partial_ml = nullptr, *group_ml = nullptr;
   int32_t *counters = nullptr, *group_counters = nullptr;  // one allocation
+  // prefill workspace: see attention_prefill.cu
+  float4* pf_partial = nullptr;
+  float2* pf_ml = nullptr;
+  int32_t* pf_counters = nullptr;  // arrivals, then the two work words
   int32_t* err = nullptr;
+  size_t counter_bytes = 0, pf_counter_bytes = 0;
   int64_t bytes = 0;
   CUtensorMap k_map, v_map;  // prefill's page boxes
 };
@@ -66,6 +71,10 @@ struct PrefillParams {
   int window;
   void* y;
   float* lse;
+  float4* partial;     // pieces of items that are cut along the keys
+  float2* partial_ml;
+  int32_t* counters;   // arrivals per (item, tile, warp)
+  int32_t* work;       // [0] pieces taken, [1] CTAs that have left
   int32_t* err;
 };
 
@@ -77,6 +86,9 @@ int decode_max_ctas(int sms);
 // Per-device kernel attributes of the handle's variant; called with its device current.
 moe_status prepare_decode(const moe_attn& a);
 moe_status prepare_prefill(const moe_attn& a);
+size_t prefill_partial_bytes(const moe_attn& a);
+size_t prefill_ml_bytes(const moe_attn& a);
+size_t prefill_counters(const moe_attn& a);
 moe_status launch_decode(const moe_attn& a, const DecodeParams& p, cudaStream_t st);
 moe_status launch_prefill(const moe_attn& a, const PrefillParams& p, cudaStream_t st);
 // 4-D map over a pool: box of 64 values x min(page_size, 128) tokens of one head of one page, SWIZZLE_128B.

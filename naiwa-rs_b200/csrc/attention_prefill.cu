@@ -5,17 +5,20 @@
 //   y_i  = sum_j exp(x_ij - m_i) v_j / sum_j exp(x_ij - m_i),   lse_i = m_i + log sum_j exp(x_ij - m_i)
 //
 // A tile is 128 rows = (128 / group) tokens x the group's query heads, so the heads that share keys and
-// values share their loads. A CTA owns two tiles (256 rows, consecutive tokens of one sequence and one
-// key/value head) and walks the keys 128 at a time:
-//   * one warp loads K and V pages by TMA (64 values x a page's tokens per box, SWIZZLE_128B) into rings of
-//     STAGES tiles;
+// values share their loads. An item is two tiles (256 rows, consecutive tokens of one sequence and one key/value
+// head); its keys are walked 128 at a time (a step). Few items are each cut along the keys into equal pieces, whose
+// results are joined by the last to arrive, in the pieces' order. The kernel is persistent: one CTA per SM takes
+// pieces from a counter, those with the most keys first, and runs its roles over them without a break:
+//   * one warp takes the pieces, hands them to the other roles through a small ring, and loads K and V pages by TMA
+//     (64 values x a page's tokens per box, SWIZZLE_128B) into rings of STAGES tiles;
+//   * two warps load the next piece's Q while the last step of the piece before runs;
 //   * one thread issues S_i = Q_i K^T (128 x 128, f32 in tensor memory) and O_i += P_i V, alternating the
 //     two tiles, so the tensor cores work on one tile while the other's softmax runs;
 //   * four warps per tile hold one row per thread: maximum, exponentials and sum in f32, P rounded to the
-//     values' type and written over S in tensor memory, from where the second product reads it. O is
-//     rescaled only when a row's maximum grows by more than 2^RESCALE (rare after the first tiles), which leaves
-//     P below 2^RESCALE: sums stay exact enough in f32 and the quotient does not change.
-// Bound by the tensor cores and by the exponentials (16 per clock and SM against 128 x 128 per 1024 clocks of MMA).
+//     values' type (what the tensor cores take; the sum is of the unrounded weights) and written over S in tensor
+//     memory, from where the second product reads it. O is rescaled only when a row's maximum grows by more than
+//     2^RESCALE (rare after the first steps), which leaves P below 2^RESCALE: the quotient does not change.
+// Bound by the tensor cores (1024 clocks of MMA per 128 x 128 step) and as much by the exponentials (16 per clock and SM).
 //
 // Every wait is bounded: one that runs out sets MOE_ERR_TIMEOUT, the CTA stops issuing work, waits for its
 // own MMAs and copies, frees its tensor memory and returns.
@@ -34,7 +37,14 @@ constexpr int STAGES = 2;    // K tiles and V tiles in flight
 constexpr int SOFTMAX_WARPS = 4 * NQ;
 constexpr int MMA_WARP = SOFTMAX_WARPS;
 constexpr int LOAD_WARP = SOFTMAX_WARPS + 1;
-constexpr int PF_THREADS = (SOFTMAX_WARPS + 2) * 32;
+constexpr int Q_WARP = SOFTMAX_WARPS + 2;  // two of them
+constexpr int PF_THREADS = (SOFTMAX_WARPS + 4) * 32;
+// registers per thread: 168 at launch (384 threads), shared out anew: 2 x 216 + 72 = 3 x 168
+constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 72;
+constexpr int RING = 4;              // pieces handed out ahead
+constexpr int CONSUMERS = SOFTMAX_WARPS + 3;
+constexpr int MAX_CUT = 16;          // pieces of an item
+constexpr int PIECE_COST = 3;        // what a piece costs beside its steps, in steps (Q, epilogue, join)
 constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0;            // S_i / P_i at columns BN * i
 constexpr int O_COL = NQ * BN;      // O_i at columns O_COL + D * i
@@ -116,15 +126,38 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16u(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
+}
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 x, y, z;\n"
+      "mov.b64 x, {%2, %3};\n"
+      "mov.b64 y, {%4, %5};\n"
+      "mov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 x, x, y, z;\n"
+      "mov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y;\n"
+      "mov.b64 x, {%2, %3};\n"
+      "mov.b64 y, {%4, %5};\n"
+      "add.rn.f32x2 x, x, y;\n"
+      "mov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 template <int D>
@@ -136,8 +169,99 @@ struct PfShape {
 
 struct Bars {
   uint64_t k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES];
-  uint64_t s_full[NQ], p_full[NQ], o_full[NQ], drained;
+  uint64_t s_full[NQ], p_full[NQ], o_full[NQ], q_full, q_free, item_full[RING], item_free[RING], drained;
 };
+
+// A piece of work: steps [j0, j0 + steps) over the keys of one item. row0: the sequence's first row; past: the position
+// of that row; [t0, t1): the item's tokens. b < 0: no more work.
+struct Piece {
+  int b, kvh, row0, past, t0, t1, len, j0, steps, cut, k, item;
+};
+
+// The batch as the load warp sees it: each lane holds the tiles of its sequences and their prefix.
+struct Batch {
+  int per, before, mine, items, cut;
+};
+
+__device__ __forceinline__ int tokens_of(const PrefillParams& p, int b) {
+  return max(0, min(__ldg(p.cu_q + b + 1), p.T) - max(0, __ldg(p.cu_q + b)));
+}
+
+__device__ __forceinline__ Batch read_batch(const PrefillParams& p, int span, int lane, int ctas) {
+  Batch s;
+  s.per = (p.B + 31) / 32;
+  s.mine = 0;
+  int most = 0;  // steps of the longest item
+  for (int b = min(p.B, lane * s.per); b < min(p.B, (lane + 1) * s.per); ++b) {
+    const int n = tokens_of(p, b);
+    if (n == 0) continue;
+    s.mine += (n + span - 1) / span;
+    const int len = min(__ldg(p.seq_lens + b), p.max_pages << p.page_shift);
+    most = max(most, (p.window > 0 ? min(len, p.window + span + BN) : len) / BN + 1);
+  }
+  int incl = s.mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(FULL, incl, o);
+    if (lane >= o) incl += v;
+  }
+  s.before = incl - s.mine;
+  s.items = __shfl_sync(FULL, incl, 31) * p.kv_heads;
+  most = __reduce_max_sync(FULL, most);
+  // the cut that takes the fewest steps in the longest CTA, pieces taken in equal rounds
+  s.cut = 1;
+  if (s.items > 0) {
+    int best = 0x7fffffff;
+    const int cut = lane + 1;
+    if (cut <= MAX_CUT && (cut == 1 || (int64_t)s.items * cut <= 2 * ctas)) {
+      const int rounds = (s.items * cut + ctas - 1) / ctas;
+      best = rounds * ((most + cut - 1) / cut + PIECE_COST);
+    }
+    const int least = __reduce_min_sync(FULL, best);
+    s.cut = __ffs(__ballot_sync(FULL, best == least));  // the smallest such cut
+  }
+  return s;
+}
+
+// Piece number w of the launch (warp-collective): items by sequence, the last tokens (the most keys) first.
+__device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s, int w, int span, int lane) {
+  Piece q{};
+  q.b = -1;
+  if (w >= s.items * s.cut) return q;
+  q.cut = s.cut;
+  q.item = w / s.cut;
+  q.k = w % s.cut;
+  q.kvh = q.item % p.kv_heads;
+  const int u = s.items / p.kv_heads - 1 - q.item / p.kv_heads;
+  const bool here = u >= s.before && u < s.before + s.mine;
+  int b = 0, tile = 0;
+  if (here) {
+    int at = s.before;
+    for (b = lane * s.per;; ++b) {
+      const int n = (tokens_of(p, b) + span - 1) / span;
+      if (u < at + n) break;
+      at += n;
+    }
+    tile = u - at;
+  }
+  const int src = __ffs(__ballot_sync(FULL, here)) - 1;
+  q.b = __shfl_sync(FULL, b, src);
+  tile = __shfl_sync(FULL, tile, src);
+  q.row0 = max(0, __ldg(p.cu_q + q.b));
+  const int news = tokens_of(p, q.b), asked = __ldg(p.seq_lens + q.b);
+  q.len = max(0, min(asked, p.max_pages << p.page_shift));
+  q.past = q.len - news;  // negative: rows before position 0 see nothing
+  if (lane == 0 && (asked != q.len || q.past < 0)) latch(p.err, MOE_ERR_BAD_IDS);
+  q.t0 = tile * span;
+  q.t1 = min(news, q.t0 + span);
+  const int hi = max(0, q.past + q.t1);  // keys [lo, hi)
+  const int lo = p.window > 0 ? max(0, q.past + q.t0 - p.window + 1) : 0;
+  const int first = lo / BN, all = hi > lo ? (hi + BN - 1) / BN - first : 0;
+  const int a = (int)((int64_t)all * q.k / q.cut);
+  q.j0 = first + a;
+  q.steps = (int)((int64_t)all * (q.k + 1) / q.cut) - a;
+  return q;
+}
 
 template <class T, int D, bool CAP>
 __global__ void __launch_bounds__(PF_THREADS, 1)
@@ -149,48 +273,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   unsigned char* sK = sQ + NQ * S::TILE;
   unsigned char* sV = sK + STAGES * S::TILE;
   __shared__ Bars bars;
+  __shared__ Piece s_items[RING];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  __shared__ int s_scan[PF_THREADS / 32];
-  __shared__ int s_b, s_tile, s_k_issued, s_v_issued;
+  __shared__ int s_k_issued, s_v_issued;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort = &s_abort;
+  const int tq = BM / p.group, span = NQ * tq;  // tokens of a tile, of an item
 
-  pdl_wait();
-  pdl_trigger();
-  if (*reinterpret_cast<volatile int32_t*>(p.err) == (int32_t)MOE_ERR_TIMEOUT) return;
-
-  // ---- which sequence and which token tile: CTAs in order of sequence, the last tiles (the most keys) first ----
-  const int tq = BM / p.group, span = NQ * tq;  // tokens of a tile, of a CTA
-  const int kvh = blockIdx.x % p.kv_heads;
-  const int u = gridDim.x / p.kv_heads - 1 - blockIdx.x / p.kv_heads;
-  {
-    const int per = (p.B + PF_THREADS - 1) / PF_THREADS;
-    int mine = 0;
-    const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-    for (int b = b0; b < b1; ++b) mine += (max(0, __ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b)) + span - 1) / span;
-    int incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(FULL, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    if (tid == 0) s_b = -1;
-    __syncthreads();
-    int before = incl - mine;
-    for (int w = 0; w < warp; ++w) before += s_scan[w];
-    if (u >= before && u < before + mine) {
-      int b = b0, at = before;
-      for (;; ++b) {
-        const int n = (max(0, __ldg(p.cu_q + b + 1) - __ldg(p.cu_q + b)) + span - 1) / span;
-        if (u < at + n) break;
-        at += n;
-      }
-      s_b = b;
-      s_tile = u - at;
-    }
-  }
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&bars.k_full[i], 1);
@@ -203,38 +293,20 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       mbar_init(&bars.p_full[i], 4);
       mbar_init(&bars.o_full[i], 1);
     }
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&bars.item_full[i], 1);
+      mbar_init(&bars.item_free[i], CONSUMERS);
+    }
+    mbar_init(&bars.q_full, 2);
+    mbar_init(&bars.q_free, 1);
     mbar_init(&bars.drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = 0;
     s_k_issued = s_v_issued = 0;
   }
-  __syncthreads();
-  const int b = s_b;
-  if (b < 0) return;  // uniform over the CTA: no tile left
-  const int row0 = __ldg(p.cu_q + b), news = min(__ldg(p.cu_q + b + 1), p.T) - row0;
-  const int asked = __ldg(p.seq_lens + b);
-  const int len = max(0, min(asked, p.max_pages << p.page_shift));
-  const int past = len - news;  // position of the chunk's first row (negative: rows before position 0 see nothing)
-  if ((asked != len || past < 0 || row0 < 0) && tid == 0) latch(p.err, MOE_ERR_BAD_IDS);
-  if (row0 < 0) return;
-  const int t0 = s_tile * span;                         // first token of the CTA within the chunk
-  const int t1 = min(news, t0 + span);                  // one past its last
-  const int hi = max(0, past + t1);                     // keys [lo, hi)
-  const int lo = p.window > 0 ? max(0, past + t0 - p.window + 1) : 0;
-  const int j0 = lo / BN;
-  const int tiles = hi > lo ? (hi + BN - 1) / BN - j0 : 0;
-
-  // ---- Q into shared memory, swizzled as TMA would ----
-  for (int e = tid; e < NQ * BM * (D / 8); e += PF_THREADS) {
-    const int c = e % (D / 8), r = e / (D / 8), i = r / BM, rr = r % BM;
-    const int tok = t0 + i * tq + rr / p.group;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (rr < tq * p.group && tok < t1)
-      v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(row0 + tok) * p.q_token_stride +
-                                          (int64_t)(kvh * p.group + rr % p.group) * p.q_head_stride + c * 8);
-    *reinterpret_cast<uint4*>(sQ + i * S::TILE + (c / 8) * S::SLAB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = v;
-  }
-  proxy_fence();
+  pdl_wait();
+  pdl_trigger();
+  if (*reinterpret_cast<volatile int32_t*>(p.err) == (int32_t)MOE_ERR_TIMEOUT) return;
   if (warp == MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(TMEM_COLS));
@@ -245,240 +317,392 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   tc_after();
   const uint32_t tmem = s_tmem;
 
-  if (warp == LOAD_WARP) {
-    // ---------------- K and V tiles: each lane loads the boxes of its pages ----------------
-    const int box_rows = 1 << p.page_shift;
-    const int pages = BN >> p.page_shift;  // per tile
-    const int boxes = pages * (D / 64);    // at most 16
-    for (int j = 0; j < tiles; ++j) {
-      const int base = (j0 + j) * BN;
-      const int live = min(pages, (len - base + box_rows - 1) >> p.page_shift);  // pages that hold tokens
-      const int st = j % STAGES;
-      int page = 0;
-      const int my = lane % pages;  // this lane's page and 64-value half
-      const int half = lane / pages;
-      const bool on = lane < boxes && my < live;
-      if (on) page = __ldg(p.page_table + (int64_t)b * p.max_pages + (base >> p.page_shift) + my);
-      if (on && (unsigned)page >= (unsigned)p.num_pages) {
-        latch(p.err, MOE_ERR_BAD_IDS);
-        page = p.num_pages;  // out of the map: the box reads as zeros
-      }
+  // The n-th piece for a consuming warp; false once a wait gave up. Lane 0 releases the slot.
+  auto take = [&](int n, Piece* q) -> bool {
+    const int slot = n % RING;
+    const bool ok = __all_sync(FULL, mbar_wait(&bars.item_full[slot], (n / RING) & 1, abort));
+    if (!ok) return false;
+    *q = s_items[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.item_free[slot]);
+    return true;
+  };
+
+  if (warp >= SOFTMAX_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+    if (warp == LOAD_WARP) {
+      // ---------------- pieces, and their K and V tiles: each lane loads the boxes of its pages ----------------
+      const Batch batch = read_batch(p, span, lane, gridDim.x);
+      const int box_rows = 1 << p.page_shift;
+      const int pages = BN >> p.page_shift;  // per tile
+      const int my = lane % pages, half = lane / pages;  // this lane's page and 64-value half: at most 16 boxes
+      int g = 0, w = blockIdx.x;
       bool ok = true;
-      for (int kv = 0; kv < 2 && ok; ++kv) {
-        uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
-        uint64_t* free_ = kv ? &bars.v_free[st] : &bars.k_free[st];
-        ok = j < STAGES || mbar_wait(free_, ((j / STAGES) - 1) & 1, abort);
-        ok = __all_sync(FULL, ok);
+      for (int n = 0; ok; ++n) {
+        const Piece q = piece_of(p, batch, w, span, lane);
+        const int slot = n % RING;
+        ok = __all_sync(FULL, n < RING || mbar_wait(&bars.item_free[slot], ((n / RING) - 1) & 1, abort));
         if (!ok) break;
         if (lane == 0) {
-          mbar_expect_tx(full, (uint32_t)(live * box_rows * (D / 64) * 128));
-          if (kv) s_v_issued = j + 1;
-          else s_k_issued = j + 1;
+          s_items[slot] = q;
+          mbar_arrive(&bars.item_full[slot]);
+          if (q.b >= 0) w = gridDim.x + atomicAdd(p.work, 1);
         }
-        __syncwarp();
-        if (on)
-          tma_load_4d((kv ? sV : sK) + st * S::TILE + half * S::SLAB + my * box_rows * 128, kv ? &v_map : &k_map, half * 64,
-                      0, kvh, page, full);
-      }
-      if (!ok) {
-        if (lane == 0) s_abort = 1;
-        break;
-      }
-    }
-  } else if (warp == MMA_WARP) {
-    // ---------------- MMA issue (lane 0); the whole warp clears values past the length ----------------
-    const uint64_t qd = sw128_desc(smem_u32(sQ), 16), kd = sw128_desc(smem_u32(sK), 16);
-    const uint64_t vd = sw128_desc(smem_u32(sV), S::SLAB);
-    const uint32_t id_s = idesc<T>(BN, false), id_o = idesc<T>(D, true);
-    auto qk = [&](int i, int st) {
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const uint32_t off = (uint32_t)((k >> 2) * S::SLAB + (k & 3) * 32);
-        umma_ss(tmem + S_COL + i * BN, qd + ((i * S::TILE + off) >> 4), kd + ((st * S::TILE + off) >> 4), id_s, k > 0);
-      }
-      commit(&bars.s_full[i]);
-    };
-    bool ok = true;
-    for (int j = -1; j < tiles && ok && tiles > 0; ++j) {
-      const int sv = j % STAGES, sk = (j + 1) % STAGES;
-      const bool more = j + 1 < tiles;
-      if (more) ok = mbar_wait(&bars.k_full[sk], ((j + 1) / STAGES) & 1, abort);
-      if (j >= 0) {
-        ok = ok && mbar_wait(&bars.v_full[sv], (j / STAGES) & 1, abort);
-        ok = __all_sync(FULL, ok);
-        if (!ok) break;
-        // values past the sequence's length (the rest of its last page, pages not loaded) may be anything, and
-        // 0 * NaN is NaN: clear them
-        const int valid = len - (j0 + j) * BN;
-        if (valid < BN) {
-          for (int e = lane; e < (BN - valid) * (D / 8); e += 32) {
-            const int r = valid + e / (D / 8), c = e % (D / 8);
-            *reinterpret_cast<uint4*>(sV + sv * S::TILE + (c / 8) * S::SLAB + r * 128 + ((c & 7) << 4)) =
-                make_uint4(0, 0, 0, 0);
+        if (q.b < 0) break;
+        w = __shfl_sync(FULL, w, 0);
+        for (int j = 0; j < q.steps && ok; ++j, ++g) {
+          const int base = (q.j0 + j) * BN;
+          const int live = min(pages, (q.len - base + box_rows - 1) >> p.page_shift);  // pages that hold tokens
+          const int st = g % STAGES;
+          const bool on = half < D / 64 && my < live;
+          int page = 0;
+          if (on) page = __ldg(p.page_table + (int64_t)q.b * p.max_pages + (base >> p.page_shift) + my);
+          if (on && (unsigned)page >= (unsigned)p.num_pages) {
+            latch(p.err, MOE_ERR_BAD_IDS);
+            page = p.num_pages;  // out of the map: the box reads as zeros
           }
-          proxy_fence();
+          for (int kv = 0; kv < 2; ++kv) {
+            uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
+            uint64_t* free_ = kv ? &bars.v_free[st] : &bars.k_free[st];
+            ok = __all_sync(FULL, g < STAGES || mbar_wait(free_, ((g / STAGES) - 1) & 1, abort));
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_expect_tx(full, (uint32_t)(live * box_rows * (D / 64) * 128));
+              if (kv) s_v_issued = g + 1;
+              else s_k_issued = g + 1;
+            }
+            __syncwarp();
+            if (on)
+              tma_load_4d((kv ? sV : sK) + st * S::TILE + half * S::SLAB + my * box_rows * 128, kv ? &v_map : &k_map,
+                          half * 64, 0, q.kvh, page, full);
+          }
         }
-        __syncwarp();
       }
-      ok = __all_sync(FULL, ok);
-      if (!ok) break;
-      for (int i = 0; i < NQ; ++i) {
-        if (j >= 0) {
-          ok = mbar_wait(&bars.p_full[i], j & 1, abort);
+      if (!ok && lane == 0) s_abort = 1;
+      // the commits that released the last stages have landed before the CTA ends
+      for (int c = max(0, g - STAGES); c < g && ok; ++c)
+        ok = mbar_wait(&bars.k_free[c % STAGES], (c / STAGES) & 1, abort) &&
+             mbar_wait(&bars.v_free[c % STAGES], (c / STAGES) & 1, abort);
+      if (!ok && lane == 0) s_abort = 1;
+      __syncwarp();
+    } else if (warp >= Q_WARP) {
+      // ---------------- Q into shared memory, swizzled as TMA would ----------------
+      bool ok = true;
+      int used = 0;  // pieces with steps so far
+      for (int n = 0; ok; ++n) {
+        Piece q;
+        ok = take(n, &q);
+        if (!ok || q.b < 0) break;
+        if (q.steps == 0) continue;
+        ok = __all_sync(FULL, used == 0 || mbar_wait(&bars.q_free, (used - 1) & 1, abort));
+        if (!ok) break;
+        ++used;
+        constexpr int CH = D / 8;
+        const int me = (warp - Q_WARP) * 32 + lane;
+        const int c = me % CH;
+        for (int r = me / CH; r < NQ * BM; r += 64 / CH) {
+          const int i = r / BM, rr = r % BM, tok = q.t0 + i * tq + rr / p.group;
+          const bool in = rr < tq * p.group && tok < q.t1;
+          const T* src = static_cast<const T*>(p.q) +
+                         (in ? (int64_t)(q.row0 + tok) * p.q_token_stride +
+                                   (int64_t)(q.kvh * p.group + rr % p.group) * p.q_head_stride + c * 8
+                             : 0);
+          const uint32_t dst =
+              smem_u32(sQ + i * S::TILE + (c / 8) * S::SLAB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        proxy_fence();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_full);
+      }
+      // the last piece's release has landed
+      if (ok && used > 0) ok = mbar_wait(&bars.q_free, (used - 1) & 1, abort);
+      if (!ok && lane == 0) s_abort = 1;
+      __syncwarp();
+    } else {
+      // ---------------- MMA issue (lane 0); the whole warp clears values past the length ----------------
+      const uint64_t qd = sw128_desc(smem_u32(sQ), 16), kd = sw128_desc(smem_u32(sK), 16);
+      const uint64_t vd = sw128_desc(smem_u32(sV), S::SLAB);
+      const uint32_t id_s = idesc<T>(BN, false), id_o = idesc<T>(D, true);
+      bool ok = true;
+      int g = 0, used = 0, done[NQ] = {0, 0};
+      for (int n = 0; ok; ++n) {
+        Piece q;
+        ok = take(n, &q);
+        if (!ok || q.b < 0) break;
+        if (q.steps == 0) continue;
+        ok = __all_sync(FULL, mbar_wait(&bars.q_full, used & 1, abort));
+        if (!ok) break;
+        ++used;
+        tc_after();
+        const int tiles = q.t0 + tq < q.t1 ? 2 : 1;  // tiles with rows
+        for (int j = -1; j < q.steps && ok; ++j) {
+          // step j of this piece is the CTA's step g + j
+          const int sv = (g + j + STAGES) % STAGES, sk = (g + j + 1) % STAGES;
+          const bool more = j + 1 < q.steps;
+          if (more) ok = mbar_wait(&bars.k_full[sk], ((g + j + 1) / STAGES) & 1, abort);
+          if (j >= 0) {
+            ok = ok && mbar_wait(&bars.v_full[sv], ((g + j) / STAGES) & 1, abort);
+            // values past the sequence's length (the rest of its last page, pages not loaded) may be anything, and
+            // 0 * NaN is NaN: clear them
+            const int valid = q.len - (q.j0 + j) * BN;
+            if (valid < BN && __all_sync(FULL, ok)) {
+              for (int e = lane; e < (BN - valid) * (D / 8); e += 32) {
+                const int r = valid + e / (D / 8), c = e % (D / 8);
+                *reinterpret_cast<uint4*>(sV + sv * S::TILE + (c / 8) * S::SLAB + r * 128 + ((c & 7) << 4)) =
+                    make_uint4(0, 0, 0, 0);
+              }
+              proxy_fence();
+            }
+            __syncwarp();
+          }
           ok = __all_sync(FULL, ok);
           if (!ok) break;
-          tc_after();
-          if (lane == 0) {
 #pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
-              umma_ts(tmem + O_COL + i * D, tmem + S_COL + i * BN + k * 8, vd + ((sv * S::TILE + k * 2048) >> 4), id_o,
-                      j > 0 || k > 0);
-            commit(&bars.o_full[i]);
-            if (i == NQ - 1 && j + STAGES < tiles) commit(&bars.v_free[sv]);
+          for (int i = 0; i < NQ; ++i) {
+            if (i >= tiles) break;
+            if (j >= 0) {
+              ok = __all_sync(FULL, mbar_wait(&bars.p_full[i], done[i] & 1, abort));
+              if (!ok) break;
+              ++done[i];
+              tc_after();
+              if (lane == 0) {
+#pragma unroll
+                for (int k = 0; k < BN / 16; ++k)
+                  umma_ts(tmem + O_COL + i * D, tmem + S_COL + i * BN + k * 8, vd + ((sv * S::TILE + k * 2048) >> 4), id_o,
+                          j > 0 || k > 0);
+                commit(&bars.o_full[i]);
+                if (i == tiles - 1) commit(&bars.v_free[sv]);
+              }
+            }
+            // S_i of the next keys: issued behind the product that reads P_i from the same columns
+            if (more && lane == 0) {
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (uint32_t)((k >> 2) * S::SLAB + (k & 3) * 32);
+                umma_ss(tmem + S_COL + i * BN, qd + ((i * S::TILE + off) >> 4), kd + ((sk * S::TILE + off) >> 4), id_s,
+                        k > 0);
+              }
+              commit(&bars.s_full[i]);
+              if (i == tiles - 1) {
+                commit(&bars.k_free[sk]);
+                if (j + 2 == q.steps) commit(&bars.q_free);
+              }
+            }
+            __syncwarp();
           }
         }
-        // S_i of the next keys: issued behind the product that reads P_i from the same columns
-        if (more && lane == 0) {
-          qk(i, sk);
-          if (i == NQ - 1 && j + 1 + STAGES < tiles) commit(&bars.k_free[sk]);
+        g += q.steps;
+      }
+      if (!ok) {
+        if (lane == 0) {
+          s_abort = 1;
+          commit(&bars.drained);  // every MMA issued so far lands before the CTA goes on
+          (void)mbar_wait(&bars.drained, 0, nullptr);
         }
         __syncwarp();
       }
-    }
-    if (!ok) {
-      if (lane == 0) {
-        s_abort = 1;
-        commit(&bars.drained);  // every MMA issued so far lands before the CTA goes on
-        (void)mbar_wait(&bars.drained, 0, nullptr);
-      }
-      __syncwarp();
     }
   } else {
     // ---------------- softmax: one row per thread ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
     const int i = warp >> 2, quad = warp & 3;
     const int rr = quad * 32 + lane;
-    const int first = t0 + i * tq;  // first token of the tile
-    const int tok = first + rr / p.group;
-    const bool live = rr < tq * p.group && tok < t1;
-    const int pos = past + tok;  // this row sees keys (pos - window, pos]
-    const int key_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+    const int my_tok = i * tq + rr / p.group, my_head = rr % p.group;
+    const bool my_row = rr < tq * p.group;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t s_at = lane_base + S_COL + i * BN, o_at = lane_base + O_COL + i * D;
-    const float c_log2 = p.scale * LOG2E;
-    float m = -INFINITY, l = 0.0f;  // reference in units of log2, sum of weights
+    const float c_log2 = CAP ? 1.0f : p.scale * LOG2E;
+    const float cap_in = CAP ? 2.0f * LOG2E * p.scale / p.softcap : 0.0f, cap_out = p.softcap * LOG2E;
     bool ok = true;
-    for (int j = 0; j < tiles; ++j) {
-      ok = mbar_wait(&bars.s_full[i], j & 1, abort);
-      // the product with the previous tile's P has been issued before this S, and finished: its phase is taken
-      // note of here, and O may be rescaled
-      if (ok && j > 0) ok = mbar_wait(&bars.o_full[i], (j - 1) & 1, abort);
-      ok = __all_sync(FULL, ok);
-      if (!ok) break;
-      tc_after();
-      const int base = (j0 + j) * BN;
-      // keys that every live row of the tile sees need no mask
-      const bool full = base + BN - 1 <= past + first &&
-                        (p.window <= 0 || base > past + min(t1, first + tq) - 1 - p.window);
-      const int from = full ? 0 : key_lo - base, to = full ? BN : pos + 1 - base;  // columns [from, to)
-      auto score = [&](uint32_t raw, int col) {
-        float x = __uint_as_float(raw);
-        if (CAP) {
-          // softcap * tanh(x): 1 - 2 / (e^2x + 1), absolute error about 1e-7 of the cap
-          const float e = ex2(x * (2.0f * LOG2E * p.scale / p.softcap));
-          x = p.softcap * LOG2E * (1.0f - __fdividef(2.0f, e + 1.0f));
-        } else {
-          x *= c_log2;
-        }
-        return (col >= from && col < to) ? x : -INFINITY;
-      };
-      uint32_t r[32];
-      float mx = -INFINITY;
+    int seen = 0;  // steps so far
+    for (int n = 0; ok; ++n) {
+      Piece q;
+      ok = take(n, &q);
+      if (!ok || q.b < 0) break;
+      const int first = q.t0 + i * tq;  // first token of the tile
+      if (first >= q.t1) continue;      // no rows in this tile
+      const int tok = q.t0 + my_tok;
+      const bool live = my_row && tok < q.t1;
+      const int pos = q.past + tok;  // this row sees keys (pos - window, pos]
+      const int key_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+      float m = -INFINITY, l = 0.0f;  // reference in units of log2, sum of weights
+      for (int j = 0; j < q.steps; ++j, ++seen) {
+        ok = mbar_wait(&bars.s_full[i], seen & 1, abort);
+        // the product with the previous step's P has been issued before this S, and finished: its phase is taken
+        // note of here, and O may be rescaled
+        if (ok && j > 0) ok = mbar_wait(&bars.o_full[i], (seen - 1) & 1, abort);
+        ok = __all_sync(FULL, ok);
+        if (!ok) break;
+        tc_after();
+        uint32_t r[BN];
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c) {
-        tmem_ld32(s_at + c * 32, r);
+        for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
         tmem_wait_ld();
+        if (CAP) {
+          // softcap * tanh(x) = softcap * (1 - 2 / (e^2x + 1)), absolute error about 1e-7 of the cap
 #pragma unroll
-        for (int k = 0; k < 32; ++k) mx = fmaxf(mx, score(r[k], c * 32 + k));
-      }
-      const bool grow = mx > m + RESCALE;  // also the first finite maximum
-      if (__any_sync(FULL, grow)) {
-        const float mn = grow ? mx : m;
-        const float f = grow ? ex2(m - mn) : 1.0f;
-        m = mn;
-        l *= f;
-        if (j > 0) {
+          for (int k = 0; k < BN; ++k)
+            r[k] = __float_as_uint(cap_out - __fdividef(2.0f * cap_out, ex2(__uint_as_float(r[k]) * cap_in) + 1.0f));
+        }
+        const int base = (q.j0 + j) * BN;
+        // keys that every live row of the tile sees need no mask
+        if (base + BN - 1 > q.past + first || (p.window > 0 && base <= q.past + min(q.t1, first + tq) - 1 - p.window)) {
+          const int from = key_lo - base;
+          const unsigned width = (unsigned)max(0, pos + 1 - key_lo);  // columns [from, from + width)
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            tmem_ld32(o_at + c * 32, r);
-            tmem_wait_ld();
+          for (int k = 0; k < BN; ++k)
+            if ((unsigned)(k - from) >= width) r[k] = 0xff800000u;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * f);
-            tmem_st32(o_at + c * 32, r);
+        for (int k = 0; k < BN; k += 8)
+#pragma unroll
+          for (int a = 0; a < 4; ++a)
+            mx[a] = fmaxf(fmaxf(mx[a], __uint_as_float(r[k + 2 * a])), __uint_as_float(r[k + 2 * a + 1]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c_log2;  // scale > 0
+        const bool grow = top > m + RESCALE;  // also the first finite maximum
+        if (__any_sync(FULL, grow)) {
+          const float mn = grow ? top : m;
+          const float f = grow ? ex2(m - mn) : 1.0f;
+          m = mn;
+          l *= f;
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16u(o_at + c * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st16(o_at + c * 16, o);
+            }
           }
         }
-      }
-      const float ref = m == -INFINITY ? 0.0f : m;
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c) {
-        tmem_ld32(s_at + c * 32, r);
-        tmem_wait_ld();
-        uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float a = ex2(score(r[2 * k], c * 32 + 2 * k) - ref);
-          const float e = ex2(score(r[2 * k + 1], c * 32 + 2 * k + 1) - ref);
-          l += a + e;
-          w[k] = Elem<T>::pack(a, e);
-        }
-        tmem_st16(s_at + c * 16, w);  // columns of S that this row has already read
-      }
-      tmem_wait_st();
-      tc_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.p_full[i]);
-    }
-    if (ok && tiles > 0) {
-      ok = mbar_wait(&bars.o_full[i], (tiles - 1) & 1, abort);
-      ok = __all_sync(FULL, ok);
-    }
-    if (!ok) {
-      if (lane == 0) s_abort = 1;
-    } else {
-      tc_after();
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int64_t row = (int64_t)(row0 + tok) * p.heads + kvh * p.group + rr % p.group;
-      T* dst = static_cast<T*>(p.y) + row * D;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t r[32];
-        if (tiles > 0) {
-          tmem_ld32(o_at + c * 32, r);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) r[k] = 0;
-        }
-        if (live) {
+        for (int c = 0; c < BN / 32; ++c) {
           uint32_t w[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k)  // a row that saw nothing gives zeros
-            w[k] = l == 0.0f ? 0u
-                             : Elem<T>::pack(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv);
+          for (int k = 0; k < 16; ++k) {
+            float2 x = fma2(make_float2(__uint_as_float(r[c * 32 + 2 * k]), __uint_as_float(r[c * 32 + 2 * k + 1])),
+                            make_float2(c_log2, c_log2), make_float2(-ref, -ref));
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            sum = add2(sum, x);
+            w[k] = Elem<T>::pack(x.x, x.y);
+          }
+          tmem_st16(s_at + c * 16, w);  // columns of S, all of which this row has read
+        }
+        l += sum.x + sum.y;
+        tmem_wait_st();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_full[i]);
+      }
+      if (ok && q.steps > 0) ok = __all_sync(FULL, mbar_wait(&bars.o_full[i], (seen - 1) & 1, abort));
+      if (!ok) break;
+      tc_after();
+      // ---- the piece's rows: out, or into the workspace ----
+      const int64_t row = (int64_t)(q.row0 + tok) * p.heads + q.kvh * p.group + my_head;
+      T* dst = static_cast<T*>(p.y) + row * D;
+      float4* part = p.partial + ((int64_t)(q.item * q.cut + q.k) * NQ + i) * (D / 4) * BM + rr;  // [D / 4][BM]
+      const float inv = q.cut > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t o[16];
+        if (q.steps > 0) {
+          tmem_ld16u(o_at + c * 16, o);
+          tmem_wait_ld();
+        }
+        float f[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) f[k] = l == 0.0f ? 0.0f : __uint_as_float(o[k]) * inv;  // nothing seen: zeros
+        if (q.cut > 1) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            *reinterpret_cast<uint4*>(dst + c * 32 + k * 8) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+            __stcg(part + (c * 4 + k) * BM, make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]));
+        } else if (live) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<uint4*>(dst + c * 16 + k * 8) =
+                make_uint4(Elem<T>::pack(f[8 * k], f[8 * k + 1]), Elem<T>::pack(f[8 * k + 2], f[8 * k + 3]),
+                           Elem<T>::pack(f[8 * k + 4], f[8 * k + 5]), Elem<T>::pack(f[8 * k + 6], f[8 * k + 7]));
         }
       }
-      if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
+      if (q.cut == 1) {
+        if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
+        continue;
+      }
+      // ---- the last of the item's pieces to arrive joins them in order, each warp its own rows ----
+      float2* ml = p.partial_ml + ((int64_t)q.item * q.cut * NQ + i) * BM + rr;  // piece k at k * NQ * BM
+      __stcg(ml + q.k * NQ * BM, make_float2(m, l));
+      __threadfence();
+      __syncwarp();
+      int last = 0;
+      if (lane == 0) {
+        int32_t* cnt = p.counters + (q.item * NQ + i) * 4 + quad;
+        last = atomicAdd(cnt, 1) == q.cut - 1;
+        if (last) *cnt = 0;  // ready for the next call
+      }
+      if (__shfl_sync(FULL, last, 0)) {
+        __threadfence();
+        float M = -INFINITY, L = 0.0f, f[MAX_CUT];
+#pragma unroll
+        for (int k = 0; k < MAX_CUT; ++k) {
+          f[k] = -INFINITY;
+          if (k < q.cut) f[k] = __ldcg(ml + k * NQ * BM).x;
+          M = fmaxf(M, f[k]);
+        }
+        const float at = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int k = 0; k < MAX_CUT; ++k) {
+          f[k] = ex2(f[k] - at);
+          if (k < q.cut) L += __ldcg(ml + k * NQ * BM).y * f[k];
+        }
+        const float il = L == 0.0f ? 0.0f : 1.0f / L;
+        const float4* src = p.partial + ((int64_t)q.item * q.cut * NQ + i) * (D / 4) * BM + rr;
+#pragma unroll 1
+        for (int c = 0; c < D / 8; ++c) {
+          float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+#pragma unroll
+          for (int k = 0; k < MAX_CUT; ++k) {
+            if (k < q.cut) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float4 v = __ldcg(src + ((int64_t)k * NQ * (D / 4) + c * 2 + h) * BM);
+                o[h].x = fmaf(v.x, f[k], o[h].x), o[h].y = fmaf(v.y, f[k], o[h].y);
+                o[h].z = fmaf(v.z, f[k], o[h].z), o[h].w = fmaf(v.w, f[k], o[h].w);
+              }
+            }
+          }
+          if (live)
+            *reinterpret_cast<uint4*>(dst + c * 8) =
+                make_uint4(Elem<T>::pack(o[0].x * il, o[0].y * il), Elem<T>::pack(o[0].z * il, o[0].w * il),
+                           Elem<T>::pack(o[1].x * il, o[1].y * il), Elem<T>::pack(o[1].z * il, o[1].w * il));
+        }
+        if (live && p.lse) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
+      }
     }
+    if (!ok && lane == 0) s_abort = 1;
   }
   __syncthreads();
-  if (s_abort && tid == 0) {  // the copies still in flight land before the CTA's shared memory goes
-    for (int j = max(0, s_k_issued - STAGES); j < s_k_issued; ++j)
-      (void)mbar_wait(&bars.k_full[j % STAGES], (j / STAGES) & 1, nullptr);
-    for (int j = max(0, s_v_issued - STAGES); j < s_v_issued; ++j)
-      (void)mbar_wait(&bars.v_full[j % STAGES], (j / STAGES) & 1, nullptr);
-    atomicExch(p.err, (int)MOE_ERR_TIMEOUT);
+  if (tid == 0) {
+    if (s_abort) {  // the copies still in flight land before the CTA's shared memory goes
+      for (int j = max(0, s_k_issued - STAGES); j < s_k_issued; ++j)
+        (void)mbar_wait(&bars.k_full[j % STAGES], (j / STAGES) & 1, nullptr);
+      for (int j = max(0, s_v_issued - STAGES); j < s_v_issued; ++j)
+        (void)mbar_wait(&bars.v_full[j % STAGES], (j / STAGES) & 1, nullptr);
+      atomicExch(p.err, (int)MOE_ERR_TIMEOUT);
+    }
+    // the last CTA to leave puts the counter of pieces back for the next call
+    __threadfence();
+    if (atomicAdd(p.work + 1, 1) == (int)gridDim.x - 1) {
+      p.work[0] = 0;
+      p.work[1] = 0;
+    }
   }
   tc_before();
   __syncthreads();
@@ -509,14 +733,19 @@ moe_status prepare_prefill(const moe_attn& a) {
 
 moe_status launch_prefill(const moe_attn& a, const PrefillParams& p, cudaStream_t st) {
   const int span = NQ * (BM / p.group);
-  // every sequence wastes less than one tile: CTAs past the last tile leave at once
-  const int64_t grid = ((int64_t)p.T / span + std::min(p.B, p.T)) * p.kv_heads;
-  if (grid > 0x7fffffffll) return fail(MOE_ERR_INVALID, "moe_attn_prefill: too many rows");
+  // every sequence wastes less than one item
+  const int64_t items = ((int64_t)p.T / span + std::min(p.B, p.T)) * p.kv_heads;
+  if (items > 0x3fffffff) return fail(MOE_ERR_INVALID, "moe_attn_prefill: too many rows");
+  const int grid = (int)std::min<int64_t>(a.sms, items * MAX_CUT);
   return with_kernel(a, [&](auto kernel, int smem) -> moe_status {
-    MOE_CUDA_TRY(launch_pdl(kernel, dim3((unsigned)grid), dim3(PF_THREADS), smem, st, p, a.k_map, a.v_map));
+    MOE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(PF_THREADS), smem, st, p, a.k_map, a.v_map));
     return MOE_OK;
   });
 }
+
+size_t prefill_partial_bytes(const moe_attn& a) { return (size_t)2 * a.sms * NQ * BM * a.d.head_dim * sizeof(float); }
+size_t prefill_ml_bytes(const moe_attn& a) { return (size_t)2 * a.sms * NQ * BM * sizeof(float2); }
+size_t prefill_counters(const moe_attn& a) { return (size_t)2 * a.sms * NQ * 4; }
 
 moe_status make_page_tmap(CUtensorMap* map, int dtype, const void* pool, int head_dim, int page_size, int kv_heads,
                           int64_t num_pages, int64_t page_stride) {
