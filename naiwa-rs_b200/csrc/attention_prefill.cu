@@ -48,6 +48,9 @@ constexpr int PIECE_COST = 3;        // what a piece costs beside its steps, in 
 constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0;            // S_i / P_i at columns BN * i
 constexpr int O_COL = NQ * BN;      // O_i at columns O_COL + D * i
+#ifndef POLY
+#define POLY 0
+#endif
 constexpr float RESCALE = 8.0f;     // log2 of how far a row's reference may lag behind its maximum
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
@@ -63,6 +66,51 @@ __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::befor
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{.reg .b64 x, y, z;\n"
+      "mov.b64 x, {%2, %3};\n"
+      "mov.b64 y, {%4, %5};\n"
+      "mov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 x, x, y, z;\n"
+      "mov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{.reg .b64 x, y;\n"
+      "mov.b64 x, {%2, %3};\n"
+      "mov.b64 y, {%4, %5};\n"
+      "add.rn.f32x2 x, x, y;\n"
+      "mov.b64 {%0, %1}, x;}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+// 2^x of two values by arithmetic alone: x = n + f with |f| <= 1/2 (adding and taking away 1.5 * 2^23 rounds to n), a
+// degree-5 polynomial of 2^f (coefficients fitted to equal relative error over the interval, 2.3e-7 in f32), n added
+// to the exponent. Inputs below -126 give 2^-126.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  const float magic = 12582912.0f;
+  x.x = fmaxf(x.x, -126.0f);
+  x.y = fmaxf(x.y, -126.0f);
+  const float2 t = add2(x, make_float2(magic, magic));
+  const float2 n = add2(t, make_float2(-magic, -magic));
+  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+  auto c = [](float v) { return make_float2(v, v); };
+  float2 r = fma2(f, c(0x1.5c08e6p-10f), c(0x1.3d0c52p-7f));
+  r = fma2(r, f, c(0x1.c6b6e4p-5f));
+  r = fma2(r, f, c(0x1.ebf918p-3f));
+  r = fma2(r, f, c(0x1.62e428p-1f));
+  r = fma2(r, f, c(0x1.000002p+0f));
+  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
+}
+
 // SWIZZLE_128B shared-memory matrix descriptor, slabs of 64 values x n rows of 128 bytes, 8-row groups 1024 bytes
 // apart. Q and K: K-major (the leading offset is not used). V: MN-major, the next 64 output columns lie
 // `leading` bytes on.
@@ -73,34 +121,47 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t leading) 
 
 // kind::f16 instruction descriptor: f32 accumulator, A and B both bf16 or both f16, M = 128, N = n.
 template <class T>
-__device__ __forceinline__ uint32_t idesc(int n, bool b_mn_major) {
+__device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn_major) {
   const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(BM >> 4) << 24);
 }
 
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+// The MMA warp issues converged, with one lane's predicate on each instruction: operands that the compiler can prove
+// uniform stay in uniform registers. (Inside an `if (lane == 0)` every operand was moved there one by one: 105 clocks per
+// instruction against 65 of execution.)
+__device__ __forceinline__ void umma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                        uint32_t accumulate) {
   asm volatile(
-      "{.reg .pred p;\n"
+      "{.reg .pred p, e;\n"
+      "setp.ne.b32 e, %5, 0;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(accumulate)
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(lead)
       : "memory");
 }
 
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+                                        uint32_t accumulate) {
   asm volatile(
-      "{.reg .pred p;\n"
+      "{.reg .pred p, e;\n"
+      "setp.ne.b32 e, %5, 0;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(accumulate)
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(accumulate), "r"(lead)
       : "memory");
 }
 
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{.reg .pred e;\n"
+      "setp.ne.b32 e, %1, 0;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
 }
+
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(FULL, v, 0); }
 
 // 32 columns of this warp's 32 tensor-memory lanes.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -133,31 +194,6 @@ __device__ __forceinline__ void tmem_ld16u(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
-}
-
-// Two f32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("{.reg .b64 x, y, z;\n"
-      "mov.b64 x, {%2, %3};\n"
-      "mov.b64 y, {%4, %5};\n"
-      "mov.b64 z, {%6, %7};\n"
-      "fma.rn.f32x2 x, x, y, z;\n"
-      "mov.b64 {%0, %1}, x;}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{.reg .b64 x, y;\n"
-      "mov.b64 x, {%2, %3};\n"
-      "mov.b64 y, {%4, %5};\n"
-      "add.rn.f32x2 x, x, y;\n"
-      "mov.b64 {%0, %1}, x;}"
-      : "=f"(d.x), "=f"(d.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
 }
 
 template <int D>
@@ -421,26 +457,28 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       if (!ok && lane == 0) s_abort = 1;
       __syncwarp();
     } else {
-      // ---------------- MMA issue (lane 0); the whole warp clears values past the length ----------------
+      // ---------------- MMA issue (one lane); the whole warp clears values past the length ----------------
       const uint64_t qd = sw128_desc(smem_u32(sQ), 16), kd = sw128_desc(smem_u32(sK), 16);
       const uint64_t vd = sw128_desc(smem_u32(sV), S::SLAB);
-      const uint32_t id_s = idesc<T>(BN, false), id_o = idesc<T>(D, true);
+      constexpr uint32_t id_s = idesc<T>(BN, false), id_o = idesc<T>(D, true);
+      const uint32_t lead = lane == 0, tm = (uint32_t)uniform((int)tmem);
       bool ok = true;
       int g = 0, used = 0, done[NQ] = {0, 0};
       for (int n = 0; ok; ++n) {
         Piece q;
         ok = take(n, &q);
-        if (!ok || q.b < 0) break;
-        if (q.steps == 0) continue;
+        if (!ok || uniform(q.b) < 0) break;
+        const int steps = uniform(q.steps);
+        if (steps == 0) continue;
         ok = __all_sync(FULL, mbar_wait(&bars.q_full, used & 1, abort));
         if (!ok) break;
         ++used;
         tc_after();
-        const int tiles = q.t0 + tq < q.t1 ? 2 : 1;  // tiles with rows
-        for (int j = -1; j < q.steps && ok; ++j) {
+        const int tiles = uniform(q.t0 + tq < q.t1 ? 2 : 1);  // tiles with rows
+        for (int j = -1; j < steps && ok; ++j) {
           // step j of this piece is the CTA's step g + j
           const int sv = (g + j + STAGES) % STAGES, sk = (g + j + 1) % STAGES;
-          const bool more = j + 1 < q.steps;
+          const bool more = j + 1 < steps;
           if (more) ok = mbar_wait(&bars.k_full[sk], ((g + j + 1) / STAGES) & 1, abort);
           if (j >= 0) {
             ok = ok && mbar_wait(&bars.v_full[sv], ((g + j) / STAGES) & 1, abort);
@@ -459,6 +497,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           }
           ok = __all_sync(FULL, ok);
           if (!ok) break;
+          const uint64_t vb = vd + (uint32_t)((sv * S::TILE) >> 4), kb = kd + (uint32_t)((sk * S::TILE) >> 4);
 #pragma unroll
           for (int i = 0; i < NQ; ++i) {
             if (i >= tiles) break;
@@ -467,40 +506,34 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
               if (!ok) break;
               ++done[i];
               tc_after();
-              if (lane == 0) {
 #pragma unroll
-                for (int k = 0; k < BN / 16; ++k)
-                  umma_ts(tmem + O_COL + i * D, tmem + S_COL + i * BN + k * 8, vd + ((sv * S::TILE + k * 2048) >> 4), id_o,
-                          j > 0 || k > 0);
-                commit(&bars.o_full[i]);
-                if (i == tiles - 1) commit(&bars.v_free[sv]);
-              }
+              for (int k = 0; k < BN / 16; ++k)
+                umma_ts(lead, tm + O_COL + i * D, tm + S_COL + i * BN + k * 8, vb + (uint32_t)((k * 2048) >> 4), id_o,
+                        j > 0 || k > 0);
+              commit(lead, &bars.o_full[i]);
+              if (i == tiles - 1) commit(lead, &bars.v_free[sv]);
             }
             // S_i of the next keys: issued behind the product that reads P_i from the same columns
-            if (more && lane == 0) {
+            if (more) {
 #pragma unroll
               for (int k = 0; k < D / 16; ++k) {
                 const uint32_t off = (uint32_t)((k >> 2) * S::SLAB + (k & 3) * 32);
-                umma_ss(tmem + S_COL + i * BN, qd + ((i * S::TILE + off) >> 4), kd + ((sk * S::TILE + off) >> 4), id_s,
-                        k > 0);
+                umma_ss(lead, tm + S_COL + i * BN, qd + ((i * S::TILE + off) >> 4), kb + (off >> 4), id_s, k > 0);
               }
-              commit(&bars.s_full[i]);
+              commit(lead, &bars.s_full[i]);
               if (i == tiles - 1) {
-                commit(&bars.k_free[sk]);
-                if (j + 2 == q.steps) commit(&bars.q_free);
+                commit(lead, &bars.k_free[sk]);
+                if (j + 2 == steps) commit(lead, &bars.q_free);
               }
             }
-            __syncwarp();
           }
         }
-        g += q.steps;
+        g += steps;
       }
       if (!ok) {
-        if (lane == 0) {
-          s_abort = 1;
-          commit(&bars.drained);  // every MMA issued so far lands before the CTA goes on
-          (void)mbar_wait(&bars.drained, 0, nullptr);
-        }
+        if (lane == 0) s_abort = 1;
+        commit(lead, &bars.drained);  // every MMA issued so far lands before the CTA goes on
+        (void)mbar_wait(&bars.drained, 0, nullptr);
         __syncwarp();
       }
     }
@@ -548,7 +581,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
         const int base = (q.j0 + j) * BN;
         // keys that every live row of the tile sees need no mask
-        if (base + BN - 1 > q.past + first || (p.window > 0 && base <= q.past + min(q.t1, first + tq) - 1 - p.window)) {
+        const bool masked =
+            base + BN - 1 > q.past + first || (p.window > 0 && base <= q.past + min(q.t1, first + tq) - 1 - p.window);
+        if (masked) {
           const int from = key_lo - base;
           const unsigned width = (unsigned)max(0, pos + 1 - key_lo);  // columns [from, from + width)
 #pragma unroll
@@ -581,21 +616,27 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
+        // Of every four pairs of weights POLY are computed by arithmetic, the others by the exponential unit, which
+        // alone would take as long as both products. A masked step uses the unit alone: its -inf must give 0.
         float2 sum = make_float2(0.0f, 0.0f);
+        auto weights = [&](auto mixed) {
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
-          uint32_t w[16];
+          for (int c = 0; c < BN / 32; ++c) {
+            uint32_t w[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float2 x = fma2(make_float2(__uint_as_float(r[c * 32 + 2 * k]), __uint_as_float(r[c * 32 + 2 * k + 1])),
-                            make_float2(c_log2, c_log2), make_float2(-ref, -ref));
-            x.x = ex2(x.x);
-            x.y = ex2(x.y);
-            sum = add2(sum, x);
-            w[k] = Elem<T>::pack(x.x, x.y);
+            for (int k = 0; k < 16; ++k) {
+              float2 x = fma2(make_float2(__uint_as_float(r[c * 32 + 2 * k]), __uint_as_float(r[c * 32 + 2 * k + 1])),
+                              make_float2(c_log2, c_log2), make_float2(-ref, -ref));
+              if (decltype(mixed)::value && (k & 7) < POLY) x = exp2_poly(x);
+              else x = make_float2(ex2(x.x), ex2(x.y));
+              sum = add2(sum, x);
+              w[k] = Elem<T>::pack(x.x, x.y);
+            }
+            tmem_st16(s_at + c * 16, w);  // columns of S, all of which this row has read
           }
-          tmem_st16(s_at + c * 16, w);  // columns of S, all of which this row has read
-        }
+        };
+        if (masked) weights(std::false_type());
+        else weights(std::true_type());
         l += sum.x + sum.y;
         tmem_wait_st();
         tc_before();
