@@ -9,9 +9,9 @@
 // head); its keys are walked 128 at a time (a step). Few items are each cut along the keys into equal pieces, whose
 // results are joined by the last to arrive, in the pieces' order. The kernel is persistent: one CTA per SM takes
 // pieces from a counter, those with the most keys first, and runs its roles over them without a break:
-//   * one warp takes the pieces, hands them to the other roles through a small ring, and loads K and V pages by TMA
-//     (64 values x a page's tokens per box, SWIZZLE_128B) into rings of STAGES tiles;
-//   * two warps load the next piece's Q while the last step of the piece before runs;
+//   * one warp takes the pieces, hands them to the other roles through a small ring, and loads by TMA (SWIZZLE_128B): Q
+//     (64 values x the group's heads x a tile's tokens per box) once the piece before has issued its last scores, K and V
+//     pages (64 values x a page's tokens per box) into rings of STAGES tiles;
 //   * one thread issues S_i = Q_i K^T (128 x 128, f32 in tensor memory) and O_i += P_i V, alternating the
 //     two tiles, so the tensor cores work on one tile while the other's softmax runs;
 //   * four warps per tile hold one row per thread: maximum, exponentials and sum in f32, P rounded to the
@@ -34,22 +34,37 @@ constexpr int BM = 128;      // rows of a tile
 constexpr int BN = 128;      // keys of a tile
 constexpr int NQ = 2;        // tiles of a CTA
 constexpr int STAGES = 2;    // K tiles and V tiles in flight
-constexpr int SOFTMAX_WARPS = 4 * NQ;
+#ifndef WAITM
+#define WAITM 0
+#endif
+#ifndef WAITS
+#define WAITS 0
+#endif
+#ifndef HALVES
+#define HALVES 2
+#endif
+#ifndef SUMS
+#define SUMS 1
+#endif
+#ifndef PARTS_
+#define PARTS_ 1
+#endif
+constexpr int PARTS = PARTS_;     // column halves of a step, each with its own four warps
+constexpr int SOFTMAX_WARPS = 4 * NQ * PARTS;
 constexpr int MMA_WARP = SOFTMAX_WARPS;
 constexpr int LOAD_WARP = SOFTMAX_WARPS + 1;
-constexpr int Q_WARP = SOFTMAX_WARPS + 2;  // two of them
-constexpr int PF_THREADS = (SOFTMAX_WARPS + 4) * 32;
-// registers per thread: 168 at launch (384 threads), shared out anew: 2 x 216 + 72 = 3 x 168
-constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 72;
+constexpr int PF_THREADS = (SOFTMAX_WARPS + 4) * 32;  // the last two warps only give up their registers
+// registers per thread: 96 at launch (640 threads), shared out anew: 4 x 104 + 64 = 5 x 96
+constexpr int SOFTMAX_REGS = PARTS == 2 ? 104 : 216, OTHER_REGS = PARTS == 2 ? 64 : 72;
 constexpr int RING = 4;              // pieces handed out ahead
-constexpr int CONSUMERS = SOFTMAX_WARPS + 3;
+constexpr int CONSUMERS = SOFTMAX_WARPS + 1;
 constexpr int MAX_CUT = 16;          // pieces of an item
 constexpr int PIECE_COST = 3;        // what a piece costs beside its steps, in steps (Q, epilogue, join)
 constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0;            // S_i / P_i at columns BN * i
 constexpr int O_COL = NQ * BN;      // O_i at columns O_COL + D * i
 #ifndef POLY
-#define POLY 0
+#define POLY 1
 #endif
 constexpr float RESCALE = 8.0f;     // log2 of how far a row's reference may lag behind its maximum
 
@@ -59,6 +74,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
       "[%6];" ::"r"(smem_u32(dst)),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
 
@@ -90,6 +113,19 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+
+// mbar_wait without the suspend-time hint.
+__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_try(a, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t i = 0; i < WAIT_POLLS; ++i) {
+    if (mbar_try(a, parity)) return true;
+    if (*abort || clock64() - t0 > WAIT_CYCLES) return false;
+  }
+  return false;
+}
+template<int W> __device__ __forceinline__ bool wait_(uint64_t* bar, uint32_t parity, volatile int* abort) { return W ? mbar_poll(bar,parity,abort) : mbar_wait(bar,parity,abort); }
 
 // 2^x of two values by arithmetic alone: x = n + f with |f| <= 1/2 (adding and taking away 1.5 * 2^23 rounds to n), a
 // degree-5 polynomial of 2^f (coefficients fitted to equal relative error over the interval, 2.3e-7 in f32), n added
@@ -127,38 +163,41 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn_major) {
          ((uint32_t)(BM >> 4) << 24);
 }
 
-// The MMA warp issues converged, with one lane's predicate on each instruction: operands that the compiler can prove
-// uniform stay in uniform registers. (Inside an `if (lane == 0)` every operand was moved there one by one: 105 clocks per
-// instruction against 65 of execution.)
-__device__ __forceinline__ void umma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t id,
-                                        uint32_t accumulate) {
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
-      "{.reg .pred p, e;\n"
-      "setp.ne.b32 e, %5, 0;\n"
+      "{.reg .pred p;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(lead)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d),
+      "l"(a), "l"(b), "r"(id), "r"(accumulate)
       : "memory");
 }
 
-__device__ __forceinline__ void umma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t id,
-                                        uint32_t accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
-      "{.reg .pred p, e;\n"
-      "setp.ne.b32 e, %5, 0;\n"
+      "{.reg .pred p;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(accumulate), "r"(lead)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d),
+      "r"(a), "l"(b), "r"(id), "r"(accumulate)
       : "memory");
 }
 
-__device__ __forceinline__ void commit(uint32_t lead, uint64_t* bar) {
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+// One lane of the converged warp, the same one each time. The MMA warp runs converged on values made uniform and issues
+// inside `if (elect())`, where the compiler keeps the operands in uniform registers. Measured beside 16 warps of
+// arithmetic: 64 clocks per tcgen05.mma, its execution time; inside an `if (lane == 0)` 77, with a predicate per
+// instruction 87, and 105 with operands that were not made uniform first.
+__device__ __forceinline__ bool elect() {
+  uint32_t e;
   asm volatile(
-      "{.reg .pred e;\n"
-      "setp.ne.b32 e, %1, 0;\n"
-      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];}" ::"r"(smem_u32(bar)),
-      "r"(lead)
-      : "memory");
+      "{.reg .pred p;\n"
+      "elect.sync _|p, 0xffffffff;\n"
+      "selp.u32 %0, 1, 0, p;}"
+      : "=r"(e));
+  return e != 0;
 }
 
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(FULL, v, 0); }
@@ -205,7 +244,7 @@ struct PfShape {
 
 struct Bars {
   uint64_t k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES];
-  uint64_t s_full[NQ], p_full[NQ], o_full[NQ], q_full, q_free, item_full[RING], item_free[RING], drained;
+  uint64_t s_full[NQ], p_half[NQ], p_full[NQ], o_full[NQ], pair[NQ][4], q_full, q_free, item_full[RING], item_free[RING], drained;
 };
 
 // A piece of work: steps [j0, j0 + steps) over the keys of one item. row0: the sequence's first row; past: the position
@@ -301,7 +340,8 @@ __device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s
 
 template <class T, int D, bool CAP>
 __global__ void __launch_bounds__(PF_THREADS, 1)
-    prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                   const __grid_constant__ CUtensorMap v_map) {
   using S = PfShape<D>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -312,7 +352,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   __shared__ Piece s_items[RING];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
-  __shared__ int s_k_issued, s_v_issued;
+  __shared__ int s_k_issued, s_v_issued, s_q_issued;
+  __shared__ float s_swap[2][NQ][PARTS][BM];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort = &s_abort;
   const int tq = BM / p.group, span = NQ * tq;  // tokens of a tile, of an item
@@ -326,20 +367,26 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     }
     for (int i = 0; i < NQ; ++i) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.p_half[i], 4 * PARTS);
+      mbar_init(&bars.p_full[i], 4 * PARTS);
+      for (int w = 0; w < 4; ++w) mbar_init(&bars.pair[i][w], PARTS);
       mbar_init(&bars.o_full[i], 1);
     }
     for (int i = 0; i < RING; ++i) {
       mbar_init(&bars.item_full[i], 1);
       mbar_init(&bars.item_free[i], CONSUMERS);
     }
-    mbar_init(&bars.q_full, 2);
+    mbar_init(&bars.q_full, 1);
     mbar_init(&bars.q_free, 1);
     mbar_init(&bars.drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = 0;
-    s_k_issued = s_v_issued = 0;
+    s_k_issued = s_v_issued = s_q_issued = 0;
   }
+  // rows of a tile that no box fills (a group that does not divide 128) stay zero
+  if (tq * p.group < BM)
+    for (int e = tid; e < NQ * S::TILE / 16; e += PF_THREADS) reinterpret_cast<uint4*>(sQ)[e] = make_uint4(0, 0, 0, 0);
+  proxy_fence();
   pdl_wait();
   pdl_trigger();
   if (*reinterpret_cast<volatile int32_t*>(p.err) == (int32_t)MOE_ERR_TIMEOUT) return;
@@ -372,7 +419,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       const int box_rows = 1 << p.page_shift;
       const int pages = BN >> p.page_shift;  // per tile
       const int my = lane % pages, half = lane / pages;  // this lane's page and 64-value half: at most 16 boxes
-      int g = 0, w = blockIdx.x;
+      int g = 0, used = 0, w = blockIdx.x;
       bool ok = true;
       for (int n = 0; ok; ++n) {
         const Piece q = piece_of(p, batch, w, span, lane);
@@ -411,6 +458,19 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             if (on)
               tma_load_4d((kv ? sV : sK) + st * S::TILE + half * S::SLAB + my * box_rows * 128, kv ? &v_map : &k_map,
                           half * 64, 0, q.kvh, page, full);
+            if (kv == 0 && j == 0) {  // Q behind the first K tile: its place is the last to come free
+              ok = __all_sync(FULL, used == 0 || mbar_wait(&bars.q_free, (used - 1) & 1, abort));
+              if (!ok) break;
+              ++used;
+              if (lane == 0) {
+                mbar_expect_tx(&bars.q_full, (uint32_t)(NQ * (D / 64) * tq * p.group * 128));
+                s_q_issued = used;
+              }
+              __syncwarp();
+              if (lane < NQ * (D / 64))
+                tma_load_3d(sQ + (lane % NQ) * S::TILE + (lane / NQ) * S::SLAB, &q_map, lane / NQ * 64, q.kvh * p.group,
+                            q.row0 + q.t0 + (lane % NQ) * tq, &bars.q_full);
+            }
           }
         }
       }
@@ -419,49 +479,15 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       for (int c = max(0, g - STAGES); c < g && ok; ++c)
         ok = mbar_wait(&bars.k_free[c % STAGES], (c / STAGES) & 1, abort) &&
              mbar_wait(&bars.v_free[c % STAGES], (c / STAGES) & 1, abort);
-      if (!ok && lane == 0) s_abort = 1;
-      __syncwarp();
-    } else if (warp >= Q_WARP) {
-      // ---------------- Q into shared memory, swizzled as TMA would ----------------
-      bool ok = true;
-      int used = 0;  // pieces with steps so far
-      for (int n = 0; ok; ++n) {
-        Piece q;
-        ok = take(n, &q);
-        if (!ok || q.b < 0) break;
-        if (q.steps == 0) continue;
-        ok = __all_sync(FULL, used == 0 || mbar_wait(&bars.q_free, (used - 1) & 1, abort));
-        if (!ok) break;
-        ++used;
-        constexpr int CH = D / 8;
-        const int me = (warp - Q_WARP) * 32 + lane;
-        const int c = me % CH;
-        for (int r = me / CH; r < NQ * BM; r += 64 / CH) {
-          const int i = r / BM, rr = r % BM, tok = q.t0 + i * tq + rr / p.group;
-          const bool in = rr < tq * p.group && tok < q.t1;
-          const T* src = static_cast<const T*>(p.q) +
-                         (in ? (int64_t)(q.row0 + tok) * p.q_token_stride +
-                                   (int64_t)(q.kvh * p.group + rr % p.group) * p.q_head_stride + c * 8
-                             : 0);
-          const uint32_t dst =
-              smem_u32(sQ + i * S::TILE + (c / 8) * S::SLAB + rr * 128 + (((c & 7) ^ (rr & 7)) << 4));
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        proxy_fence();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.q_full);
-      }
-      // the last piece's release has landed
       if (ok && used > 0) ok = mbar_wait(&bars.q_free, (used - 1) & 1, abort);
       if (!ok && lane == 0) s_abort = 1;
       __syncwarp();
-    } else {
+    } else if (warp == MMA_WARP) {
       // ---------------- MMA issue (one lane); the whole warp clears values past the length ----------------
       const uint64_t qd = sw128_desc(smem_u32(sQ), 16), kd = sw128_desc(smem_u32(sK), 16);
       const uint64_t vd = sw128_desc(smem_u32(sV), S::SLAB);
       constexpr uint32_t id_s = idesc<T>(BN, false), id_o = idesc<T>(D, true);
-      const uint32_t lead = lane == 0, tm = (uint32_t)uniform((int)tmem);
+      const uint32_t tm = (uint32_t)uniform((int)tmem);
       bool ok = true;
       int g = 0, used = 0, done[NQ] = {0, 0};
       for (int n = 0; ok; ++n) {
@@ -502,54 +528,80 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           for (int i = 0; i < NQ; ++i) {
             if (i >= tiles) break;
             if (j >= 0) {
-              ok = __all_sync(FULL, mbar_wait(&bars.p_full[i], done[i] & 1, abort));
+              // the product starts on the first keys' weights while the last ones are being computed
+#pragma unroll
+              for (int e = 0; e < HALVES; ++e) {
+                ok = __all_sync(FULL, wait_<WAITM>(e == HALVES - 1 ? &bars.p_full[i] : &bars.p_half[i], done[i] & 1, abort));
+                if (!ok) break;
+                tc_after();
+                if (elect()) {
+#pragma unroll
+                  for (int k = e * (BN / 16) / HALVES; k < (e + 1) * (BN / 16) / HALVES; ++k)
+                    umma_ts(tm + O_COL + i * D, tm + S_COL + i * BN + k * 8, vb + (uint32_t)((k * 2048) >> 4), id_o,
+                            j > 0 || k > 0);
+                }
+                __syncwarp();
+              }
               if (!ok) break;
               ++done[i];
-              tc_after();
-#pragma unroll
-              for (int k = 0; k < BN / 16; ++k)
-                umma_ts(lead, tm + O_COL + i * D, tm + S_COL + i * BN + k * 8, vb + (uint32_t)((k * 2048) >> 4), id_o,
-                        j > 0 || k > 0);
-              commit(lead, &bars.o_full[i]);
-              if (i == tiles - 1) commit(lead, &bars.v_free[sv]);
             }
-            // S_i of the next keys: issued behind the product that reads P_i from the same columns
-            if (more) {
-#pragma unroll
-              for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (uint32_t)((k >> 2) * S::SLAB + (k & 3) * 32);
-                umma_ss(lead, tm + S_COL + i * BN, qd + ((i * S::TILE + off) >> 4), kb + (off >> 4), id_s, k > 0);
+            if (elect()) {
+              if (j >= 0) {
+                commit(&bars.o_full[i]);
+                if (i == tiles - 1) commit(&bars.v_free[sv]);
               }
-              commit(lead, &bars.s_full[i]);
-              if (i == tiles - 1) {
-                commit(lead, &bars.k_free[sk]);
-                if (j + 2 == steps) commit(lead, &bars.q_free);
+              // S_i of the next keys: issued behind the product that reads P_i from the same columns
+              if (more) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                  const uint32_t off = (uint32_t)((k >> 2) * S::SLAB + (k & 3) * 32);
+                  umma_ss(tm + S_COL + i * BN, qd + ((i * S::TILE + off) >> 4), kb + (off >> 4), id_s, k > 0);
+                }
+                commit(&bars.s_full[i]);
+                if (i == tiles - 1) {
+                  commit(&bars.k_free[sk]);
+                  if (j + 2 == steps) commit(&bars.q_free);
+                }
               }
             }
+            __syncwarp();
           }
         }
         g += steps;
       }
       if (!ok) {
         if (lane == 0) s_abort = 1;
-        commit(lead, &bars.drained);  // every MMA issued so far lands before the CTA goes on
+        if (elect()) commit(&bars.drained);  // every MMA issued so far lands before the CTA goes on
         (void)mbar_wait(&bars.drained, 0, nullptr);
         __syncwarp();
       }
     }
   } else {
-    // ---------------- softmax: one row per thread ----------------
+    // ---------------- softmax: half a row per thread ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
-    const int i = warp >> 2, quad = warp & 3;
+    constexpr int COLS = BN / PARTS, DCOLS = D / PARTS;  // this thread's keys of a step, its values of the output
+    const int i = warp / (4 * PARTS), h = (warp >> 2) % PARTS, quad = warp & 3;
     const int rr = quad * 32 + lane;
     const int my_tok = i * tq + rr / p.group, my_head = rr % p.group;
     const bool my_row = rr < tq * p.group;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t s_at = lane_base + S_COL + i * BN, o_at = lane_base + O_COL + i * D;
+    const uint32_t s_at = lane_base + S_COL + i * BN, o_at = lane_base + O_COL + i * D + h * DCOLS;
     const float c_log2 = CAP ? 1.0f : p.scale * LOG2E;
     const float cap_in = CAP ? 2.0f * LOG2E * p.scale / p.softcap : 0.0f, cap_out = p.softcap * LOG2E;
     bool ok = true;
-    int seen = 0;  // steps so far
+    int seen = 0;   // steps so far
+    int swaps = 0;  // exchanges so far
+    // The other half's value of this row (warp-collective; false once a wait gave up). Two buffers: a warp that is one
+    // exchange ahead writes the other one.
+    auto swap = [&](float mine, float* other) -> bool {
+      s_swap[swaps & 1][i][h][rr] = mine;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.pair[i][quad]);
+      const bool got = __all_sync(FULL, mbar_wait(&bars.pair[i][quad], swaps & 1, abort));
+      *other = s_swap[swaps & 1][i][h ^ 1][rr];
+      ++swaps;
+      return got;
+    };
     for (int n = 0; ok; ++n) {
       Piece q;
       ok = take(n, &q);
@@ -560,23 +612,24 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       const bool live = my_row && tok < q.t1;
       const int pos = q.past + tok;  // this row sees keys (pos - window, pos]
       const int key_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-      float m = -INFINITY, l = 0.0f;  // reference in units of log2, sum of weights
+      float m = -INFINITY, l = 0.0f;  // reference in units of log2, sum of this half's weights
       for (int j = 0; j < q.steps; ++j, ++seen) {
-        ok = mbar_wait(&bars.s_full[i], seen & 1, abort);
+        ok = wait_<WAITS>(&bars.s_full[i], seen & 1, abort);
         // the product with the previous step's P has been issued before this S, and finished: its phase is taken
         // note of here, and O may be rescaled
         if (ok && j > 0) ok = mbar_wait(&bars.o_full[i], (seen - 1) & 1, abort);
         ok = __all_sync(FULL, ok);
         if (!ok) break;
         tc_after();
-        uint32_t r[BN];
+        uint32_t r[COLS];
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+        for (int c = 0; c < COLS / 32; ++c)
+          tmem_ld32(s_at + h * COLS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
         tmem_wait_ld();
         if (CAP) {
           // softcap * tanh(x) = softcap * (1 - 2 / (e^2x + 1)), absolute error about 1e-7 of the cap
 #pragma unroll
-          for (int k = 0; k < BN; ++k)
+          for (int k = 0; k < COLS; ++k)
             r[k] = __float_as_uint(cap_out - __fdividef(2.0f * cap_out, ex2(__uint_as_float(r[k]) * cap_in) + 1.0f));
         }
         const int base = (q.j0 + j) * BN;
@@ -584,19 +637,28 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         const bool masked =
             base + BN - 1 > q.past + first || (p.window > 0 && base <= q.past + min(q.t1, first + tq) - 1 - p.window);
         if (masked) {
-          const int from = key_lo - base;
+          const int from = key_lo - base - h * COLS;
           const unsigned width = (unsigned)max(0, pos + 1 - key_lo);  // columns [from, from + width)
 #pragma unroll
-          for (int k = 0; k < BN; ++k)
+          for (int k = 0; k < COLS; ++k)
             if ((unsigned)(k - from) >= width) r[k] = 0xff800000u;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < BN; k += 8)
+        for (int k = 0; k < COLS; k += 8)
 #pragma unroll
           for (int a = 0; a < 4; ++a)
             mx[a] = fmaxf(fmaxf(mx[a], __uint_as_float(r[k + 2 * a])), __uint_as_float(r[k + 2 * a + 1]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c_log2;  // scale > 0
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), top2;
+        // both halves have read S once the exchange is done: P may be written over it
+        if (PARTS == 2) {
+          tc_before();
+          ok = swap(top, &top2);
+          if (!ok) break;
+          tc_after();
+          top = fmaxf(top, top2);
+        }
+        top *= c_log2;  // scale > 0
         const bool grow = top > m + RESCALE;  // also the first finite maximum
         if (__any_sync(FULL, grow)) {
           const float mn = grow ? top : m;
@@ -605,7 +667,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           l *= f;
           if (j > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
+            for (int c = 0; c < DCOLS / 16; ++c) {
               uint32_t o[16];
               tmem_ld16u(o_at + c * 16, o);
               tmem_wait_ld();
@@ -616,12 +678,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        // Of every four pairs of weights POLY are computed by arithmetic, the others by the exponential unit, which
+        // Of every eight pairs of weights POLY are computed by arithmetic, the others by the exponential unit, which
         // alone would take as long as both products. A masked step uses the unit alone: its -inf must give 0.
-        float2 sum = make_float2(0.0f, 0.0f);
+        float2 sum = make_float2(0.0f, 0.0f), sum1 = sum;
         auto weights = [&](auto mixed) {
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) {
+          for (int c = 0; c < COLS / 32; ++c) {
             uint32_t w[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
@@ -629,30 +691,40 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                               make_float2(c_log2, c_log2), make_float2(-ref, -ref));
               if (decltype(mixed)::value && (k & 7) < POLY) x = exp2_poly(x);
               else x = make_float2(ex2(x.x), ex2(x.y));
-              sum = add2(sum, x);
+              if (SUMS == 2 && (k & 1)) sum1 = add2(sum1, x); else sum = add2(sum, x);
               w[k] = Elem<T>::pack(x.x, x.y);
             }
-            tmem_st16(s_at + c * 16, w);  // columns of S, all of which this row has read
+            tmem_st16(s_at + h * (COLS / 2) + c * 16, w);
+            if (HALVES == 2 && c == COLS / 64 - 1) {
+              tmem_wait_st();
+              tc_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&bars.p_half[i]);
+            }
           }
         };
         if (masked) weights(std::false_type());
         else weights(std::true_type());
-        l += sum.x + sum.y;
+        l += (sum.x + sum1.x) + (sum.y + sum1.y);
         tmem_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.p_full[i]);
       }
       if (ok && q.steps > 0) ok = __all_sync(FULL, mbar_wait(&bars.o_full[i], (seen - 1) & 1, abort));
+      float l2 = 0.0f;
+      if (ok && PARTS == 2) ok = swap(l, &l2);
       if (!ok) break;
       tc_after();
+      l = h ? l2 + l : l + l2;  // one order for both halves
       // ---- the piece's rows: out, or into the workspace ----
       const int64_t row = (int64_t)(q.row0 + tok) * p.heads + q.kvh * p.group + my_head;
-      T* dst = static_cast<T*>(p.y) + row * D;
-      float4* part = p.partial + ((int64_t)(q.item * q.cut + q.k) * NQ + i) * (D / 4) * BM + rr;  // [D / 4][BM]
+      T* dst = static_cast<T*>(p.y) + row * D + h * DCOLS;
+      const int64_t slot = (int64_t)q.item * q.cut * NQ + i;  // piece k of this tile at slot + k * NQ
+      float4* part = p.partial + (slot * (D / 4) + h * (DCOLS / 4)) * BM + rr;  // [D / 4][BM] of a slot
       const float inv = q.cut > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {
+      for (int c = 0; c < DCOLS / 16; ++c) {
         uint32_t o[16];
         if (q.steps > 0) {
           tmem_ld16u(o_at + c * 16, o);
@@ -664,7 +736,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (q.cut > 1) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            __stcg(part + (c * 4 + k) * BM, make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]));
+            __stcg(part + ((int64_t)q.k * NQ * (D / 4) + c * 4 + k) * BM,
+                   make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]));
         } else if (live) {
 #pragma unroll
           for (int k = 0; k < 2; ++k)
@@ -674,49 +747,44 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
       }
       if (q.cut == 1) {
-        if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
+        if (h == 0 && live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
         continue;
       }
-      // ---- the last of the item's pieces to arrive joins them in order, each warp its own rows ----
-      float2* ml = p.partial_ml + ((int64_t)q.item * q.cut * NQ + i) * BM + rr;  // piece k at k * NQ * BM
-      __stcg(ml + q.k * NQ * BM, make_float2(m, l));
+      // ---- the last of the item's pieces to arrive joins them in order, each warp its own rows and values ----
+      float2* ml = p.partial_ml + (slot * PARTS + h) * BM + rr;  // piece k at k * NQ * PARTS * BM
+      constexpr int MLS = NQ * PARTS * BM;
+      __stcg(ml + q.k * MLS, make_float2(m, l));
       __threadfence();
       __syncwarp();
       int last = 0;
       if (lane == 0) {
-        int32_t* cnt = p.counters + (q.item * NQ + i) * 4 + quad;
+        int32_t* cnt = p.counters + ((q.item * NQ + i) * PARTS + h) * 4 + quad;
         last = atomicAdd(cnt, 1) == q.cut - 1;
         if (last) *cnt = 0;  // ready for the next call
       }
       if (__shfl_sync(FULL, last, 0)) {
         __threadfence();
-        float M = -INFINITY, L = 0.0f, f[MAX_CUT];
-#pragma unroll
-        for (int k = 0; k < MAX_CUT; ++k) {
-          f[k] = -INFINITY;
-          if (k < q.cut) f[k] = __ldcg(ml + k * NQ * BM).x;
-          M = fmaxf(M, f[k]);
-        }
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll 4
+        for (int k = 0; k < q.cut; ++k) M = fmaxf(M, __ldcg(ml + k * MLS).x);
         const float at = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-        for (int k = 0; k < MAX_CUT; ++k) {
-          f[k] = ex2(f[k] - at);
-          if (k < q.cut) L += __ldcg(ml + k * NQ * BM).y * f[k];
+#pragma unroll 4
+        for (int k = 0; k < q.cut; ++k) {
+          const float2 v = __ldcg(ml + k * MLS);
+          L += v.y * ex2(v.x - at);
         }
         const float il = L == 0.0f ? 0.0f : 1.0f / L;
-        const float4* src = p.partial + ((int64_t)q.item * q.cut * NQ + i) * (D / 4) * BM + rr;
 #pragma unroll 1
-        for (int c = 0; c < D / 8; ++c) {
+        for (int c = 0; c < DCOLS / 8; ++c) {
           float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+#pragma unroll 4
+          for (int k = 0; k < q.cut; ++k) {
+            const float f = ex2(__ldcg(ml + k * MLS).x - at);
 #pragma unroll
-          for (int k = 0; k < MAX_CUT; ++k) {
-            if (k < q.cut) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float4 v = __ldcg(src + ((int64_t)k * NQ * (D / 4) + c * 2 + h) * BM);
-                o[h].x = fmaf(v.x, f[k], o[h].x), o[h].y = fmaf(v.y, f[k], o[h].y);
-                o[h].z = fmaf(v.z, f[k], o[h].z), o[h].w = fmaf(v.w, f[k], o[h].w);
-              }
+            for (int e = 0; e < 2; ++e) {
+              const float4 v = __ldcg(part + ((int64_t)k * NQ * (D / 4) + c * 2 + e) * BM);
+              o[e].x = fmaf(v.x, f, o[e].x), o[e].y = fmaf(v.y, f, o[e].y);
+              o[e].z = fmaf(v.z, f, o[e].z), o[e].w = fmaf(v.w, f, o[e].w);
             }
           }
           if (live)
@@ -724,14 +792,16 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 make_uint4(Elem<T>::pack(o[0].x * il, o[0].y * il), Elem<T>::pack(o[0].z * il, o[0].w * il),
                            Elem<T>::pack(o[1].x * il, o[1].y * il), Elem<T>::pack(o[1].z * il, o[1].w * il));
         }
-        if (live && p.lse) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
+        if (h == 0 && live && p.lse) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
       }
     }
     if (!ok && lane == 0) s_abort = 1;
   }
   __syncthreads();
   if (tid == 0) {
-    if (s_abort) {  // the copies still in flight land before the CTA's shared memory goes
+    if (s_abort) {
+      if (s_q_issued) (void)mbar_wait(&bars.q_full, (s_q_issued - 1) & 1, nullptr);
+      // the copies still in flight land before the CTA's shared memory goes
       for (int j = max(0, s_k_issued - STAGES); j < s_k_issued; ++j)
         (void)mbar_wait(&bars.k_full[j % STAGES], (j / STAGES) & 1, nullptr);
       for (int j = max(0, s_v_issued - STAGES); j < s_v_issued; ++j)
@@ -765,6 +835,10 @@ static moe_status with_kernel(const moe_attn& a, F&& f) {
   return a.d.dtype == MOE_ATTN_BF16 ? by_type(__nv_bfloat16()) : by_type(__half());
 }
 
+static CUtensorMapDataType map_type(int dtype) {
+  return dtype == MOE_ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
 moe_status prepare_prefill(const moe_attn& a) {
   return with_kernel(a, [](auto kernel, int smem) -> moe_status {
     MOE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -773,20 +847,30 @@ moe_status prepare_prefill(const moe_attn& a) {
 }
 
 moe_status launch_prefill(const moe_attn& a, const PrefillParams& p, cudaStream_t st) {
-  const int span = NQ * (BM / p.group);
+  const int tq = BM / p.group, span = NQ * tq;
   // every sequence wastes less than one item
   const int64_t items = ((int64_t)p.T / span + std::min(p.B, p.T)) * p.kv_heads;
   if (items > 0x3fffffff) return fail(MOE_ERR_INVALID, "moe_attn_prefill: too many rows");
   const int grid = (int)std::min<int64_t>(a.sms, items * MAX_CUT);
+  // strides of dimensions of size 1 are never used and may be anything
+  const int64_t ts = p.T > 1 ? p.q_token_stride : (int64_t)p.heads * a.d.head_dim;
+  const int64_t hs = p.heads > 1 ? p.q_head_stride : a.d.head_dim;
+  if (ts <= 0 || hs <= 0 || ts >= (1ll << 38) || hs >= (1ll << 38))
+    return fail(MOE_ERR_INVALID, "moe_attn_prefill: q strides must be positive");
+  const cuuint64_t dims[3] = {(cuuint64_t)a.d.head_dim, (cuuint64_t)p.heads, (cuuint64_t)p.T};
+  const cuuint64_t strides[2] = {(cuuint64_t)hs * 2, (cuuint64_t)ts * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)tq};
+  CUtensorMap q_map;
+  MOE_TRY(encode_tmap_sw128(&q_map, map_type(a.d.dtype), 3, p.q, dims, strides, box));
   return with_kernel(a, [&](auto kernel, int smem) -> moe_status {
-    MOE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(PF_THREADS), smem, st, p, a.k_map, a.v_map));
+    MOE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(PF_THREADS), smem, st, p, q_map, a.k_map, a.v_map));
     return MOE_OK;
   });
 }
 
 size_t prefill_partial_bytes(const moe_attn& a) { return (size_t)2 * a.sms * NQ * BM * a.d.head_dim * sizeof(float); }
-size_t prefill_ml_bytes(const moe_attn& a) { return (size_t)2 * a.sms * NQ * BM * sizeof(float2); }
-size_t prefill_counters(const moe_attn& a) { return (size_t)2 * a.sms * NQ * 4; }
+size_t prefill_ml_bytes(const moe_attn& a) { return (size_t)2 * a.sms * NQ * PARTS * BM * sizeof(float2); }
+size_t prefill_counters(const moe_attn& a) { return (size_t)2 * a.sms * NQ * PARTS * 4; }
 
 moe_status make_page_tmap(CUtensorMap* map, int dtype, const void* pool, int head_dim, int page_size, int kv_heads,
                           int64_t num_pages, int64_t page_stride) {
@@ -794,8 +878,7 @@ moe_status make_page_tmap(CUtensorMap* map, int dtype, const void* pool, int hea
   const cuuint64_t strides[3] = {(cuuint64_t)head_dim * 2, (cuuint64_t)page_size * head_dim * 2,
                                  (cuuint64_t)page_stride * 2};
   const cuuint32_t box[4] = {64, (cuuint32_t)page_size, 1, 1};
-  return encode_tmap_sw128(map, dtype == MOE_ATTN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                           4, pool, dims, strides, box);
+  return encode_tmap_sw128(map, map_type(dtype), 4, pool, dims, strides, box);
 }
 
 }  // namespace attn

@@ -252,6 +252,8 @@ class PagedAttention:
         [T, num_heads, head_dim], or (y, lse)."""
         torch = _torch()
         q = self._rows(q, self.config.num_heads, "prefill: q")
+        if not all(q.stride()):  # an expanded tensor: the tile loads take positive strides only
+            q = q.contiguous()
         B = seq_lens.shape[0]
         cu_q = self._ints(cu_q, (B + 1,), "prefill: cu_q", torch.int32)
         seq_lens = self._ints(seq_lens, (B,), "prefill: seq_lens", torch.int32)
