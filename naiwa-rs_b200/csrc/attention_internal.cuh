@@ -126,6 +126,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// The same, kept in program order with its like.
+__device__ __forceinline__ float ex2_ordered(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void latch(int32_t* err, moe_status st) { atomicCAS(err, 0, (int32_t)st); }
 
 }  // namespace attn

@@ -30,32 +30,62 @@
 namespace moe {
 namespace attn {
 
+#ifndef LEAN
+#define LEAN 2
+#endif
+#if LEAN & 1
+#define WAITM_ wait_poll
+#else
+#define WAITM_ mbar_wait
+#endif
+#if LEAN & 2
+#define WAITS_ wait_poll
+#else
+#define WAITS_ mbar_wait
+#endif
+#if LEAN & 4
+#define WAITL_ wait_poll
+#else
+#define WAITL_ mbar_wait
+#endif
+#ifndef ROLLI
+#define ROLLI 0
+#endif
+#ifndef EXPECT
+#define EXPECT 1
+#endif
+#ifndef EXV
+#define EXV 1
+#endif
+#ifndef SPLIT
+#define SPLIT 4
+#endif
+constexpr int kUnrI = ROLLI ? 1 : 2;
 constexpr int BM = 128;      // rows of a tile
 constexpr int BN = 128;      // keys of a tile
 constexpr int NQ = 2;        // tiles of a CTA
-constexpr int STAGES = 2;    // K tiles and V tiles in flight
-#ifndef WAITM
-#define WAITM 0
+#ifndef KST
+#define KST 3
 #endif
-#ifndef WAITS
-#define WAITS 0
+#ifndef VST
+#define VST 2
 #endif
-#ifndef HALVES
-#define HALVES 2
+constexpr int KS = KST, VS = VST;  // K tiles and V tiles in flight
+#ifndef EXPECT
+#define EXPECT 1
 #endif
-#ifndef SUMS
-#define SUMS 1
+#ifndef EXV
+#define EXV 1
 #endif
-#ifndef PARTS_
-#define PARTS_ 1
+#ifndef SPLIT
+#define SPLIT 6
 #endif
-constexpr int PARTS = PARTS_;     // column halves of a step, each with its own four warps
-constexpr int SOFTMAX_WARPS = 4 * NQ * PARTS;
+constexpr int SOFTMAX_WARPS = 4 * NQ;
 constexpr int MMA_WARP = SOFTMAX_WARPS;
 constexpr int LOAD_WARP = SOFTMAX_WARPS + 1;
 constexpr int PF_THREADS = (SOFTMAX_WARPS + 4) * 32;  // the last two warps only give up their registers
-// registers per thread: 96 at launch (640 threads), shared out anew: 4 x 104 + 64 = 5 x 96
-constexpr int SOFTMAX_REGS = PARTS == 2 ? 104 : 216, OTHER_REGS = PARTS == 2 ? 64 : 72;
+// registers per thread: 168 at launch (384 threads), shared out anew: 2 x 216 + 72 = 3 x 168
+constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 72;
 constexpr int RING = 4;              // pieces handed out ahead
 constexpr int CONSUMERS = SOFTMAX_WARPS + 1;
 constexpr int MAX_CUT = 16;          // pieces of an item
@@ -63,9 +93,6 @@ constexpr int PIECE_COST = 3;        // what a piece costs beside its steps, in 
 constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0;            // S_i / P_i at columns BN * i
 constexpr int O_COL = NQ * BN;      // O_i at columns O_COL + D * i
-#ifndef POLY
-#define POLY 1
-#endif
 constexpr float RESCALE = 8.0f;     // log2 of how far a row's reference may lag behind its maximum
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
@@ -114,46 +141,26 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-// mbar_wait without the suspend-time hint.
-__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, volatile int* abort) {
+// mbar_wait without the suspend-time hint and in few instructions.
+__device__ __forceinline__ bool wait_poll(uint64_t* bar, uint32_t parity, volatile int* abort) {
   const uint32_t a = smem_u32(bar);
-  if (mbar_try(a, parity)) return true;
-  const long long t0 = clock64();
-  for (uint32_t i = 0; i < WAIT_POLLS; ++i) {
-    if (mbar_try(a, parity)) return true;
-    if (*abort || clock64() - t0 > WAIT_CYCLES) return false;
+  uint32_t t0 = 0;
+#pragma unroll 1
+  while (!mbar_try(a, parity)) {
+    const uint32_t t = (uint32_t)clock() | 1u;
+    if (t0 == 0) t0 = t;
+    if (*abort || t - t0 > (uint32_t)WAIT_CYCLES) return false;
   }
-  return false;
-}
-template<int W> __device__ __forceinline__ bool wait_(uint64_t* bar, uint32_t parity, volatile int* abort) { return W ? mbar_poll(bar,parity,abort) : mbar_wait(bar,parity,abort); }
-
-// 2^x of two values by arithmetic alone: x = n + f with |f| <= 1/2 (adding and taking away 1.5 * 2^23 rounds to n), a
-// degree-5 polynomial of 2^f (coefficients fitted to equal relative error over the interval, 2.3e-7 in f32), n added
-// to the exponent. Inputs below -126 give 2^-126.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-  const float magic = 12582912.0f;
-  x.x = fmaxf(x.x, -126.0f);
-  x.y = fmaxf(x.y, -126.0f);
-  const float2 t = add2(x, make_float2(magic, magic));
-  const float2 n = add2(t, make_float2(-magic, -magic));
-  const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
-  auto c = [](float v) { return make_float2(v, v); };
-  float2 r = fma2(f, c(0x1.5c08e6p-10f), c(0x1.3d0c52p-7f));
-  r = fma2(r, f, c(0x1.c6b6e4p-5f));
-  r = fma2(r, f, c(0x1.ebf918p-3f));
-  r = fma2(r, f, c(0x1.62e428p-1f));
-  r = fma2(r, f, c(0x1.000002p+0f));
-  return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
+  return true;
 }
 
-// SWIZZLE_128B shared-memory matrix descriptor, slabs of 64 values x n rows of 128 bytes, 8-row groups 1024 bytes
-// apart. Q and K: K-major (the leading offset is not used). V: MN-major, the next 64 output columns lie
-// `leading` bytes on.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t leading) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(leading >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// Low word of a SWIZZLE_128B shared-memory matrix descriptor, slabs of 64 values x n rows of 128 bytes, 8-row groups 1024
+// bytes apart; the high word is the same for all. Q and K: K-major (the leading offset is not used). V: MN-major, the next
+// 64 output columns lie `leading` bytes on. Addresses below 256 KB: adding (bytes >> 4) moves the start.
+__device__ __forceinline__ uint32_t sw128_desc(uint32_t addr, uint32_t leading) {
+  return ((addr >> 4) & 0x3FFF) | ((leading >> 4) << 16);
 }
+constexpr uint32_t SW128_HIGH = (1024 >> 4) | (1u << 14) | (2u << 29);
 
 // kind::f16 instruction descriptor: f32 accumulator, A and B both bf16 or both f16, M = 128, N = n.
 template <class T>
@@ -163,21 +170,26 @@ __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn_major) {
          ((uint32_t)(BM >> 4) << 24);
 }
 
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
       "{.reg .pred p;\n"
+      ".reg .b64 x, y;\n"
+      "mov.b64 x, {%1, %5};\n"
+      "mov.b64 y, {%2, %5};\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;}" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(accumulate), "n"(SW128_HIGH)
       : "memory");
 }
 
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t accumulate) {
   asm volatile(
       "{.reg .pred p;\n"
+      ".reg .b64 y;\n"
+      "mov.b64 y, {%2, %5};\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;}" ::"r"(d),
+      "r"(a), "r"(b), "r"(id), "r"(accumulate), "n"(SW128_HIGH)
       : "memory");
 }
 
@@ -239,12 +251,12 @@ template <int D>
 struct PfShape {
   static constexpr int SLAB = BN * 128;            // 64 values x 128 rows
   static constexpr int TILE = (D / 64) * SLAB;     // a Q, K or V tile
-  static constexpr int BYTES = (NQ + 2 * STAGES) * TILE + 1024;
+  static constexpr int BYTES = (NQ + KS + VS) * TILE + 1024;
 };
 
 struct Bars {
-  uint64_t k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES];
-  uint64_t s_full[NQ], p_half[NQ], p_full[NQ], o_full[NQ], pair[NQ][4], q_full, q_free, item_full[RING], item_free[RING], drained;
+  uint64_t k_full[KS], v_full[VS], k_free[KS], v_free[VS];
+  uint64_t s_full[NQ], p_most[NQ], p_full[NQ], o_full[NQ], q_full, q_free, item_full[RING], item_free[RING], drained;
 };
 
 // A piece of work: steps [j0, j0 + steps) over the keys of one item. row0: the sequence's first row; past: the position
@@ -267,6 +279,7 @@ __device__ __forceinline__ Batch read_batch(const PrefillParams& p, int span, in
   s.per = (p.B + 31) / 32;
   s.mine = 0;
   int most = 0;  // steps of the longest item
+#pragma unroll 1
   for (int b = min(p.B, lane * s.per); b < min(p.B, (lane + 1) * s.per); ++b) {
     const int n = tokens_of(p, b);
     if (n == 0) continue;
@@ -312,6 +325,7 @@ __device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s
   int b = 0, tile = 0;
   if (here) {
     int at = s.before;
+#pragma unroll 1
     for (b = lane * s.per;; ++b) {
       const int n = (tokens_of(p, b) + span - 1) / span;
       if (u < at + n) break;
@@ -332,9 +346,9 @@ __device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s
   const int hi = max(0, q.past + q.t1);  // keys [lo, hi)
   const int lo = p.window > 0 ? max(0, q.past + q.t0 - p.window + 1) : 0;
   const int first = lo / BN, all = hi > lo ? (hi + BN - 1) / BN - first : 0;
-  const int a = (int)((int64_t)all * q.k / q.cut);
+  const int a = all * q.k / q.cut;  // all < 2^24, cut <= MAX_CUT
   q.j0 = first + a;
-  q.steps = (int)((int64_t)all * (q.k + 1) / q.cut) - a;
+  q.steps = all * (q.k + 1) / q.cut - a;
   return q;
 }
 
@@ -347,29 +361,29 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* sQ = smem;
   unsigned char* sK = sQ + NQ * S::TILE;
-  unsigned char* sV = sK + STAGES * S::TILE;
+  unsigned char* sV = sK + KS * S::TILE;
   __shared__ Bars bars;
   __shared__ Piece s_items[RING];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ int s_k_issued, s_v_issued, s_q_issued;
-  __shared__ float s_swap[2][NQ][PARTS][BM];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort = &s_abort;
   const int tq = BM / p.group, span = NQ * tq;  // tokens of a tile, of an item
 
   if (tid == 0) {
-    for (int i = 0; i < STAGES; ++i) {
+    for (int i = 0; i < KS; ++i) {
       mbar_init(&bars.k_full[i], 1);
-      mbar_init(&bars.v_full[i], 1);
       mbar_init(&bars.k_free[i], 1);
+    }
+    for (int i = 0; i < VS; ++i) {
+      mbar_init(&bars.v_full[i], 1);
       mbar_init(&bars.v_free[i], 1);
     }
     for (int i = 0; i < NQ; ++i) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_half[i], 4 * PARTS);
-      mbar_init(&bars.p_full[i], 4 * PARTS);
-      for (int w = 0; w < 4; ++w) mbar_init(&bars.pair[i][w], PARTS);
+      mbar_init(&bars.p_most[i], 4);
+      mbar_init(&bars.p_full[i], 4);
       mbar_init(&bars.o_full[i], 1);
     }
     for (int i = 0; i < RING; ++i) {
@@ -403,7 +417,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   // The n-th piece for a consuming warp; false once a wait gave up. Lane 0 releases the slot.
   auto take = [&](int n, Piece* q) -> bool {
     const int slot = n % RING;
-    const bool ok = __all_sync(FULL, mbar_wait(&bars.item_full[slot], (n / RING) & 1, abort));
+    const bool ok = __all_sync(FULL, WAITL_(&bars.item_full[slot], (n / RING) & 1, abort));
     if (!ok) return false;
     *q = s_items[slot];
     __syncwarp();
@@ -418,13 +432,17 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       const Batch batch = read_batch(p, span, lane, gridDim.x);
       const int box_rows = 1 << p.page_shift;
       const int pages = BN >> p.page_shift;  // per tile
-      const int my = lane % pages, half = lane / pages;  // this lane's page and 64-value half: at most 16 boxes
-      int g = 0, used = 0, w = blockIdx.x;
+      const int half = lane / pages;  // this lane's 64-value half and page: at most 16 boxes
+      const int my = half < D / 64 ? lane % pages : pages;
+      const int box_bytes = box_rows * (D / 64) * 128;
+      unsigned char* dst = sK + half * S::SLAB + my * box_rows * 128;
+      int g = 0, used = 0, w = blockIdx.x, issued = 0;  // K and V tiles, in turn
       bool ok = true;
+#pragma unroll 1
       for (int n = 0; ok; ++n) {
         const Piece q = piece_of(p, batch, w, span, lane);
         const int slot = n % RING;
-        ok = __all_sync(FULL, n < RING || mbar_wait(&bars.item_free[slot], ((n / RING) - 1) & 1, abort));
+        ok = __all_sync(FULL, n < RING || WAITL_(&bars.item_free[slot], ((n / RING) - 1) & 1, abort));
         if (!ok) break;
         if (lane == 0) {
           s_items[slot] = q;
@@ -433,39 +451,32 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
         if (q.b < 0) break;
         w = __shfl_sync(FULL, w, 0);
+        const int32_t* table = p.page_table + (int64_t)q.b * p.max_pages + my;
+#pragma unroll 1
         for (int j = 0; j < q.steps && ok; ++j, ++g) {
           const int base = (q.j0 + j) * BN;
           const int live = min(pages, (q.len - base + box_rows - 1) >> p.page_shift);  // pages that hold tokens
-          const int st = g % STAGES;
-          const bool on = half < D / 64 && my < live;
-          int page = 0;
-          if (on) page = __ldg(p.page_table + (int64_t)q.b * p.max_pages + (base >> p.page_shift) + my);
-          if (on && (unsigned)page >= (unsigned)p.num_pages) {
+          const bool on = my < live;
+          int page = on ? __ldg(table + (base >> p.page_shift)) : 0;
+          if ((unsigned)page >= (unsigned)p.num_pages) {
             latch(p.err, MOE_ERR_BAD_IDS);
             page = p.num_pages;  // out of the map: the box reads as zeros
           }
+#pragma unroll 1
           for (int kv = 0; kv < 2; ++kv) {
+            const int n_st = kv ? VS : KS, st = g % n_st;
             uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
-            uint64_t* free_ = kv ? &bars.v_free[st] : &bars.k_free[st];
-            ok = __all_sync(FULL, g < STAGES || mbar_wait(free_, ((g / STAGES) - 1) & 1, abort));
+            ok = __all_sync(FULL, WAITL_(kv ? &bars.v_free[st] : &bars.k_free[st], ((g / n_st) & 1) ^ 1, abort));
             if (!ok) break;
-            if (lane == 0) {
-              mbar_expect_tx(full, (uint32_t)(live * box_rows * (D / 64) * 128));
-              if (kv) s_v_issued = g + 1;
-              else s_k_issued = g + 1;
-            }
+            if (lane == 0) mbar_expect_tx(full, (uint32_t)(live * box_bytes));
             __syncwarp();
-            if (on)
-              tma_load_4d((kv ? sV : sK) + st * S::TILE + half * S::SLAB + my * box_rows * 128, kv ? &v_map : &k_map,
-                          half * 64, 0, q.kvh, page, full);
-            if (kv == 0 && j == 0) {  // Q behind the first K tile: its place is the last to come free
-              ok = __all_sync(FULL, used == 0 || mbar_wait(&bars.q_free, (used - 1) & 1, abort));
+            if (on) tma_load_4d(dst + (kv * KS + st) * S::TILE, kv ? &v_map : &k_map, half * 64, 0, q.kvh, page, full);
+            ++issued;
+            if (kv + j == 0) {  // Q behind the first K tile: its place is the last to come free
+              ok = __all_sync(FULL, WAITL_(&bars.q_free, (used & 1) ^ 1, abort));
               if (!ok) break;
               ++used;
-              if (lane == 0) {
-                mbar_expect_tx(&bars.q_full, (uint32_t)(NQ * (D / 64) * tq * p.group * 128));
-                s_q_issued = used;
-              }
+              if (lane == 0) mbar_expect_tx(&bars.q_full, (uint32_t)(NQ * (D / 64) * tq * p.group * 128));
               __syncwarp();
               if (lane < NQ * (D / 64))
                 tma_load_3d(sQ + (lane % NQ) * S::TILE + (lane / NQ) * S::SLAB, &q_map, lane / NQ * 64, q.kvh * p.group,
@@ -474,44 +485,52 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           }
         }
       }
-      if (!ok && lane == 0) s_abort = 1;
+      if (lane == 0) {
+        s_k_issued = (issued + 1) / 2, s_v_issued = issued / 2, s_q_issued = used;
+        if (!ok) s_abort = 1;
+      }
       // the commits that released the last stages have landed before the CTA ends
-      for (int c = max(0, g - STAGES); c < g && ok; ++c)
-        ok = mbar_wait(&bars.k_free[c % STAGES], (c / STAGES) & 1, abort) &&
-             mbar_wait(&bars.v_free[c % STAGES], (c / STAGES) & 1, abort);
-      if (ok && used > 0) ok = mbar_wait(&bars.q_free, (used - 1) & 1, abort);
+#pragma unroll 1
+      for (int c = max(0, g - KS); c < g && ok; ++c) ok = WAITL_(&bars.k_free[c % KS], (c / KS) & 1, abort);
+#pragma unroll 1
+      for (int c = max(0, g - VS); c < g && ok; ++c) ok = WAITL_(&bars.v_free[c % VS], (c / VS) & 1, abort);
+      if (ok && used > 0) ok = WAITL_(&bars.q_free, (used - 1) & 1, abort);
       if (!ok && lane == 0) s_abort = 1;
       __syncwarp();
     } else if (warp == MMA_WARP) {
-      // ---------------- MMA issue (one lane); the whole warp clears values past the length ----------------
-      const uint64_t qd = sw128_desc(smem_u32(sQ), 16), kd = sw128_desc(smem_u32(sK), 16);
-      const uint64_t vd = sw128_desc(smem_u32(sV), S::SLAB);
-      constexpr uint32_t id_s = idesc<T>(BN, false), id_o = idesc<T>(D, true);
+      // ---------------- the products; the whole warp clears values past the length ----------------
       const uint32_t tm = (uint32_t)uniform((int)tmem);
+      const uint32_t qd = uniform(sw128_desc(smem_u32(sQ), 16)), kd = uniform(sw128_desc(smem_u32(sK), 16));
+      const uint32_t vd = uniform(sw128_desc(smem_u32(sV), S::SLAB));
+      constexpr uint32_t id_s = idesc<T>(BN, false), id_o = idesc<T>(D, true);
       bool ok = true;
-      int g = 0, used = 0, done[NQ] = {0, 0};
+      int g = 0, used = 0;
+      uint32_t phase = 0;  // bit i: parity of tile i's next P
+#pragma unroll 1
       for (int n = 0; ok; ++n) {
         Piece q;
         ok = take(n, &q);
         if (!ok || uniform(q.b) < 0) break;
         const int steps = uniform(q.steps);
         if (steps == 0) continue;
-        ok = __all_sync(FULL, mbar_wait(&bars.q_full, used & 1, abort));
+        ok = __all_sync(FULL, WAITM_(&bars.q_full, used & 1, abort));
         if (!ok) break;
         ++used;
         tc_after();
         const int tiles = uniform(q.t0 + tq < q.t1 ? 2 : 1);  // tiles with rows
+#pragma unroll 1
         for (int j = -1; j < steps && ok; ++j) {
           // step j of this piece is the CTA's step g + j
-          const int sv = (g + j + STAGES) % STAGES, sk = (g + j + 1) % STAGES;
+          const int sv = (g + j + VS) % VS, sk = (g + j + 1) % KS;
           const bool more = j + 1 < steps;
-          if (more) ok = mbar_wait(&bars.k_full[sk], ((g + j + 1) / STAGES) & 1, abort);
+          if (more) ok = WAITM_(&bars.k_full[sk], ((g + j + 1) / KS) & 1, abort);
           if (j >= 0) {
-            ok = ok && mbar_wait(&bars.v_full[sv], ((g + j) / STAGES) & 1, abort);
+            ok = ok && WAITM_(&bars.v_full[sv], ((g + j) / VS) & 1, abort);
             // values past the sequence's length (the rest of its last page, pages not loaded) may be anything, and
             // 0 * NaN is NaN: clear them
             const int valid = q.len - (q.j0 + j) * BN;
             if (valid < BN && __all_sync(FULL, ok)) {
+#pragma unroll 1
               for (int e = lane; e < (BN - valid) * (D / 8); e += 32) {
                 const int r = valid + e / (D / 8), c = e % (D / 8);
                 *reinterpret_cast<uint4*>(sV + sv * S::TILE + (c / 8) * S::SLAB + r * 128 + ((c & 7) << 4)) =
@@ -523,34 +542,32 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           }
           ok = __all_sync(FULL, ok);
           if (!ok) break;
-          const uint64_t vb = vd + (uint32_t)((sv * S::TILE) >> 4), kb = kd + (uint32_t)((sk * S::TILE) >> 4);
-#pragma unroll
+          const uint32_t vb = vd + (uint32_t)(sv * (S::TILE >> 4)), kb = kd + (uint32_t)(sk * (S::TILE >> 4));
+          // both tiles unrolled: this warp's own instructions lie on the chain from P to the next S
+#pragma unroll kUnrI
           for (int i = 0; i < NQ; ++i) {
             if (i >= tiles) break;
             if (j >= 0) {
               // the product starts on the first keys' weights while the last ones are being computed
 #pragma unroll
-              for (int e = 0; e < HALVES; ++e) {
-                ok = __all_sync(FULL, wait_<WAITM>(e == HALVES - 1 ? &bars.p_full[i] : &bars.p_half[i], done[i] & 1, abort));
+              for (int e = 0; e < 2; ++e) {
+                ok = __all_sync(FULL, WAITM_(e ? &bars.p_full[i] : &bars.p_most[i], (phase >> i) & 1, abort));
                 if (!ok) break;
                 tc_after();
                 if (elect()) {
 #pragma unroll
-                  for (int k = e * (BN / 16) / HALVES; k < (e + 1) * (BN / 16) / HALVES; ++k)
+                  for (int k = e ? SPLIT : 0; k < (e ? BN / 16 : SPLIT); ++k)
                     umma_ts(tm + O_COL + i * D, tm + S_COL + i * BN + k * 8, vb + (uint32_t)((k * 2048) >> 4), id_o,
                             j > 0 || k > 0);
                 }
                 __syncwarp();
               }
               if (!ok) break;
-              ++done[i];
+              phase ^= 1u << i;
             }
+            // S_i of the next keys: issued behind the product that reads P_i from the same columns. One commit covers both
+            // products: a commit costs the issuing warp as much as several products.
             if (elect()) {
-              if (j >= 0) {
-                commit(&bars.o_full[i]);
-                if (i == tiles - 1) commit(&bars.v_free[sv]);
-              }
-              // S_i of the next keys: issued behind the product that reads P_i from the same columns
               if (more) {
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
@@ -558,10 +575,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                   umma_ss(tm + S_COL + i * BN, qd + ((i * S::TILE + off) >> 4), kb + (off >> 4), id_s, k > 0);
                 }
                 commit(&bars.s_full[i]);
-                if (i == tiles - 1) {
-                  commit(&bars.k_free[sk]);
-                  if (j + 2 == steps) commit(&bars.q_free);
-                }
+              } else {
+                commit(&bars.o_full[i]);
               }
             }
             __syncwarp();
@@ -577,97 +592,87 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
     }
   } else {
-    // ---------------- softmax: half a row per thread ----------------
+    // ---------------- softmax: one row per thread ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
-    constexpr int COLS = BN / PARTS, DCOLS = D / PARTS;  // this thread's keys of a step, its values of the output
-    const int i = warp / (4 * PARTS), h = (warp >> 2) % PARTS, quad = warp & 3;
+    const int i = warp >> 2, quad = warp & 3;
     const int rr = quad * 32 + lane;
     const int my_tok = i * tq + rr / p.group, my_head = rr % p.group;
     const bool my_row = rr < tq * p.group;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t s_at = lane_base + S_COL + i * BN, o_at = lane_base + O_COL + i * D + h * DCOLS;
+    const uint32_t s_at = lane_base + S_COL + i * BN, o_at = lane_base + O_COL + i * D;
     const float c_log2 = CAP ? 1.0f : p.scale * LOG2E;
     const float cap_in = CAP ? 2.0f * LOG2E * p.scale / p.softcap : 0.0f, cap_out = p.softcap * LOG2E;
     bool ok = true;
-    int seen = 0;   // steps so far
-    int swaps = 0;  // exchanges so far
-    // The other half's value of this row (warp-collective; false once a wait gave up). Two buffers: a warp that is one
-    // exchange ahead writes the other one.
-    auto swap = [&](float mine, float* other) -> bool {
-      s_swap[swaps & 1][i][h][rr] = mine;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.pair[i][quad]);
-      const bool got = __all_sync(FULL, mbar_wait(&bars.pair[i][quad], swaps & 1, abort));
-      *other = s_swap[swaps & 1][i][h ^ 1][rr];
-      ++swaps;
-      return got;
-    };
+    int seen = 0;           // this tile's steps so far
+    int g = 0, pieces = 0;  // the CTA's steps so far, this tile's pieces
+#pragma unroll 1
     for (int n = 0; ok; ++n) {
       Piece q;
       ok = take(n, &q);
       if (!ok || q.b < 0) break;
       const int first = q.t0 + i * tq;  // first token of the tile
-      if (first >= q.t1) continue;      // no rows in this tile
+      if (first >= q.t1) {              // no rows in this tile
+        g += q.steps;
+        continue;
+      }
+      // the last tile with rows, whose products are issued last, lets go of Q, K and V for both
+      const bool frees = (i == NQ - 1 || first + tq >= q.t1) && quad == 0 && lane == 0;
       const int tok = q.t0 + my_tok;
       const bool live = my_row && tok < q.t1;
       const int pos = q.past + tok;  // this row sees keys (pos - window, pos]
       const int key_lo = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-      float m = -INFINITY, l = 0.0f;  // reference in units of log2, sum of this half's weights
+      float m = -INFINITY, l = 0.0f;  // reference in units of log2, sum of weights
+#pragma unroll 1
       for (int j = 0; j < q.steps; ++j, ++seen) {
-        ok = wait_<WAITS>(&bars.s_full[i], seen & 1, abort);
-        // the product with the previous step's P has been issued before this S, and finished: its phase is taken
-        // note of here, and O may be rescaled
-        if (ok && j > 0) ok = mbar_wait(&bars.o_full[i], (seen - 1) & 1, abort);
+        ok = WAITS_(&bars.s_full[i], seen & 1, abort);
         ok = __all_sync(FULL, ok);
         if (!ok) break;
+        // S complete means that every product issued before it is: the previous step's with P (O may be rescaled), and
+        // the reads of its V and of this K
+        if (frees) {
+          mbar_arrive(&bars.k_free[(g + j) % KS]);
+          if (j > 0) mbar_arrive(&bars.v_free[(g + j - 1) % VS]);
+          if (j == q.steps - 1) mbar_arrive(&bars.q_free);
+        }
         tc_after();
-        uint32_t r[COLS];
+        uint32_t r[BN];
 #pragma unroll
-        for (int c = 0; c < COLS / 32; ++c)
-          tmem_ld32(s_at + h * COLS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+        for (int c = 0; c < BN / 32; ++c)
+          tmem_ld32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
         tmem_wait_ld();
         if (CAP) {
           // softcap * tanh(x) = softcap * (1 - 2 / (e^2x + 1)), absolute error about 1e-7 of the cap
 #pragma unroll
-          for (int k = 0; k < COLS; ++k)
+          for (int k = 0; k < BN; ++k)
             r[k] = __float_as_uint(cap_out - __fdividef(2.0f * cap_out, ex2(__uint_as_float(r[k]) * cap_in) + 1.0f));
         }
         const int base = (q.j0 + j) * BN;
         // keys that every live row of the tile sees need no mask
         const bool masked =
             base + BN - 1 > q.past + first || (p.window > 0 && base <= q.past + min(q.t1, first + tq) - 1 - p.window);
-        if (masked) {
-          const int from = key_lo - base - h * COLS;
+        if (EXPECT ? __builtin_expect(masked, 0) : masked) {
+          const int from = key_lo - base;
           const unsigned width = (unsigned)max(0, pos + 1 - key_lo);  // columns [from, from + width)
 #pragma unroll
-          for (int k = 0; k < COLS; ++k)
+          for (int k = 0; k < BN; ++k)
             if ((unsigned)(k - from) >= width) r[k] = 0xff800000u;
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < COLS; k += 8)
+        for (int k = 0; k < BN; k += 8)
 #pragma unroll
           for (int a = 0; a < 4; ++a)
             mx[a] = fmaxf(fmaxf(mx[a], __uint_as_float(r[k + 2 * a])), __uint_as_float(r[k + 2 * a + 1]));
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), top2;
-        // both halves have read S once the exchange is done: P may be written over it
-        if (PARTS == 2) {
-          tc_before();
-          ok = swap(top, &top2);
-          if (!ok) break;
-          tc_after();
-          top = fmaxf(top, top2);
-        }
-        top *= c_log2;  // scale > 0
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c_log2;  // scale > 0
         const bool grow = top > m + RESCALE;  // also the first finite maximum
-        if (__any_sync(FULL, grow)) {
+        if (EXPECT ? __builtin_expect(__any_sync(FULL, grow), 0) : __any_sync(FULL, grow)) {
           const float mn = grow ? top : m;
           const float f = grow ? ex2(m - mn) : 1.0f;
           m = mn;
           l *= f;
           if (j > 0) {
 #pragma unroll 1
-            for (int c = 0; c < DCOLS / 16; ++c) {
+            for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
               tmem_ld16u(o_at + c * 16, o);
               tmem_wait_ld();
@@ -678,53 +683,57 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-        // Of every eight pairs of weights POLY are computed by arithmetic, the others by the exponential unit, which
-        // alone would take as long as both products. A masked step uses the unit alone: its -inf must give 0.
-        float2 sum = make_float2(0.0f, 0.0f), sum1 = sum;
-        auto weights = [&](auto mixed) {
+        // The weights, 32 columns at a time. The exponential unit sets the pace (a pair per 16 clocks): its instructions are
+        // kept in program order, and the packing and summing of a pair follow AHEAD pairs behind, so that no chunk waits for
+        // the unit's latency.
+        constexpr int PAIRS = BN / 2, AHEAD = 4;
+        float2 sum = make_float2(0.0f, 0.0f);
+        float2 x[PAIRS];
+        uint32_t w[16];
 #pragma unroll
-          for (int c = 0; c < COLS / 32; ++c) {
-            uint32_t w[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float2 x = fma2(make_float2(__uint_as_float(r[c * 32 + 2 * k]), __uint_as_float(r[c * 32 + 2 * k + 1])),
-                              make_float2(c_log2, c_log2), make_float2(-ref, -ref));
-              if (decltype(mixed)::value && (k & 7) < POLY) x = exp2_poly(x);
-              else x = make_float2(ex2(x.x), ex2(x.y));
-              if (SUMS == 2 && (k & 1)) sum1 = add2(sum1, x); else sum = add2(sum, x);
-              w[k] = Elem<T>::pack(x.x, x.y);
-            }
-            tmem_st16(s_at + h * (COLS / 2) + c * 16, w);
-            if (HALVES == 2 && c == COLS / 64 - 1) {
+        for (int k = 0; k < PAIRS + AHEAD; ++k) {
+          if (k < PAIRS) {
+            x[k] = fma2(make_float2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), make_float2(c_log2, c_log2),
+                        make_float2(-ref, -ref));
+            x[k].x = EXV ? ex2_ordered(x[k].x) : ex2(x[k].x);
+            x[k].y = EXV ? ex2_ordered(x[k].y) : ex2(x[k].y);
+          }
+          const int e = k - AHEAD;
+          if (e < 0) continue;
+          sum = add2(sum, x[e]);
+          w[e % 16] = Elem<T>::pack(x[e].x, x[e].y);
+          if (e % 16 == 15) {
+            tmem_st16(s_at + e / 16 * 16, w);  // columns of S, all of which this row has read
+            if (e == SPLIT * 8 - 1) {
               tmem_wait_st();
               tc_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(&bars.p_half[i]);
+              if (lane == 0) mbar_arrive(&bars.p_most[i]);
             }
           }
-        };
-        if (masked) weights(std::false_type());
-        else weights(std::true_type());
-        l += (sum.x + sum1.x) + (sum.y + sum1.y);
+        }
+        l += sum.x + sum.y;
         tmem_wait_st();
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.p_full[i]);
       }
-      if (ok && q.steps > 0) ok = __all_sync(FULL, mbar_wait(&bars.o_full[i], (seen - 1) & 1, abort));
-      float l2 = 0.0f;
-      if (ok && PARTS == 2) ok = swap(l, &l2);
+      if (ok && q.steps > 0) {
+        ok = __all_sync(FULL, WAITS_(&bars.o_full[i], pieces & 1, abort));
+        ++pieces;
+        if (ok && frees) mbar_arrive(&bars.v_free[(g + q.steps - 1) % VS]);
+      }
       if (!ok) break;
+      g += q.steps;
       tc_after();
-      l = h ? l2 + l : l + l2;  // one order for both halves
       // ---- the piece's rows: out, or into the workspace ----
       const int64_t row = (int64_t)(q.row0 + tok) * p.heads + q.kvh * p.group + my_head;
-      T* dst = static_cast<T*>(p.y) + row * D + h * DCOLS;
+      T* dst = static_cast<T*>(p.y) + row * D;
       const int64_t slot = (int64_t)q.item * q.cut * NQ + i;  // piece k of this tile at slot + k * NQ
-      float4* part = p.partial + (slot * (D / 4) + h * (DCOLS / 4)) * BM + rr;  // [D / 4][BM] of a slot
+      float4* part = p.partial + slot * (D / 4) * BM + rr;  // [D / 4][BM] of a slot
       const float inv = q.cut > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll 1
-      for (int c = 0; c < DCOLS / 16; ++c) {
+      for (int c = 0; c < D / 16; ++c) {
         uint32_t o[16];
         if (q.steps > 0) {
           tmem_ld16u(o_at + c * 16, o);
@@ -747,18 +756,18 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
       }
       if (q.cut == 1) {
-        if (h == 0 && live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
+        if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
         continue;
       }
-      // ---- the last of the item's pieces to arrive joins them in order, each warp its own rows and values ----
-      float2* ml = p.partial_ml + (slot * PARTS + h) * BM + rr;  // piece k at k * NQ * PARTS * BM
-      constexpr int MLS = NQ * PARTS * BM;
+      // ---- the last of the item's pieces to arrive joins them in order, each warp its own rows ----
+      float2* ml = p.partial_ml + slot * BM + rr;  // piece k at k * NQ * BM
+      constexpr int MLS = NQ * BM;
       __stcg(ml + q.k * MLS, make_float2(m, l));
       __threadfence();
       __syncwarp();
       int last = 0;
       if (lane == 0) {
-        int32_t* cnt = p.counters + ((q.item * NQ + i) * PARTS + h) * 4 + quad;
+        int32_t* cnt = p.counters + (q.item * NQ + i) * 4 + quad;
         last = atomicAdd(cnt, 1) == q.cut - 1;
         if (last) *cnt = 0;  // ready for the next call
       }
@@ -775,7 +784,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
         const float il = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll 1
-        for (int c = 0; c < DCOLS / 8; ++c) {
+        for (int c = 0; c < D / 8; ++c) {
           float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
 #pragma unroll 4
           for (int k = 0; k < q.cut; ++k) {
@@ -792,7 +801,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                 make_uint4(Elem<T>::pack(o[0].x * il, o[0].y * il), Elem<T>::pack(o[0].z * il, o[0].w * il),
                            Elem<T>::pack(o[1].x * il, o[1].y * il), Elem<T>::pack(o[1].z * il, o[1].w * il));
         }
-        if (h == 0 && live && p.lse) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
+        if (live && p.lse) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
       }
     }
     if (!ok && lane == 0) s_abort = 1;
@@ -802,10 +811,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     if (s_abort) {
       if (s_q_issued) (void)mbar_wait(&bars.q_full, (s_q_issued - 1) & 1, nullptr);
       // the copies still in flight land before the CTA's shared memory goes
-      for (int j = max(0, s_k_issued - STAGES); j < s_k_issued; ++j)
-        (void)mbar_wait(&bars.k_full[j % STAGES], (j / STAGES) & 1, nullptr);
-      for (int j = max(0, s_v_issued - STAGES); j < s_v_issued; ++j)
-        (void)mbar_wait(&bars.v_full[j % STAGES], (j / STAGES) & 1, nullptr);
+#pragma unroll 1
+      for (int j = max(0, s_k_issued - KS); j < s_k_issued; ++j)
+        (void)mbar_wait(&bars.k_full[j % KS], (j / KS) & 1, nullptr);
+#pragma unroll 1
+      for (int j = max(0, s_v_issued - VS); j < s_v_issued; ++j)
+        (void)mbar_wait(&bars.v_full[j % VS], (j / VS) & 1, nullptr);
       atomicExch(p.err, (int)MOE_ERR_TIMEOUT);
     }
     // the last CTA to leave puts the counter of pieces back for the next call
@@ -869,8 +880,8 @@ moe_status launch_prefill(const moe_attn& a, const PrefillParams& p, cudaStream_
 }
 
 size_t prefill_partial_bytes(const moe_attn& a) { return (size_t)2 * a.sms * NQ * BM * a.d.head_dim * sizeof(float); }
-size_t prefill_ml_bytes(const moe_attn& a) { return (size_t)2 * a.sms * NQ * PARTS * BM * sizeof(float2); }
-size_t prefill_counters(const moe_attn& a) { return (size_t)2 * a.sms * NQ * PARTS * 4; }
+size_t prefill_ml_bytes(const moe_attn& a) { return (size_t)2 * a.sms * NQ * BM * sizeof(float2); }
+size_t prefill_counters(const moe_attn& a) { return (size_t)2 * a.sms * NQ * 4; }
 
 moe_status make_page_tmap(CUtensorMap* map, int dtype, const void* pool, int head_dim, int page_size, int kv_heads,
                           int64_t num_pages, int64_t page_stride) {
