@@ -10,8 +10,8 @@
 // results are joined by the last to arrive, in the pieces' order. The kernel is persistent: one CTA per SM takes
 // pieces from a counter, those with the most keys first, and runs its roles over them without a break:
 //   * one warp takes the pieces, hands them to the other roles through a small ring, and loads by TMA (SWIZZLE_128B): Q
-//     (64 values x the group's heads x a tile's tokens per box) once the piece before has issued its last scores, K and V
-//     pages (64 values x a page's tokens per box) into rings of STAGES tiles;
+//     (64 values x the group's heads x a tile's tokens per box) once the piece before has issued its last scores, and K
+//     (64 values x a page's tokens per box) into a ring of STAGES tiles; another warp loads V likewise;
 //   * one thread issues S_i = Q_i K^T (128 x 128, f32 in tensor memory) and O_i += P_i V, alternating the
 //     two tiles, so the tensor cores work on one tile while the other's softmax runs;
 //   * four warps per tile hold one row per thread: maximum, exponentials and sum in f32, P rounded to the
@@ -30,66 +30,22 @@
 namespace moe {
 namespace attn {
 
-#ifndef LEAN
-#define LEAN 2
-#endif
-#if LEAN & 1
-#define WAITM_ wait_poll
-#else
-#define WAITM_ mbar_wait
-#endif
-#if LEAN & 2
-#define WAITS_ wait_poll
-#else
-#define WAITS_ mbar_wait
-#endif
-#if LEAN & 4
-#define WAITL_ wait_poll
-#else
-#define WAITL_ mbar_wait
-#endif
-#ifndef ROLLI
-#define ROLLI 0
-#endif
-#ifndef EXPECT
-#define EXPECT 1
-#endif
-#ifndef EXV
-#define EXV 1
-#endif
-#ifndef SPLIT
-#define SPLIT 4
-#endif
-constexpr int kUnrI = ROLLI ? 1 : 2;
 constexpr int BM = 128;      // rows of a tile
 constexpr int BN = 128;      // keys of a tile
 constexpr int NQ = 2;        // tiles of a CTA
-#ifndef KST
-#define KST 3
-#endif
-#ifndef VST
-#define VST 2
-#endif
-constexpr int KS = KST, VS = VST;  // K tiles and V tiles in flight
-#ifndef EXPECT
-#define EXPECT 1
-#endif
-#ifndef EXV
-#define EXV 1
-#endif
-#ifndef SPLIT
-#define SPLIT 6
-#endif
+constexpr int STAGES = 2;    // K tiles and V tiles in flight
 constexpr int SOFTMAX_WARPS = 4 * NQ;
 constexpr int MMA_WARP = SOFTMAX_WARPS;
 constexpr int LOAD_WARP = SOFTMAX_WARPS + 1;
-constexpr int PF_THREADS = (SOFTMAX_WARPS + 4) * 32;  // the last two warps only give up their registers
+constexpr int V_WARP = SOFTMAX_WARPS + 2;
+constexpr int PF_THREADS = (SOFTMAX_WARPS + 4) * 32;  // the last warp only gives up its registers
 // registers per thread: 168 at launch (384 threads), shared out anew: 2 x 216 + 72 = 3 x 168
 constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 72;
 constexpr int RING = 4;              // pieces handed out ahead
-constexpr int CONSUMERS = SOFTMAX_WARPS + 1;
+constexpr int CONSUMERS = SOFTMAX_WARPS + 2;
 constexpr int MAX_CUT = 16;          // pieces of an item
 constexpr int PIECE_COST = 3;        // what a piece costs beside its steps, in steps (Q, epilogue, join)
+constexpr int MOST = BN / 32;        // products of P V (of BN / 16) that start before the rest of P is there
 constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0;            // S_i / P_i at columns BN * i
 constexpr int O_COL = NQ * BN;      // O_i at columns O_COL + D * i
@@ -251,11 +207,11 @@ template <int D>
 struct PfShape {
   static constexpr int SLAB = BN * 128;            // 64 values x 128 rows
   static constexpr int TILE = (D / 64) * SLAB;     // a Q, K or V tile
-  static constexpr int BYTES = (NQ + KS + VS) * TILE + 1024;
+  static constexpr int BYTES = (NQ + 2 * STAGES) * TILE + 1024;
 };
 
 struct Bars {
-  uint64_t k_full[KS], v_full[VS], k_free[KS], v_free[VS];
+  uint64_t k_full[STAGES], v_full[STAGES], k_free[STAGES], v_free[STAGES];
   uint64_t s_full[NQ], p_most[NQ], p_full[NQ], o_full[NQ], q_full, q_free, item_full[RING], item_free[RING], drained;
 };
 
@@ -361,7 +317,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* sQ = smem;
   unsigned char* sK = sQ + NQ * S::TILE;
-  unsigned char* sV = sK + KS * S::TILE;
+  unsigned char* sV = sK + STAGES * S::TILE;
   __shared__ Bars bars;
   __shared__ Piece s_items[RING];
   __shared__ uint32_t s_tmem;
@@ -372,12 +328,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   const int tq = BM / p.group, span = NQ * tq;  // tokens of a tile, of an item
 
   if (tid == 0) {
-    for (int i = 0; i < KS; ++i) {
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&bars.k_full[i], 1);
-      mbar_init(&bars.k_free[i], 1);
-    }
-    for (int i = 0; i < VS; ++i) {
       mbar_init(&bars.v_full[i], 1);
+      mbar_init(&bars.k_free[i], 1);
       mbar_init(&bars.v_free[i], 1);
     }
     for (int i = 0; i < NQ; ++i) {
@@ -417,7 +371,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   // The n-th piece for a consuming warp; false once a wait gave up. Lane 0 releases the slot.
   auto take = [&](int n, Piece* q) -> bool {
     const int slot = n % RING;
-    const bool ok = __all_sync(FULL, WAITL_(&bars.item_full[slot], (n / RING) & 1, abort));
+    const bool ok = __all_sync(FULL, mbar_wait(&bars.item_full[slot], (n / RING) & 1, abort));
     if (!ok) return false;
     *q = s_items[slot];
     __syncwarp();
@@ -427,34 +381,46 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 
   if (warp >= SOFTMAX_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-    if (warp == LOAD_WARP) {
-      // ---------------- pieces, and their K and V tiles: each lane loads the boxes of its pages ----------------
-      const Batch batch = read_batch(p, span, lane, gridDim.x);
+    if (warp == LOAD_WARP || warp == V_WARP) {
+      // One warp takes the pieces and loads their Q and K tiles, another their V tiles: with 16-token pages a tile is 16
+      // boxes, one lane each, and they are issued one after the other.
+      const bool is_v = warp == V_WARP;
       const int box_rows = 1 << p.page_shift;
       const int pages = BN >> p.page_shift;  // per tile
-      const int half = lane / pages;  // this lane's 64-value half and page: at most 16 boxes
+      const int half = lane / pages;         // this lane's 64-value half and page: at most 16 boxes
       const int my = half < D / 64 ? lane % pages : pages;
       const int box_bytes = box_rows * (D / 64) * 128;
-      unsigned char* dst = sK + half * S::SLAB + my * box_rows * 128;
-      int g = 0, used = 0, w = blockIdx.x, issued = 0;  // K and V tiles, in turn
+      unsigned char* dst = (is_v ? sV : sK) + half * S::SLAB + my * box_rows * 128;
+      uint64_t* full = is_v ? bars.v_full : bars.k_full;
+      uint64_t* free_ = is_v ? bars.v_free : bars.k_free;
+      const CUtensorMap* map = is_v ? &v_map : &k_map;
+      Batch batch;
+      if (!is_v) batch = read_batch(p, span, lane, gridDim.x);
+      int g = 0, used = 0, w = blockIdx.x;
       bool ok = true;
 #pragma unroll 1
       for (int n = 0; ok; ++n) {
-        const Piece q = piece_of(p, batch, w, span, lane);
-        const int slot = n % RING;
-        ok = __all_sync(FULL, n < RING || WAITL_(&bars.item_free[slot], ((n / RING) - 1) & 1, abort));
-        if (!ok) break;
-        if (lane == 0) {
-          s_items[slot] = q;
-          mbar_arrive(&bars.item_full[slot]);
-          if (q.b >= 0) w = gridDim.x + atomicAdd(p.work, 1);
+        Piece q;
+        if (is_v) {
+          ok = take(n, &q);
+          if (!ok) break;
+        } else {
+          q = piece_of(p, batch, w, span, lane);
+          const int slot = n % RING;
+          ok = __all_sync(FULL, n < RING || mbar_wait(&bars.item_free[slot], ((n / RING) - 1) & 1, abort));
+          if (!ok) break;
+          if (lane == 0) {
+            s_items[slot] = q;
+            mbar_arrive(&bars.item_full[slot]);
+            if (q.b >= 0) w = gridDim.x + atomicAdd(p.work, 1);
+          }
+          w = __shfl_sync(FULL, w, 0);
         }
         if (q.b < 0) break;
-        w = __shfl_sync(FULL, w, 0);
         const int32_t* table = p.page_table + (int64_t)q.b * p.max_pages + my;
 #pragma unroll 1
-        for (int j = 0; j < q.steps && ok; ++j, ++g) {
-          const int base = (q.j0 + j) * BN;
+        for (int j = 0; j < q.steps; ++j, ++g) {
+          const int base = (q.j0 + j) * BN, st = g % STAGES;
           const int live = min(pages, (q.len - base + box_rows - 1) >> p.page_shift);  // pages that hold tokens
           const bool on = my < live;
           int page = on ? __ldg(table + (base >> p.page_shift)) : 0;
@@ -462,39 +428,39 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             latch(p.err, MOE_ERR_BAD_IDS);
             page = p.num_pages;  // out of the map: the box reads as zeros
           }
-#pragma unroll 1
-          for (int kv = 0; kv < 2; ++kv) {
-            const int n_st = kv ? VS : KS, st = g % n_st;
-            uint64_t* full = kv ? &bars.v_full[st] : &bars.k_full[st];
-            ok = __all_sync(FULL, WAITL_(kv ? &bars.v_free[st] : &bars.k_free[st], ((g / n_st) & 1) ^ 1, abort));
-            if (!ok) break;
-            if (lane == 0) mbar_expect_tx(full, (uint32_t)(live * box_bytes));
-            __syncwarp();
-            if (on) tma_load_4d(dst + (kv * KS + st) * S::TILE, kv ? &v_map : &k_map, half * 64, 0, q.kvh, page, full);
-            ++issued;
-            if (kv + j == 0) {  // Q behind the first K tile: its place is the last to come free
-              ok = __all_sync(FULL, WAITL_(&bars.q_free, (used & 1) ^ 1, abort));
-              if (!ok) break;
-              ++used;
-              if (lane == 0) mbar_expect_tx(&bars.q_full, (uint32_t)(NQ * (D / 64) * tq * p.group * 128));
-              __syncwarp();
-              if (lane < NQ * (D / 64))
-                tma_load_3d(sQ + (lane % NQ) * S::TILE + (lane / NQ) * S::SLAB, &q_map, lane / NQ * 64, q.kvh * p.group,
-                            q.row0 + q.t0 + (lane % NQ) * tq, &bars.q_full);
+          ok = __all_sync(FULL, mbar_wait(&free_[st], ((g / STAGES) & 1) ^ 1, abort));
+          if (!ok) break;
+          if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)(live * box_bytes));
+          __syncwarp();
+          if (on) tma_load_4d(dst + st * S::TILE, map, half * 64, 0, q.kvh, page, &full[st]);
+          if (j == 0 && !is_v) {  // Q behind the first K tile: its place is the last to come free
+            ok = __all_sync(FULL, mbar_wait(&bars.q_free, (used & 1) ^ 1, abort));
+            if (!ok) {
+              ++g;
+              break;
             }
+            ++used;
+            if (lane == 0) mbar_expect_tx(&bars.q_full, (uint32_t)(NQ * (D / 64) * tq * p.group * 128));
+            __syncwarp();
+            if (lane < NQ * (D / 64))
+              tma_load_3d(sQ + (lane % NQ) * S::TILE + (lane / NQ) * S::SLAB, &q_map, lane / NQ * 64, q.kvh * p.group,
+                          q.row0 + q.t0 + (lane % NQ) * tq, &bars.q_full);
           }
         }
       }
       if (lane == 0) {
-        s_k_issued = (issued + 1) / 2, s_v_issued = issued / 2, s_q_issued = used;
+        if (is_v) {
+          s_v_issued = g;
+        } else {
+          s_k_issued = g;
+          s_q_issued = used;
+        }
         if (!ok) s_abort = 1;
       }
-      // the commits that released the last stages have landed before the CTA ends
+      // the releases of the last stages have landed before the CTA ends
 #pragma unroll 1
-      for (int c = max(0, g - KS); c < g && ok; ++c) ok = WAITL_(&bars.k_free[c % KS], (c / KS) & 1, abort);
-#pragma unroll 1
-      for (int c = max(0, g - VS); c < g && ok; ++c) ok = WAITL_(&bars.v_free[c % VS], (c / VS) & 1, abort);
-      if (ok && used > 0) ok = WAITL_(&bars.q_free, (used - 1) & 1, abort);
+      for (int c = max(0, g - STAGES); c < g && ok; ++c) ok = mbar_wait(&free_[c % STAGES], (c / STAGES) & 1, abort);
+      if (ok && used > 0) ok = mbar_wait(&bars.q_free, (used - 1) & 1, abort);
       if (!ok && lane == 0) s_abort = 1;
       __syncwarp();
     } else if (warp == MMA_WARP) {
@@ -513,7 +479,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (!ok || uniform(q.b) < 0) break;
         const int steps = uniform(q.steps);
         if (steps == 0) continue;
-        ok = __all_sync(FULL, WAITM_(&bars.q_full, used & 1, abort));
+        ok = __all_sync(FULL, mbar_wait(&bars.q_full, used & 1, abort));
         if (!ok) break;
         ++used;
         tc_after();
@@ -521,11 +487,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 #pragma unroll 1
         for (int j = -1; j < steps && ok; ++j) {
           // step j of this piece is the CTA's step g + j
-          const int sv = (g + j + VS) % VS, sk = (g + j + 1) % KS;
+          const int sv = (g + j + STAGES) % STAGES, sk = (g + j + 1) % STAGES;
           const bool more = j + 1 < steps;
-          if (more) ok = WAITM_(&bars.k_full[sk], ((g + j + 1) / KS) & 1, abort);
+          if (more) ok = mbar_wait(&bars.k_full[sk], ((g + j + 1) / STAGES) & 1, abort);
           if (j >= 0) {
-            ok = ok && WAITM_(&bars.v_full[sv], ((g + j) / VS) & 1, abort);
+            ok = ok && mbar_wait(&bars.v_full[sv], ((g + j) / STAGES) & 1, abort);
             // values past the sequence's length (the rest of its last page, pages not loaded) may be anything, and
             // 0 * NaN is NaN: clear them
             const int valid = q.len - (q.j0 + j) * BN;
@@ -544,19 +510,19 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           if (!ok) break;
           const uint32_t vb = vd + (uint32_t)(sv * (S::TILE >> 4)), kb = kd + (uint32_t)(sk * (S::TILE >> 4));
           // both tiles unrolled: this warp's own instructions lie on the chain from P to the next S
-#pragma unroll kUnrI
+#pragma unroll
           for (int i = 0; i < NQ; ++i) {
             if (i >= tiles) break;
             if (j >= 0) {
               // the product starts on the first keys' weights while the last ones are being computed
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                ok = __all_sync(FULL, WAITM_(e ? &bars.p_full[i] : &bars.p_most[i], (phase >> i) & 1, abort));
+                ok = __all_sync(FULL, mbar_wait(e ? &bars.p_full[i] : &bars.p_most[i], (phase >> i) & 1, abort));
                 if (!ok) break;
                 tc_after();
                 if (elect()) {
 #pragma unroll
-                  for (int k = e ? SPLIT : 0; k < (e ? BN / 16 : SPLIT); ++k)
+                  for (int k = e ? MOST : 0; k < (e ? BN / 16 : MOST); ++k)
                     umma_ts(tm + O_COL + i * D, tm + S_COL + i * BN + k * 8, vb + (uint32_t)((k * 2048) >> 4), id_o,
                             j > 0 || k > 0);
                 }
@@ -624,14 +590,14 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       float m = -INFINITY, l = 0.0f;  // reference in units of log2, sum of weights
 #pragma unroll 1
       for (int j = 0; j < q.steps; ++j, ++seen) {
-        ok = WAITS_(&bars.s_full[i], seen & 1, abort);
+        ok = wait_poll(&bars.s_full[i], seen & 1, abort);
         ok = __all_sync(FULL, ok);
         if (!ok) break;
         // S complete means that every product issued before it is: the previous step's with P (O may be rescaled), and
         // the reads of its V and of this K
         if (frees) {
-          mbar_arrive(&bars.k_free[(g + j) % KS]);
-          if (j > 0) mbar_arrive(&bars.v_free[(g + j - 1) % VS]);
+          mbar_arrive(&bars.k_free[(g + j) % STAGES]);
+          if (j > 0) mbar_arrive(&bars.v_free[(g + j - 1) % STAGES]);
           if (j == q.steps - 1) mbar_arrive(&bars.q_free);
         }
         tc_after();
@@ -650,7 +616,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         // keys that every live row of the tile sees need no mask
         const bool masked =
             base + BN - 1 > q.past + first || (p.window > 0 && base <= q.past + min(q.t1, first + tq) - 1 - p.window);
-        if (EXPECT ? __builtin_expect(masked, 0) : masked) {
+        if (__builtin_expect(masked, 0)) {
           const int from = key_lo - base;
           const unsigned width = (unsigned)max(0, pos + 1 - key_lo);  // columns [from, from + width)
 #pragma unroll
@@ -665,7 +631,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             mx[a] = fmaxf(fmaxf(mx[a], __uint_as_float(r[k + 2 * a])), __uint_as_float(r[k + 2 * a + 1]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c_log2;  // scale > 0
         const bool grow = top > m + RESCALE;  // also the first finite maximum
-        if (EXPECT ? __builtin_expect(__any_sync(FULL, grow), 0) : __any_sync(FULL, grow)) {
+        if (__builtin_expect(__any_sync(FULL, grow), 0)) {
           const float mn = grow ? top : m;
           const float f = grow ? ex2(m - mn) : 1.0f;
           m = mn;
@@ -695,8 +661,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           if (k < PAIRS) {
             x[k] = fma2(make_float2(__uint_as_float(r[2 * k]), __uint_as_float(r[2 * k + 1])), make_float2(c_log2, c_log2),
                         make_float2(-ref, -ref));
-            x[k].x = EXV ? ex2_ordered(x[k].x) : ex2(x[k].x);
-            x[k].y = EXV ? ex2_ordered(x[k].y) : ex2(x[k].y);
+            x[k].x = ex2_ordered(x[k].x);
+            x[k].y = ex2_ordered(x[k].y);
           }
           const int e = k - AHEAD;
           if (e < 0) continue;
@@ -704,7 +670,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           w[e % 16] = Elem<T>::pack(x[e].x, x[e].y);
           if (e % 16 == 15) {
             tmem_st16(s_at + e / 16 * 16, w);  // columns of S, all of which this row has read
-            if (e == SPLIT * 8 - 1) {
+            if (e == MOST * 8 - 1) {
               tmem_wait_st();
               tc_before();
               __syncwarp();
@@ -719,9 +685,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (lane == 0) mbar_arrive(&bars.p_full[i]);
       }
       if (ok && q.steps > 0) {
-        ok = __all_sync(FULL, WAITS_(&bars.o_full[i], pieces & 1, abort));
+        ok = __all_sync(FULL, wait_poll(&bars.o_full[i], pieces & 1, abort));
         ++pieces;
-        if (ok && frees) mbar_arrive(&bars.v_free[(g + q.steps - 1) % VS]);
+        if (ok && frees) mbar_arrive(&bars.v_free[(g + q.steps - 1) % STAGES]);
       }
       if (!ok) break;
       g += q.steps;
@@ -812,11 +778,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       if (s_q_issued) (void)mbar_wait(&bars.q_full, (s_q_issued - 1) & 1, nullptr);
       // the copies still in flight land before the CTA's shared memory goes
 #pragma unroll 1
-      for (int j = max(0, s_k_issued - KS); j < s_k_issued; ++j)
-        (void)mbar_wait(&bars.k_full[j % KS], (j / KS) & 1, nullptr);
+      for (int j = max(0, s_k_issued - STAGES); j < s_k_issued; ++j)
+        (void)mbar_wait(&bars.k_full[j % STAGES], (j / STAGES) & 1, nullptr);
 #pragma unroll 1
-      for (int j = max(0, s_v_issued - VS); j < s_v_issued; ++j)
-        (void)mbar_wait(&bars.v_full[j % VS], (j / VS) & 1, nullptr);
+      for (int j = max(0, s_v_issued - STAGES); j < s_v_issued; ++j)
+        (void)mbar_wait(&bars.v_full[j % STAGES], (j / STAGES) & 1, nullptr);
       atomicExch(p.err, (int)MOE_ERR_TIMEOUT);
     }
     // the last CTA to leave puts the counter of pieces back for the next call
