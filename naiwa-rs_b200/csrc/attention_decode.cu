@@ -135,9 +135,14 @@ struct Split {
   int rows;
 };
 
-// Counts an arrival; true for the last of `need`, which leaves the counter at zero for the next call.
+// Counts an arrival of the whole CTA (after a barrier); true for the last of `need`, which leaves the counter at zero for
+// the next call. Release and acquire: what the CTA wrote before the barrier is visible to the last one's threads behind
+// their next barrier.
 __device__ __forceinline__ bool arrive(int32_t* counter, int need) {
-  const bool last = atomicAdd(counter, 1) == need - 1;
+  int before;
+  __threadfence();
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  const bool last = before == need - 1;
   if (last) *counter = 0;
   return last;
 }
@@ -149,48 +154,67 @@ __device__ __forceinline__ bool arrive_first(const DecodeParams& p, const Split&
 }
 
 // Joins parts k0, k0 + step, .. (n of them, in this order; ml: their maxima and sums) into the output, or, with to_ml,
-// into part k0's slot of the workspace. A chunk's loads are all in flight together.
+// into part k0's slot of the workspace. A join is one CTA's work behind everything else, so its time is the number of
+// dependent trips to L2: all of a thread's loads of JOIN parts are in flight together.
 template <class T, int D, int ROWS>
 __device__ __forceinline__ void join(const DecodeParams& p, const Split& sp, int k0, int step, int n, const float2* ml,
                                      float2* to_ml) {
-  for (int e = threadIdx.x; e < sp.rows * (D / 4); e += THREADS) {
-    const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-    float M = -INFINITY, L = 0.0f;
-    float4 o = make_float4(0, 0, 0, 0);
-    for (int k = 0; k < n; k += JOIN) {
-      float2 s[JOIN];
-      float4 v[JOIN];
+  constexpr int EACH = 8 * (D / 4) / THREADS;  // values (of 4) of 8 rows per thread
+  static_assert(EACH >= 1 && 8 * (D / 4) % THREADS == 0, "whole passes");
+#pragma unroll 1
+  for (int r0 = 0; r0 < sp.rows; r0 += 8) {
+    float M[EACH], L[EACH];
+    float4 o[EACH];
 #pragma unroll
-      for (int i = 0; i < JOIN; ++i) {
-        s[i] = make_float2(-INFINITY, 0.0f);
-        v[i] = make_float4(0, 0, 0, 0);
-        if (k + i < n) {
-          const int64_t at = (int64_t)part_slot(sp.c0, k0 + (k + i) * step) * ROWS + row;
-          s[i] = __ldcg(ml + at);
-          v[i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
+    for (int c = 0; c < EACH; ++c) M[c] = -INFINITY, L[c] = 0.0f, o[c] = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int k = 0; k < n; k += JOIN) {
+      float2 s[EACH][JOIN];
+      float4 v[EACH][JOIN];
+#pragma unroll
+      for (int c = 0; c < EACH; ++c) {
+        const int e = threadIdx.x + c * THREADS, row = r0 + e / (D / 4), d = (e % (D / 4)) * 4;
+#pragma unroll
+        for (int i = 0; i < JOIN; ++i) {
+          s[c][i] = make_float2(-INFINITY, 0.0f);
+          v[c][i] = make_float4(0, 0, 0, 0);
+          if (k + i < n && row < sp.rows) {
+            const int64_t at = (int64_t)part_slot(sp.c0, k0 + (k + i) * step) * ROWS + row;
+            s[c][i] = __ldcg(ml + at);
+            v[c][i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
+          }
         }
       }
-      float mx = M;
 #pragma unroll
-      for (int i = 0; i < JOIN; ++i) mx = fmaxf(mx, s[i].x);
-      const float ref = mx == -INFINITY ? 0.0f : mx;
-      const float f = ex2(M - ref);
-      M = mx;
-      L *= f;
-      o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+      for (int c = 0; c < EACH; ++c) {
+        float mx = M[c];
 #pragma unroll
-      for (int i = 0; i < JOIN; ++i) {
-        const float w = ex2(s[i].x - ref);
-        L = fmaf(s[i].y, w, L);
-        o.x = fmaf(v[i].x, w, o.x), o.y = fmaf(v[i].y, w, o.y), o.z = fmaf(v[i].z, w, o.z), o.w = fmaf(v[i].w, w, o.w);
+        for (int i = 0; i < JOIN; ++i) mx = fmaxf(mx, s[c][i].x);
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        const float f = ex2(M[c] - ref);
+        M[c] = mx;
+        L[c] *= f;
+        o[c].x *= f, o[c].y *= f, o[c].z *= f, o[c].w *= f;
+#pragma unroll
+        for (int i = 0; i < JOIN; ++i) {
+          const float w = ex2(s[c][i].x - ref);
+          L[c] = fmaf(s[c][i].y, w, L[c]);
+          o[c].x = fmaf(v[c][i].x, w, o[c].x), o[c].y = fmaf(v[c][i].y, w, o[c].y);
+          o[c].z = fmaf(v[c][i].z, w, o[c].z), o[c].w = fmaf(v[c][i].w, w, o[c].w);
+        }
       }
     }
-    if (!to_ml) {
-      store_row<T, D>(p, sp.out_row + row, d, o, M, L);
-    } else {  // the slot's own values are read by this thread alone, its ml by others: that goes elsewhere
-      const int64_t at = (int64_t)part_slot(sp.c0, k0) * ROWS + row;
-      __stcg(reinterpret_cast<float4*>(p.partial + at * D + d), o);
-      if (d == 0) __stcg(to_ml + at, make_float2(M, L));
+#pragma unroll
+    for (int c = 0; c < EACH; ++c) {
+      const int e = threadIdx.x + c * THREADS, row = r0 + e / (D / 4), d = (e % (D / 4)) * 4;
+      if (row >= sp.rows) continue;
+      if (!to_ml) {
+        store_row<T, D>(p, sp.out_row + row, d, o[c], M[c], L[c]);
+      } else {  // the slot's own values are read by this thread alone, its ml by others: that goes elsewhere
+        const int64_t at = (int64_t)part_slot(sp.c0, k0) * ROWS + row;
+        __stcg(reinterpret_cast<float4*>(p.partial + at * D + d), o[c]);
+        if (d == 0) __stcg(to_ml + at, make_float2(M[c], L[c]));
+      }
     }
   }
 }
@@ -203,10 +227,6 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
   extern __shared__ __align__(128) unsigned char smem[];
   float* red = reinterpret_cast<float*>(smem + WARPS * S::STAGES * 2 * S::HALF);
   float2* red_ml = reinterpret_cast<float2*>(red + WARPS * 8 * RED);
-  __shared__ int s_scan[WARPS];
-  __shared__ int s_most[WARPS];
-  __shared__ int s_b;
-  __shared__ int s_base;
   __shared__ int s_last[2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int vheads = p.kv_heads * p.row_blocks;
@@ -214,10 +234,12 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
   pdl_trigger();
 
   // ---- this CTA's slice [start, end) of the line, and the sequence it starts in ----
-  const int per = (p.B + THREADS - 1) / THREADS;
-  const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-  int mine = 0;  // blocks of this thread's sequences; their number and the longest one ride along
+  // (every warp finds it for itself, its lanes sharing the sequences: no barrier)
+  const int per = (p.B + 31) / 32;
+  const int b0 = min(p.B, lane * per), b1 = min(p.B, b0 + per);
+  int mine = 0;  // blocks of this lane's sequences; their number and the longest one ride along
   int most = 0, some = 0;
+#pragma unroll 4
   for (int b = b0; b < b1; ++b) {
     const int nb = seq_of(p, b, 0).nb;
     mine += nb;
@@ -226,10 +248,6 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
     if (blockIdx.x == 0 && __ldg(p.seq_lens + b) > (p.max_pages << p.pools.page_shift)) latch(p.err, MOE_ERR_BAD_IDS);
   }
   most = __reduce_max_sync(FULL, most);
-  if (lane == 0) s_most[warp] = most;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) most = max(most, s_most[w]);
   // Short sequences are not split: each counts as many blocks as the longest, and slices hold whole (sequence, head)s.
   // The join of a split costs about as much as the blocks it would spread out.
   const int pad = most <= SHORT ? most : 0;
@@ -240,16 +258,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
     const int v = __shfl_up_sync(FULL, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) s_scan[warp] = incl;
-  __syncthreads();
-  int total = 0, before = incl - mine;
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
-  total *= vheads;
-  before *= vheads;
+  const int total = __shfl_sync(FULL, incl, 31) * vheads, before = (incl - mine) * vheads;
   mine *= vheads;
   int slice = max(total / (int)gridDim.x + (total % (int)gridDim.x ? 1 : 0), MIN_SLICE);
   if (pad) slice = (slice + pad - 1) / pad * pad;
@@ -265,24 +274,24 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
       for (int i = tid; i < p.heads; i += THREADS) p.lse[(int64_t)b * p.heads + i] = -INFINITY;
   }
   if (start >= total) return;  // uniform over the CTA
-  if (start >= before && start < before + mine) {
-    int b = b0;
-    int base = before;
-    for (;; ++b) {
-      const int n = seq_of(p, b, pad).nb * vheads;
-      if (start < base + n) break;
-      base += n;
+  const bool here = start >= before && start - before < mine;
+  int first_b = b0, first_base = before;
+  if (here) {
+    for (;; ++first_b) {
+      const int n = seq_of(p, first_b, pad).nb * vheads;
+      if (start - first_base < n) break;
+      first_base += n;
     }
-    s_b = b;
-    s_base = base;
   }
-  __syncthreads();
+  const int src = __ffs(__ballot_sync(FULL, here)) - 1;
+  first_b = __shfl_sync(FULL, first_b, src);
+  first_base = __shfl_sync(FULL, first_base, src);
 
   Cursor pre;  // the next block this warp looks up
-  pre.b = s_b;
+  pre.b = first_b;
   pre.s = seq_of(p, pre.b, pad);
-  pre.h = (start - s_base) / pre.s.nb;
-  pre.j = (start - s_base) % pre.s.nb;
+  pre.h = (start - first_base) / pre.s.nb;
+  pre.j = (start - first_base) % pre.s.nb;
   Cursor cur = pre;  // the piece being computed (j: its first block in this slice)
   int pre_idx = start + warp;
   advance(p, pre, warp, vheads, pad);
@@ -520,7 +529,6 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
 
   // ---- arrivals: the last CTA of a (sequence, head) joins its parts, or of a group of parts when there are many ----
   if (ahead.parts == 0 && behind.parts == 0) return;
-  __threadfence();
   __syncthreads();
   if (lane == 0 && warp < 2) {
     const Split& sp = warp ? behind : ahead;
@@ -531,19 +539,16 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
   for (int i = 0; i < 2; ++i) {
     if (!s_last[i]) continue;  // uniform over the CTA
     const Split sp = i ? behind : ahead;
-    __threadfence();
     if (sp.parts <= ONE_JOIN) {
       join<T, D, ROWS>(p, sp, 0, 1, sp.parts, p.partial_ml, nullptr);
       continue;
     }
     const int g0 = (blockIdx.x - sp.c0) / JOIN * JOIN;
     join<T, D, ROWS>(p, sp, g0, 1, min(JOIN, sp.parts - g0), p.partial_ml, p.group_ml);
-    __threadfence();
     __syncthreads();
     if (tid == 0) s_last[i] = arrive(p.counters + sp.unit, (sp.parts + JOIN - 1) / JOIN);
     __syncthreads();
     if (s_last[i]) {
-      __threadfence();
       join<T, D, ROWS>(p, sp, 0, JOIN, (sp.parts + JOIN - 1) / JOIN, p.group_ml, nullptr);
     }
   }
