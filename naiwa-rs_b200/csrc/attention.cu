@@ -14,13 +14,16 @@ namespace attn {
 //
 // Per token and head: u = x / sqrt(mean(x^2) + eps) * w (optional), then pair i of the first rope_dim
 // values (a, b) -> (a c - b s, b c + a s) with (c, s) = rope_table[position of the pair's axis][i].
-// Bound by bytes: (heads + 2 kv_heads) * head_dim * 2 read and as many written per token. Each row
-// (one head of one token) is held by head_dim / 8 lanes with 16 bytes each, so every load and store is a
-// full 16-byte access, the norm is a shuffle reduction within the lane group, and a half-pair partner is
-// rope_dim / 16 lanes away. A lane group takes ROWS rows of one token: their loads are in flight together
-// and the lane's table values are read once for all of them. Blocks are (lanes of a row, lane groups, tokens), so a
-// thread finds its work without a division.
+// Floor: (heads + 2 kv_heads) * head_dim * 2 bytes read and as many written per token; with a few arithmetic instructions
+// per byte the kernel is bound by its instruction count as much as by its bytes, so the layout is chosen to need no
+// exchange between lanes but the norm's sum: a row (one head of one token) is held by head_dim / 8 lanes, lane l with
+// two chunks of 4 values that contain both members of its 4 pairs 4 l .. 4 l + 3 (halves: at 4 l and rope_dim / 2 + 4 l; adjacent
+// pairs and values past rope_dim: at 8 l and 8 l + 4). A lane group takes ROWS rows of one token: their loads are in flight
+// together and the lane's table values and norm weights are read once for all of them. Blocks are (lanes of a row,
+// lane groups, tokens), so a thread finds its work without a division.
+
 constexpr int APPEND_THREADS = 256;
+// Rows per lane group, measured at 4096 tokens of 32 + 2 x 4 heads of 128: 2 rows 31 us, 3: 24.1, 4: 23.4, 5: 24.4, 8: 31.
 constexpr int ROWS = 4;
 
 struct AppendParams {
@@ -45,24 +48,28 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
   pdl_wait();
   pdl_trigger();
   const int rows = p.heads + 2 * p.kv_heads;
-  const int l = threadIdx.x;                                            // this lane's 8 values of a row
-  const int r0 = (blockIdx.y * blockDim.y + threadIdx.y) * ROWS;        // first row
+  const int l = threadIdx.x;
+  const int r0 = (blockIdx.y * blockDim.y + threadIdx.y) * ROWS;  // first row
   const int64_t t64 = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
   const bool live = t64 < p.T;
   const int64_t t = live ? t64 : 0;
-  const int lane = (threadIdx.x + blockDim.x * (threadIdx.y + blockDim.y * threadIdx.z)) & 31;
+  const int half = p.rope_dim / 2;
+  const bool turns = 8 * l < p.rope_dim;
+  const bool split = turns && !p.adjacent;  // the chunks lie half a rotation apart
+  const int off0 = split ? 4 * l : 8 * l, off1 = split ? half + 4 * l : 8 * l + 4;
 
-  uint4 x[ROWS];
+  uint2 x[ROWS][2];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int r = r0 + i;
-    x[i] = make_uint4(0, 0, 0, 0);
+    x[i][0] = x[i][1] = make_uint2(0, 0);
     if (live && r < rows) {
       const T* src;
       if (r < p.heads) src = static_cast<const T*>(p.q) + t * p.q_ts + r * p.q_hs;
       else if (r < p.heads + p.kv_heads) src = static_cast<const T*>(p.k) + t * p.k_ts + (r - p.heads) * p.k_hs;
       else src = static_cast<const T*>(p.v) + t * p.v_ts + (r - p.heads - p.kv_heads) * p.v_hs;
-      x[i] = *reinterpret_cast<const uint4*>(src + l * 8);
+      x[i][0] = *reinterpret_cast<const uint2*>(src + off0);
+      x[i][1] = *reinterpret_cast<const uint2*>(src + off1);
     }
   }
 
@@ -75,41 +82,28 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
     for (int a = 0; a < 3; ++a)
       if (a < p.rope_axes) pos[a] = p.positions[(int64_t)a * p.T + t];
   }
-  if (live) {
-    if (slot < 0 || slot >= ((int64_t)p.pools.num_pages << p.pools.page_shift)) {
-      ok = false;
-      if (slot != -1) latch(p.err, MOE_ERR_BAD_IDS);
-    }
+  if (live && (slot < 0 || slot >= ((int64_t)p.pools.num_pages << p.pools.page_shift))) {
+    ok = false;
+    if (slot != -1) latch(p.err, MOE_ERR_BAD_IDS);
   }
-  // this lane's pairs: 8 pairs j0 .. j0 + 7 (halves: value l * 8 + i pairs up at half distance), or the 4
-  // pairs l * 4 .. of its own values (adjacent)
-  const int half = p.rope_dim / 2;
-  const bool turns = l * 8 < p.rope_dim;
-  float c[8], s[8];
-  if (p.rope_dim > 0) {
-    if (ok) {
+  float c[4] = {1, 1, 1, 1}, s[4] = {0, 0, 0, 0};
+  if (ok && p.rope_dim > 0) {
 #pragma unroll
-      for (int a = 0; a < 3; ++a)
-        if (pos[a] < 0 || pos[a] >= p.rope_positions) ok = false;
-      if (!ok) latch(p.err, MOE_ERR_BAD_IDS);
-    }
-    if (ok && turns && p.rope_axes == 1) {  // one table row: two pairs per 16-byte load
-      const int j0 = p.adjacent ? l * 4 : (l * 8 >= half ? l * 8 - half : l * 8);
-      const float4* row = reinterpret_cast<const float4*>(p.rope_table + ((int64_t)pos[0] * half + j0) * 2);
+    for (int a = 0; a < 3; ++a)
+      if (pos[a] < 0 || pos[a] >= p.rope_positions) ok = false;
+    if (!ok) latch(p.err, MOE_ERR_BAD_IDS);
+    if (ok && turns) {
+      if (p.rope_axes == 1) {  // one table row: two pairs per 16-byte load
+        const float4* row = reinterpret_cast<const float4*>(p.rope_table + ((int64_t)pos[0] * half + 4 * l) * 2);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i < 2 || !p.adjacent) {
+        for (int i = 0; i < 2; ++i) {
           const float4 cs = __ldg(row + i);
           c[2 * i] = cs.x, s[2 * i] = cs.y, c[2 * i + 1] = cs.z, s[2 * i + 1] = cs.w;
         }
-      }
-    } else if (ok && turns) {
-      const int np = p.adjacent ? 4 : 8;
-      const int j0 = p.adjacent ? l * 4 : (l * 8 >= half ? l * 8 - half : l * 8);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (i < np) {
-          const int j = j0 + i;
+        for (int i = 0; i < 4; ++i) {
+          const int j = 4 * l + i;
           const int at = j >= p.axis2 ? pos[2] : j >= p.axis1 ? pos[1] : pos[0];
           const float2 cs = __ldg(reinterpret_cast<const float2*>(p.rope_table) + (int64_t)at * half + j);
           c[i] = cs.x;
@@ -120,73 +114,72 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
   }
   const int64_t page = slot >> p.pools.page_shift;
   const int off = (int)(slot & ((1 << p.pools.page_shift) - 1));
+  const bool norm = p.q_norm || p.k_norm;
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
     const int r = r0 + i;
-    const bool is_v = r >= p.heads + p.kv_heads;
-    uint4 out = x[i];
-    // Every lane runs the shuffles of its row (the branch on is_v differs between lane groups of a warp, so
-    // the value rows take part with values that are then dropped).
+    const bool is_q = r < p.heads, is_v = r >= p.heads + p.kv_heads;
+    uint2 out0 = x[i][0], out1 = x[i][1];
     float f[8];
-    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 u = Elem<T>::unpack(w[j]);
-      f[2 * j] = u.x;
-      f[2 * j + 1] = u.y;
+    for (int e = 0; e < 2; ++e) {
+      const float2 lo = Elem<T>::unpack(x[i][e].x), hi = Elem<T>::unpack(x[i][e].y);
+      f[4 * e] = lo.x, f[4 * e + 1] = lo.y, f[4 * e + 2] = hi.x, f[4 * e + 3] = hi.y;
     }
-    const T* nw = static_cast<const T*>(r < p.heads ? p.q_norm : p.k_norm);
-    if (p.q_norm || p.k_norm) {
+    float inv = 1.0f;
+    if (norm) {  // every lane takes part in the sums: a warp's lane groups may hold value rows, whose sum is not used
       float ss = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
 #pragma unroll
       for (int o = LPR / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
-      if (nw) {
-        const float inv = rsqrtf(ss * (1.0f / D) + p.eps);
-        const uint4 nv = __ldg(reinterpret_cast<const uint4*>(nw + l * 8));
-        const uint32_t n4[4] = {nv.x, nv.y, nv.z, nv.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 u = Elem<T>::unpack(n4[j]);
-          f[2 * j] = f[2 * j] * inv * u.x;
-          f[2 * j + 1] = f[2 * j + 1] * inv * u.y;
-        }
-      }
-    }
-    if (p.rope_dim > 0) {
-      if (p.adjacent) {
-        if (turns && ok) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float a = f[2 * j], b = f[2 * j + 1];
-            f[2 * j] = a * c[j] - b * s[j];
-            f[2 * j + 1] = b * c[j] + a * s[j];
-          }
-        }
-      } else {
-        const int hl = half / 8;  // lanes between the two halves of a pair
-        const bool upper = l >= hl;
-        const int from = lane + (turns ? (upper ? -hl : hl) : 0);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float other = __shfl_sync(FULL, f[j], from);
-          if (turns && ok) f[j] = upper ? f[j] * c[j] + other * s[j] : f[j] * c[j] - other * s[j];
-        }
-      }
+      inv = rsqrtf(ss * (1.0f / D) + p.eps);
     }
     if (!live || r >= rows) continue;
-    if (!is_v) out = make_uint4(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]), Elem<T>::pack(f[4], f[5]),
-                                Elem<T>::pack(f[6], f[7]));
-    if (r < p.heads) {
-      if (!ok) out = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.q_out) + t * p.o_ts + r * p.o_hs + l * 8) = out;
-    } else if (ok) {
-      const int h = is_v ? r - p.heads - p.kv_heads : r - p.heads;
-      T* dst = static_cast<T*>(is_v ? p.pools.v : p.pools.k) + page * p.pools.page_stride +
-               (((int64_t)h << p.pools.page_shift) + off) * D;
-      *reinterpret_cast<uint4*>(dst + l * 8) = out;
+    if (!is_v) {
+      const T* nw = static_cast<const T*>(is_q ? p.q_norm : p.k_norm);
+      if (nw) {
+        const uint2 w[2] = {__ldg(reinterpret_cast<const uint2*>(nw + off0)),
+                            __ldg(reinterpret_cast<const uint2*>(nw + off1))};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 lo = Elem<T>::unpack(w[e].x), hi = Elem<T>::unpack(w[e].y);
+          f[4 * e] *= inv * lo.x, f[4 * e + 1] *= inv * lo.y;
+          f[4 * e + 2] *= inv * hi.x, f[4 * e + 3] *= inv * hi.y;
+        }
+      }
+      if (!turns) {
+        // values past rope_dim stay as they are
+      } else if (p.adjacent) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a = f[2 * j], b = f[2 * j + 1];
+          f[2 * j] = a * c[j] - b * s[j];
+          f[2 * j + 1] = b * c[j] + a * s[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a = f[j], b = f[4 + j];
+          f[j] = a * c[j] - b * s[j];
+          f[4 + j] = b * c[j] + a * s[j];
+        }
+      }
+      out0 = make_uint2(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]));
+      out1 = make_uint2(Elem<T>::pack(f[4], f[5]), Elem<T>::pack(f[6], f[7]));
     }
+    T* dst;
+    if (is_q) {
+      if (!ok) out0 = out1 = make_uint2(0, 0);
+      dst = static_cast<T*>(p.q_out) + t * p.o_ts + r * p.o_hs;
+    } else {
+      if (!ok) continue;
+      const int h = is_v ? r - p.heads - p.kv_heads : r - p.heads;
+      dst = static_cast<T*>(is_v ? p.pools.v : p.pools.k) + page * p.pools.page_stride +
+            (((int64_t)h << p.pools.page_shift) + off) * D;
+    }
+    *reinterpret_cast<uint2*>(dst + off0) = out0;
+    *reinterpret_cast<uint2*>(dst + off1) = out1;
   }
 }
 

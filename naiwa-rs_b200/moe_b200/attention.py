@@ -62,16 +62,6 @@ def page_slots(page_table, seqs, positions, page_size: int):
     return page_table[seqs.long(), pos // page_size].long() * page_size + pos % page_size
 
 
-def _current_stream(device, stream):
-    """The raw handle of `stream`, or of the device's current stream (the direct lookup where torch has one: a
-    Stream object costs microseconds, a tenth of a small call)."""
-    if stream is not None:
-        return stream.cuda_stream
-    torch = _torch()
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return torch.cuda.current_stream(device).cuda_stream if raw is None else raw(device.index)
-
-
 def _invalid(msg: str):
     return MoeError(_lib.MOE_ERR_INVALID, msg)
 
@@ -116,6 +106,8 @@ class PagedAttention:
         self.axes = 3 if len(sections) == 3 else 1
         self.max_seqs = int(max_seqs)
         self.device = k_pool.device
+        self._torch, self._int32, self._dim, self._index = torch, torch.int32, dim, k_pool.get_device()
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
         d = AttnDesc()
         d.dtype = kinds[self._dtype]
         d.num_heads, d.num_kv_heads, d.head_dim = cfg.num_heads, cfg.num_kv_heads, cfg.head_dim
@@ -131,7 +123,7 @@ class PagedAttention:
         d.q_norm = None if q_norm is None else q_norm.data_ptr()
         d.k_norm = None if k_norm is None else k_norm.data_ptr()
         d.norm_eps = cfg.norm_eps
-        d.device = self.device.index or 0
+        d.device = self._index
         d.max_seqs = self.max_seqs
         handle = ctypes.c_void_p()
         check(lib().moe_attn_create(ctypes.byref(d), ctypes.byref(handle)))
@@ -155,24 +147,55 @@ class PagedAttention:
     def check(self, stream=None):
         """Raise MoeError when a previous call latched a device-side error (a slot, page, position or length out of
         range)."""
-        check(lib().moe_attn_check(self._h, _current_stream(self.device, stream)))
+        check(lib().moe_attn_check(self._h, self._stream(stream)))
 
-    # -- argument checks ---------------------------------------------------------------------------------
+    # -- argument checks (a small call is a few microseconds on the device: each of these counts) --------------
     def _rows(self, x, heads: int, what: str):
-        """x as rows the kernels take: one head's values consecutive, 16-byte aligned (else a copy)."""
-        if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != self.config.head_dim:
-            raise _invalid(f"{what}: expected [tokens, {heads}, {self.config.head_dim}]")
-        if x.dtype != self._dtype or x.device != self.device:
+        """(x, token stride, head stride) as rows the kernels take: one head's values consecutive, 16-byte aligned
+        (else a copy)."""
+        shape = x.shape
+        if len(shape) != 3 or shape[1] != heads or shape[2] != self._dim:
+            raise _invalid(f"{what}: expected [tokens, {heads}, {self._dim}]")
+        if x.dtype is not self._dtype or x.get_device() != self._index:
             raise _invalid(f"{what}: must be a CUDA tensor of the pools' type on their device")
         ts, hs, one = x.stride()
-        if one != 1 or ts % 8 or hs % 8 or x.data_ptr() % 16:
-            x = x.clone(memory_format=_torch().contiguous_format)
-        return x
+        if one != 1 or (ts | hs) & 7 or x.data_ptr() & 15:
+            x = x.clone(memory_format=self._torch.contiguous_format)
+            ts, hs, one = x.stride()
+        return x, ts, hs
 
-    def _ints(self, t, shape, what: str, dtype):
-        if tuple(t.shape) != shape or t.dtype != dtype or t.device != self.device:
-            raise _invalid(f"{what}: must be a {shape} {dtype} tensor on the pools' device")
+    def _ints(self, t, shape, dtype, what: str):
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != self._index:
+            raise _invalid(f"{what}: must be a {tuple(shape)} {dtype} tensor on the pools' device")
         return t if t.is_contiguous() else t.contiguous()
+
+    def _table(self, table, B: int, what: str):
+        shape = table.shape
+        if len(shape) != 2 or shape[0] != B:
+            raise _invalid(f"{what}: page_table must be [sequences, pages]")
+        return self._ints(table, shape, self._int32, what + ": page_table"), shape[1]
+
+    def _stream(self, stream):
+        """The raw handle of `stream`, or of the device's current stream (by torch's direct lookup where it has one)."""
+        if stream is not None:
+            return stream.cuda_stream
+        if self._raw_stream is not None:
+            return self._raw_stream(self._index)
+        return self._torch.cuda.current_stream(self.device).cuda_stream
+
+    def _outputs(self, q, out, lse, return_lse, what: str):
+        if out is None:
+            out = self._torch.empty_like(q, memory_format=self._torch.contiguous_format)
+        elif (out.shape != q.shape or out.dtype is not self._dtype or out.get_device() != self._index or
+              not out.is_contiguous() or out.data_ptr() & 15):
+            raise _invalid(f"{what}: out must be a contiguous, 16-byte aligned tensor of q's shape and type")
+        if lse is not None:
+            if (lse.shape != q.shape[:2] or lse.dtype is not self._torch.float32 or
+                    lse.get_device() != self._index or not lse.is_contiguous()):
+                raise _invalid(f"{what}: lse must be a contiguous [tokens, num_heads] f32 tensor")
+        elif return_lse:
+            lse = q.new_empty(q.shape[:2], dtype=self._torch.float32)
+        return out, lse
 
     # -- the operators -------------------------------------------------------------------------------------
     def append(self, q, k, v, positions, slots, out=None, stream=None):
@@ -180,87 +203,62 @@ class PagedAttention:
         head strides), positions [T] or [axes, T] int32 (None without rotation), slots [T] int64 (page *
         page_size + offset; -1: a padding token). Returns norm(q) rotated ([T, num_heads, head_dim], or `out`,
         which may be q)."""
-        torch = _torch()
         cfg = self.config
         T = q.shape[0]
-        q = self._rows(q, cfg.num_heads, "append: q")
-        k = self._rows(k, cfg.num_kv_heads, "append: k")
-        v = self._rows(v, cfg.num_kv_heads, "append: v")
+        q, qt, qh = self._rows(q, cfg.num_heads, "append: q")
+        k, kt, kh = self._rows(k, cfg.num_kv_heads, "append: k")
+        v, vt, vh = self._rows(v, cfg.num_kv_heads, "append: v")
         if k.shape[0] != T or v.shape[0] != T:
             raise _invalid("append: q, k and v hold different numbers of tokens")
+        where = None
         if cfg.rope_dim:
             if positions is None:
                 raise _invalid("append: positions are needed with rotation")
-            if positions.dim() == 1:
-                positions = positions[None]
-            positions = self._ints(positions, (self.axes, T), "append: positions", torch.int32)
-        slots = self._ints(slots, (T,), "append: slots", torch.int64)
+            shape = (T,) if self.axes == 1 and positions.dim() == 1 else (self.axes, T)
+            positions = self._ints(positions, shape, self._int32, "append: positions")
+            where = positions.data_ptr()
+        slots = self._ints(slots, (T,), self._torch.int64, "append: slots")
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif self._rows(out, cfg.num_heads, "append: out") is not out or out.shape[0] != T:
-            raise _invalid("append: out must be [T, num_heads, head_dim] with consecutive, 16-byte aligned heads")
-        qt, qh, _ = q.stride()
-        kt, kh, _ = k.stride()
-        vt, vh, _ = v.stride()
-        ot, oh, _ = out.stride()
-        check(self._append(self._h, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, T,
-                           positions.data_ptr() if cfg.rope_dim else None, slots.data_ptr(), out.data_ptr(), ot, oh,
-                           _current_stream(self.device, stream)))
+            out = self._torch.empty_like(q, memory_format=self._torch.contiguous_format)
+            ot, oh = cfg.num_heads * self._dim, self._dim
+        else:
+            given = out
+            out, ot, oh = self._rows(out, cfg.num_heads, "append: out")
+            if out is not given or out.shape[0] != T:
+                raise _invalid("append: out must be [T, num_heads, head_dim] with consecutive, 16-byte aligned heads")
+        check(self._append(self._h, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, T, where,
+                           slots.data_ptr(), out.data_ptr(), ot, oh, self._stream(stream)))
         return out
-
-    def _outputs(self, q, out, lse, return_lse, what):
-        torch = _torch()
-        T, H, D = q.shape
-        if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        elif out.shape != q.shape or out.dtype != self._dtype or out.device != self.device or \
-                not out.is_contiguous() or out.data_ptr() % 16:
-            raise _invalid(f"{what}: out must be a contiguous, 16-byte aligned tensor of q's shape and type")
-        if lse is None:
-            if return_lse:
-                lse = torch.empty((T, H), dtype=torch.float32, device=self.device)
-        elif lse.shape != (T, H) or lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous():
-            raise _invalid(f"{what}: lse must be a contiguous [tokens, num_heads] f32 tensor")
-        return out, lse
-
-    def _table(self, page_table, B, what):
-        if page_table.dim() != 2:
-            raise _invalid(f"{what}: page_table must be [sequences, pages]")
-        return self._ints(page_table, (B, page_table.shape[1]), f"{what}: page_table", _torch().int32)
 
     def decode(self, q, seq_lens, page_table, out=None, lse=None, return_lse=False, stream=None):
         """One new token per sequence: q [B, num_heads, head_dim] against the seq_lens[b] cached tokens (the new one
         included, int32) in the pages of page_table[b] ([B, pages] int32). Returns y [B, num_heads, head_dim],
         or (y, lse) with return_lse or an lse tensor. A sequence of length 0 gives zeros and lse = -inf."""
-        torch = _torch()
-        q = self._rows(q, self.config.num_heads, "decode: q")
+        q, qt, qh = self._rows(q, self.config.num_heads, "decode: q")
         B = q.shape[0]
         if B > self.max_seqs:
             raise _invalid("decode: more sequences than max_seqs")
-        seq_lens = self._ints(seq_lens, (B,), "decode: seq_lens", torch.int32)
-        page_table = self._table(page_table, B, "decode")
+        seq_lens = self._ints(seq_lens, (B,), self._int32, "decode: seq_lens")
+        page_table, pages = self._table(page_table, B, "decode")
         out, lse = self._outputs(q, out, lse, return_lse, "decode")
-        qt, qh, _ = q.stride()
-        check(self._decode(self._h, q.data_ptr(), qt, qh, seq_lens.data_ptr(), page_table.data_ptr(),
-                           page_table.shape[1], B, out.data_ptr(), None if lse is None else lse.data_ptr(),
-                           _current_stream(self.device, stream)))
+        check(self._decode(self._h, q.data_ptr(), qt, qh, seq_lens.data_ptr(), page_table.data_ptr(), pages, B,
+                           out.data_ptr(), None if lse is None else lse.data_ptr(), self._stream(stream)))
         return out if lse is None else (out, lse)
 
     def prefill(self, q, cu_q, seq_lens, page_table, out=None, lse=None, return_lse=False, stream=None):
         """Causal attention of prompt chunks that append has written: q [T, num_heads, head_dim], sequence b's rows
         cu_q[b] .. cu_q[b + 1] - 1 (cu_q [B + 1] int32), the last of its seq_lens[b] cached tokens. Returns y
         [T, num_heads, head_dim], or (y, lse)."""
-        torch = _torch()
-        q = self._rows(q, self.config.num_heads, "prefill: q")
-        if not all(q.stride()):  # an expanded tensor: the tile loads take positive strides only
-            q = q.contiguous()
+        q, qt, qh = self._rows(q, self.config.num_heads, "prefill: q")
+        if not (qt and qh):  # an expanded tensor: the tile loads take positive strides only
+            q = q.clone(memory_format=self._torch.contiguous_format)
+            qt, qh, _ = q.stride()
         B = seq_lens.shape[0]
-        cu_q = self._ints(cu_q, (B + 1,), "prefill: cu_q", torch.int32)
-        seq_lens = self._ints(seq_lens, (B,), "prefill: seq_lens", torch.int32)
-        page_table = self._table(page_table, B, "prefill")
+        cu_q = self._ints(cu_q, (B + 1,), self._int32, "prefill: cu_q")
+        seq_lens = self._ints(seq_lens, (B,), self._int32, "prefill: seq_lens")
+        page_table, pages = self._table(page_table, B, "prefill")
         out, lse = self._outputs(q, out, lse, return_lse, "prefill")
-        qt, qh, _ = q.stride()
-        check(self._prefill(self._h, q.data_ptr(), qt, qh, cu_q.data_ptr(), seq_lens.data_ptr(),
-                            page_table.data_ptr(), page_table.shape[1], B, q.shape[0], out.data_ptr(),
-                            None if lse is None else lse.data_ptr(), _current_stream(self.device, stream)))
+        check(self._prefill(self._h, q.data_ptr(), qt, qh, cu_q.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(),
+                            pages, B, q.shape[0], out.data_ptr(), None if lse is None else lse.data_ptr(),
+                            self._stream(stream)))
         return out if lse is None else (out, lse)
