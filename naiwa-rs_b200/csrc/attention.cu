@@ -282,29 +282,37 @@ extern "C" moe_status moe_attn_create(const moe_attn_desc* desc, moe_attn** out)
         desc->page_stride ? desc->page_stride : (int64_t)desc->num_kv_heads * desc->page_size * desc->head_dim;
     const moe_status st = [&]() -> moe_status {
       MOE_CUDA_TRY(cudaDeviceGetAttribute(&a->sms, cudaDevAttrMultiProcessorCount, desc->device));
+      // the workspace, one allocation (a handle is made per layer): each part at a multiple of 256 bytes
       const int rows = decode_rows(a->group);
-      const size_t slots = (size_t)decode_max_ctas(a->sms) * 2;  // a CTA leaves at most two partial results
-      const size_t acc = slots * rows * desc->head_dim * sizeof(float), ml = 2 * slots * rows * sizeof(float2);
+      const size_t slots = (size_t)decode_max_ctas(a->sms) * 2;  // a decode CTA leaves at most two partial results
       const size_t units = (size_t)desc->max_seqs * desc->num_kv_heads * decode_row_blocks(a->group);
-      const size_t cnt = (units + slots) * sizeof(int32_t);
-      MOE_CUDA_TRY(cudaMalloc(&a->partial, acc));
-      MOE_CUDA_TRY(cudaMalloc(&a->partial_ml, ml));
-      a->group_ml = a->partial_ml + slots * rows;
-      MOE_CUDA_TRY(cudaMalloc(&a->counters, cnt));
+      size_t end = 0;
+      auto part = [&](size_t bytes) {
+        const size_t at = end;
+        end += (bytes + 255) / 256 * 256;
+        return at;
+      };
+      const size_t o_cnt = part((units + slots) * sizeof(int32_t));
+      const size_t o_pf_cnt = part((prefill_counters(*a) + 2) * sizeof(int32_t));
+      const size_t o_err = part(sizeof(int32_t));
+      a->zeroed_bytes = end;  // the words above start at zero
+      const size_t o_acc = part(slots * rows * desc->head_dim * sizeof(float));
+      const size_t o_ml = part(2 * slots * rows * sizeof(float2));
+      const size_t o_pf_acc = part(prefill_partial_bytes(*a)), o_pf_ml = part(prefill_ml_bytes(*a));
+      MOE_CUDA_TRY(cudaMalloc(&a->workspace, end));
+      a->bytes = (int64_t)end;
+      unsigned char* w = static_cast<unsigned char*>(a->workspace);
+      a->counters = reinterpret_cast<int32_t*>(w + o_cnt);
       a->group_counters = a->counters + units;
-      const size_t pf_acc = prefill_partial_bytes(*a), pf_ml = prefill_ml_bytes(*a);
-      const size_t pf_cnt = (prefill_counters(*a) + 2) * sizeof(int32_t);
-      MOE_CUDA_TRY(cudaMalloc(&a->pf_partial, pf_acc));
-      MOE_CUDA_TRY(cudaMalloc(&a->pf_ml, pf_ml));
-      MOE_CUDA_TRY(cudaMalloc(&a->pf_counters, pf_cnt));
-      MOE_CUDA_TRY(cudaMemset(a->pf_counters, 0, pf_cnt));
-      MOE_CUDA_TRY(cudaMalloc(&a->err, sizeof(int32_t)));
-      MOE_CUDA_TRY(cudaMemset(a->counters, 0, cnt));
-      a->counter_bytes = cnt;
-      a->pf_counter_bytes = pf_cnt;
-      MOE_CUDA_TRY(cudaMemset(a->err, 0, sizeof(int32_t)));
-      MOE_CUDA_TRY(cudaDeviceSynchronize());  // the zeros are in place for a first call on any stream
-      a->bytes = (int64_t)(acc + ml + cnt + pf_acc + pf_ml + pf_cnt + sizeof(int32_t));
+      a->pf_counters = reinterpret_cast<int32_t*>(w + o_pf_cnt);
+      a->err = reinterpret_cast<int32_t*>(w + o_err);
+      a->partial = reinterpret_cast<float*>(w + o_acc);
+      a->partial_ml = reinterpret_cast<float2*>(w + o_ml);
+      a->group_ml = a->partial_ml + slots * rows;
+      a->pf_partial = reinterpret_cast<float4*>(w + o_pf_acc);
+      a->pf_ml = reinterpret_cast<float2*>(w + o_pf_ml);
+      MOE_CUDA_TRY(cudaMemset(w, 0, a->zeroed_bytes));
+      MOE_CUDA_TRY(cudaStreamSynchronize(cudaStreamLegacy));  // in place for a first call on any stream
       MOE_TRY(prepare_decode(*a));
       MOE_TRY(prepare_prefill(*a));
       for (int i = 0; i < 2; ++i)
@@ -325,13 +333,7 @@ extern "C" moe_status moe_attn_create(const moe_attn_desc* desc, moe_attn** out)
 extern "C" void moe_attn_destroy(moe_attn* a) {
   if (!a) return;
   DeviceGuard guard(a->d.device);
-  cudaFree(a->partial);
-  cudaFree(a->partial_ml);
-  cudaFree(a->counters);
-  cudaFree(a->pf_partial);
-  cudaFree(a->pf_ml);
-  cudaFree(a->pf_counters);
-  cudaFree(a->err);
+  cudaFree(a->workspace);
   delete a;
 }
 
@@ -436,10 +438,8 @@ extern "C" moe_status moe_attn_check(moe_attn* a, void* stream) {
     MOE_CUDA_TRY(cudaMemcpyAsync(&word, a->err, sizeof(word), cudaMemcpyDeviceToHost, st));
     MOE_CUDA_TRY(cudaStreamSynchronize(st));
     if (!word) return MOE_OK;
-    MOE_CUDA_TRY(cudaMemsetAsync(a->err, 0, sizeof(word), st));
-    // a call that gave up may have left its counters half way
-    MOE_CUDA_TRY(cudaMemsetAsync(a->counters, 0, a->counter_bytes, st));
-    MOE_CUDA_TRY(cudaMemsetAsync(a->pf_counters, 0, a->pf_counter_bytes, st));
+    // a call that gave up may have left its counters half way: they go back to zero with the word
+    MOE_CUDA_TRY(cudaMemsetAsync(a->workspace, 0, a->zeroed_bytes, st));
     MOE_CUDA_TRY(cudaStreamSynchronize(st));
     return fail((moe_status)word, word == MOE_ERR_TIMEOUT ? "attention: a bounded device-side wait gave up"
                                                           : "attention: a slot, page, position or length out of range");

@@ -14,17 +14,16 @@ struct moe_attn {
   int sms;
   int64_t page_stride;  // elements
   float scale;
-  // decode workspace: see attention_decode.cu
-  float* partial = nullptr;
-  float2 *partial_ml = nullptr, *group_ml = nullptr;
-  int32_t *counters = nullptr, *group_counters = nullptr;  // one allocation
-  // prefill workspace: see attention_prefill.cu
-  float4* pf_partial = nullptr;
-  float2* pf_ml = nullptr;
-  int32_t* pf_counters = nullptr;  // arrivals, then the two work words
-  int32_t* err = nullptr;
-  size_t counter_bytes = 0, pf_counter_bytes = 0;
+  void* workspace = nullptr;    // one allocation; the counters and the error word come first
+  size_t zeroed_bytes = 0;
   int64_t bytes = 0;
+  int32_t *counters = nullptr, *group_counters = nullptr;  // decode: arrivals per (sequence, head) and per group of parts
+  float* partial = nullptr;                                // parts of split (sequence, head)s: weighted values,
+  float2 *partial_ml = nullptr, *group_ml = nullptr;       // maxima and sums
+  int32_t* pf_counters = nullptr;  // prefill: arrivals per (item, tile, warp), then the two work words
+  float4* pf_partial = nullptr;    // pieces of cut items
+  float2* pf_ml = nullptr;
+  int32_t* err = nullptr;
   CUtensorMap k_map, v_map;  // prefill's page boxes
 };
 

@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   unsigned char* sV = sK + STAGES * S::TILE;
   __shared__ Bars bars;
   __shared__ Piece s_items[RING];
+  __shared__ Batch s_batch[32];  // the load warp's lanes' (registers are short there)
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_abort;
   __shared__ int s_k_issued, s_v_issued, s_q_issued;
@@ -394,8 +395,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       uint64_t* full = is_v ? bars.v_full : bars.k_full;
       uint64_t* free_ = is_v ? bars.v_free : bars.k_free;
       const CUtensorMap* map = is_v ? &v_map : &k_map;
-      Batch batch;
-      if (!is_v) batch = read_batch(p, span, lane, gridDim.x);
+      if (!is_v) s_batch[lane] = read_batch(p, span, lane, gridDim.x);
+      __syncwarp();
       int g = 0, used = 0, w = blockIdx.x;
       bool ok = true;
 #pragma unroll 1
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           ok = take(n, &q);
           if (!ok) break;
         } else {
-          q = piece_of(p, batch, w, span, lane);
+          q = piece_of(p, s_batch[lane], w, span, lane);
           const int slot = n % RING;
           ok = __all_sync(FULL, n < RING || mbar_wait(&bars.item_free[slot], ((n / RING) - 1) & 1, abort));
           if (!ok) break;
