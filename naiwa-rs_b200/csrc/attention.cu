@@ -18,12 +18,12 @@ namespace attn {
 // per byte the kernel is bound by its instruction count as much as by its bytes, so the layout is chosen to need no
 // exchange between lanes but the norm's sum: a row (one head of one token) is held by head_dim / 8 lanes, lane l with
 // two chunks of 4 values that contain both members of its 4 pairs 4 l .. 4 l + 3 (halves: at 4 l and rope_dim / 2 + 4 l; adjacent
-// pairs and values past rope_dim: at 8 l and 8 l + 4). A lane group takes ROWS rows of one token: their loads are in flight
-// together and the lane's table values and norm weights are read once for all of them. Blocks are (lanes of a row,
-// lane groups, tokens), so a thread finds its work without a division.
-
+// pairs and values past rope_dim: at 8 l and 8 l + 4). A lane group takes up to ROWS rows of one token and one kind (q, k or
+// v): their loads are in flight together, and weight and angle of a value are multiplied once for all of them,
+//   out_a = inv (a (w_a c) - b (w_b s)),  out_b = inv (b (w_b c) + a (w_a s)),  inv = 1 / sqrt(mean(x^2) + eps).
+// Blocks are (lanes of a row, lane groups, tokens), so a thread finds its work without a division.
 constexpr int APPEND_THREADS = 256;
-// Rows per lane group, measured at 4096 tokens of 32 + 2 x 4 heads of 128: 2 rows 31 us, 3: 24.1, 4: 23.4, 5: 24.4, 8: 31.
+// Rows per lane group, measured at 4096 tokens of 32 + 2 x 4 heads of 128: 2 rows 33.8 us, 4: 20.2 (4.3 TB/s), 8: 21.2.
 constexpr int ROWS = 4;
 
 struct AppendParams {
@@ -47,12 +47,20 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
   constexpr int LPR = D / 8;  // lanes of a row
   pdl_wait();
   pdl_trigger();
-  const int rows = p.heads + 2 * p.kv_heads;
   const int l = threadIdx.x;
-  const int r0 = (blockIdx.y * blockDim.y + threadIdx.y) * ROWS;  // first row
   const int64_t t64 = (int64_t)blockIdx.x * blockDim.z + threadIdx.z;
   const bool live = t64 < p.T;
   const int64_t t = live ? t64 : 0;
+  // this lane group's rows: `count` of them, row_stride apart
+  const int q_groups = (p.heads + ROWS - 1) / ROWS, kv_groups = (p.kv_heads + ROWS - 1) / ROWS;
+  int group = blockIdx.y * blockDim.y + threadIdx.y;
+  const bool is_q = group < q_groups, is_v = group >= q_groups + kv_groups;
+  group -= is_q ? 0 : is_v ? q_groups + kv_groups : q_groups;
+  const int head = group * ROWS;
+  const int count = live ? min(ROWS, (is_q ? p.heads : p.kv_heads) - head) : 0;  // <= 0: nothing here
+  const int64_t row_stride = is_q ? p.q_hs : is_v ? p.v_hs : p.k_hs;
+  const T* src = static_cast<const T*>(is_q ? p.q : is_v ? p.v : p.k) + t * (is_q ? p.q_ts : is_v ? p.v_ts : p.k_ts) +
+                 head * row_stride;
   const int half = p.rope_dim / 2;
   const bool turns = 8 * l < p.rope_dim;
   const bool split = turns && !p.adjacent;  // the chunks lie half a rotation apart
@@ -61,18 +69,23 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
   uint2 x[ROWS][2];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = r0 + i;
     x[i][0] = x[i][1] = make_uint2(0, 0);
-    if (live && r < rows) {
-      const T* src;
-      if (r < p.heads) src = static_cast<const T*>(p.q) + t * p.q_ts + r * p.q_hs;
-      else if (r < p.heads + p.kv_heads) src = static_cast<const T*>(p.k) + t * p.k_ts + (r - p.heads) * p.k_hs;
-      else src = static_cast<const T*>(p.v) + t * p.v_ts + (r - p.heads - p.kv_heads) * p.v_hs;
-      x[i][0] = *reinterpret_cast<const uint2*>(src + off0);
-      x[i][1] = *reinterpret_cast<const uint2*>(src + off1);
+    if (i < count) {
+      x[i][0] = *reinterpret_cast<const uint2*>(src + i * row_stride + off0);
+      x[i][1] = *reinterpret_cast<const uint2*>(src + i * row_stride + off1);
     }
   }
-
+  // weights of this lane's values
+  const T* nw = static_cast<const T*>(is_v ? nullptr : is_q ? p.q_norm : p.k_norm);
+  float w[8] = {1, 1, 1, 1, 1, 1, 1, 1};
+  if (nw) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(nw + (e ? off1 : off0)));
+      const float2 lo = Elem<T>::unpack(v.x), hi = Elem<T>::unpack(v.y);
+      w[4 * e] = lo.x, w[4 * e + 1] = lo.y, w[4 * e + 2] = hi.x, w[4 * e + 3] = hi.y;
+    }
+  }
   // slot and positions: a token that fails a check is stored nowhere
   bool ok = live;
   const int64_t slot = live ? p.slots[t] : -1;
@@ -92,7 +105,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
     for (int a = 0; a < 3; ++a)
       if (pos[a] < 0 || pos[a] >= p.rope_positions) ok = false;
     if (!ok) latch(p.err, MOE_ERR_BAD_IDS);
-    if (ok && turns) {
+    if (ok && turns && !is_v) {
       if (p.rope_axes == 1) {  // one table row: two pairs per 16-byte load
         const float4* row = reinterpret_cast<const float4*>(p.rope_table + ((int64_t)pos[0] * half + 4 * l) * 2);
 #pragma unroll
@@ -112,14 +125,41 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
       }
     }
   }
-  const int64_t page = slot >> p.pools.page_shift;
-  const int off = (int)(slot & ((1 << p.pools.page_shift) - 1));
-  const bool norm = p.q_norm || p.k_norm;
+  if (count <= 0) return;  // whole lane groups: the sums below are each within one
+  T* dst;
+  int64_t dst_stride;
+  if (is_q) {
+    dst = static_cast<T*>(p.q_out) + t * p.o_ts + head * p.o_hs;
+    dst_stride = p.o_hs;
+  } else {
+    if (!ok) return;
+    const int64_t page = slot >> p.pools.page_shift;
+    const int at = (int)(slot & ((1 << p.pools.page_shift) - 1));
+    dst_stride = (int64_t)D << p.pools.page_shift;
+    dst = static_cast<T*>(is_v ? p.pools.v : p.pools.k) + page * p.pools.page_stride + head * dst_stride + at * D;
+  }
+  if (is_v || (is_q && !ok)) {  // values as they are; zeros for a token that is stored nowhere
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      if (i >= count) break;
+      *reinterpret_cast<uint2*>(dst + i * dst_stride + off0) = ok ? x[i][0] : make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(dst + i * dst_stride + off1) = ok ? x[i][1] : make_uint2(0, 0);
+    }
+    return;
+  }
+  const int lane = (threadIdx.x + blockDim.x * (threadIdx.y + blockDim.y * threadIdx.z)) & 31;
+  const unsigned group_mask = ((1u << LPR) - 1u) << (lane & ~(LPR - 1));
+  // values a_i, b_i of pair i: chunk 0 and chunk 1 (halves), or neighbours
+  const bool adj = p.adjacent;
+  float wac[4], wbs[4], wbc[4], was[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float wa = adj ? w[2 * i] : w[i], wb = adj ? w[2 * i + 1] : w[4 + i];
+    wac[i] = wa * c[i], wbs[i] = wb * s[i], wbc[i] = wb * c[i], was[i] = wa * s[i];
+  }
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    const int r = r0 + i;
-    const bool is_q = r < p.heads, is_v = r >= p.heads + p.kv_heads;
-    uint2 out0 = x[i][0], out1 = x[i][1];
+    if (i >= count) break;
     float f[8];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -127,66 +167,39 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendParams p) 
       f[4 * e] = lo.x, f[4 * e + 1] = lo.y, f[4 * e + 2] = hi.x, f[4 * e + 3] = hi.y;
     }
     float inv = 1.0f;
-    if (norm) {  // every lane takes part in the sums: a warp's lane groups may hold value rows, whose sum is not used
+    if (nw) {
       float ss = 0.0f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
 #pragma unroll
-      for (int o = LPR / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(FULL, ss, o);
+      for (int o = LPR / 2; o >= 1; o >>= 1) ss += __shfl_xor_sync(group_mask, ss, o);
       inv = rsqrtf(ss * (1.0f / D) + p.eps);
     }
-    if (!live || r >= rows) continue;
-    if (!is_v) {
-      const T* nw = static_cast<const T*>(is_q ? p.q_norm : p.k_norm);
-      if (nw) {
-        const uint2 w[2] = {__ldg(reinterpret_cast<const uint2*>(nw + off0)),
-                            __ldg(reinterpret_cast<const uint2*>(nw + off1))};
+    float g[8];
+    if (!turns) {  // past rope_dim: no partner's value may reach these
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float2 lo = Elem<T>::unpack(w[e].x), hi = Elem<T>::unpack(w[e].y);
-          f[4 * e] *= inv * lo.x, f[4 * e + 1] *= inv * lo.y;
-          f[4 * e + 2] *= inv * hi.x, f[4 * e + 3] *= inv * hi.y;
-        }
+      for (int j = 0; j < 8; ++j) g[j] = inv * (f[j] * w[j]);
+    } else if (adj) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        g[2 * j] = inv * (f[2 * j] * wac[j] - f[2 * j + 1] * wbs[j]);
+        g[2 * j + 1] = inv * (f[2 * j + 1] * wbc[j] + f[2 * j] * was[j]);
       }
-      if (!turns) {
-        // values past rope_dim stay as they are
-      } else if (p.adjacent) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = f[2 * j], b = f[2 * j + 1];
-          f[2 * j] = a * c[j] - b * s[j];
-          f[2 * j + 1] = b * c[j] + a * s[j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = f[j], b = f[4 + j];
-          f[j] = a * c[j] - b * s[j];
-          f[4 + j] = b * c[j] + a * s[j];
-        }
-      }
-      out0 = make_uint2(Elem<T>::pack(f[0], f[1]), Elem<T>::pack(f[2], f[3]));
-      out1 = make_uint2(Elem<T>::pack(f[4], f[5]), Elem<T>::pack(f[6], f[7]));
-    }
-    T* dst;
-    if (is_q) {
-      if (!ok) out0 = out1 = make_uint2(0, 0);
-      dst = static_cast<T*>(p.q_out) + t * p.o_ts + r * p.o_hs;
     } else {
-      if (!ok) continue;
-      const int h = is_v ? r - p.heads - p.kv_heads : r - p.heads;
-      dst = static_cast<T*>(is_v ? p.pools.v : p.pools.k) + page * p.pools.page_stride +
-            (((int64_t)h << p.pools.page_shift) + off) * D;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        g[j] = inv * (f[j] * wac[j] - f[4 + j] * wbs[j]);
+        g[4 + j] = inv * (f[4 + j] * wbc[j] + f[j] * was[j]);
+      }
     }
-    *reinterpret_cast<uint2*>(dst + off0) = out0;
-    *reinterpret_cast<uint2*>(dst + off1) = out1;
+    *reinterpret_cast<uint2*>(dst + i * dst_stride + off0) = make_uint2(Elem<T>::pack(g[0], g[1]), Elem<T>::pack(g[2], g[3]));
+    *reinterpret_cast<uint2*>(dst + i * dst_stride + off1) = make_uint2(Elem<T>::pack(g[4], g[5]), Elem<T>::pack(g[6], g[7]));
   }
 }
 
 template <class T>
 static cudaError_t launch_append(const AppendParams& p, int D, cudaStream_t st) {
-  const int rows = p.heads + 2 * p.kv_heads;
-  const int lanes = D / 8, groups = ceil_div(rows, ROWS);
+  const int lanes = D / 8, groups = ceil_div(p.heads, ROWS) + 2 * ceil_div(p.kv_heads, ROWS);
   const int by = std::min(groups, APPEND_THREADS / lanes);
   const int bz = std::max(1, std::min(p.T, APPEND_THREADS / (lanes * by)));
   const dim3 block(lanes, by, bz), grid((unsigned)ceil_div(p.T, bz), (unsigned)ceil_div(groups, by));
