@@ -118,6 +118,26 @@ def test_decode_large_batch_and_back_to_back_calls(M):
         AO.assert_within(y, want[0][:n], want[1][:n], f"call {i}")
 
 
+@pytest.mark.parametrize("lens,kv_heads,group,D,dtype,window", [
+    ([100003, 60001, 1, 90000], 8, 4, 64, BF16, 0),
+    ([140001], 8, 9, 128, F16, 0),
+    ([70000, 0, 65000, 5, 33333, 64000], 8, 1, 64, F16, 60001),
+])
+def test_decode_long_streams_repeat_to_the_bit(M, lens, kv_heads, group, D, dtype, window):
+    heads = kv_heads * group
+    k, v, table = cache(11, lens, kv_heads, D, 128, dtype)
+    q = randn(5, (len(lens), heads, D), dtype, 1.5)
+    att = handle(M, heads, kv_heads, D, k, v, max_seqs=len(lens), window=window)
+    outs = [att.decode(q, i32(lens), table, return_lse=True) for _ in range(4)]
+    att.check()
+    want = AO.run(q, clean(k), clean(v), table, lens, list(range(len(lens) + 1)), 1 / math.sqrt(D), 0.0, window,
+                  4 * AO.U[dtype] ** 2)
+    for y, lse in outs:
+        AO.assert_within(y, want[0], want[1], "y")
+        AO.assert_within(lse, want[2], want[3], "lse")
+        assert torch.equal(y, outs[0][0]) and torch.equal(lse, outs[0][1]), "calls on the same inputs differ"
+
+
 def test_decode_strided_rows_interleaved_pools_side_stream_and_graph(M):
     lens = [100, 513, 0, 77]
     k, v, table = cache(9, lens, 2, 128, 32, BF16, interleaved=True)
