@@ -68,6 +68,13 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];\n"
+               "cp.async.bulk.commit_group;" ::"l"(map),
+               "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -207,7 +214,8 @@ template <int D>
 struct PfShape {
   static constexpr int SLAB = BN * 128;            // 64 values x 128 rows
   static constexpr int TILE = (D / 64) * SLAB;     // a Q, K or V tile
-  static constexpr int BYTES = (NQ + 2 * STAGES) * TILE + 1024;
+  static constexpr int OUT = 32 * 128;             // a softmax warp's rows x 64 output values, on their way out
+  static constexpr int BYTES = (NQ + 2 * STAGES) * TILE + SOFTMAX_WARPS * OUT + 1024;
 };
 
 struct Bars {
@@ -311,13 +319,14 @@ __device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s
 template <class T, int D, bool CAP>
 __global__ void __launch_bounds__(PF_THREADS, 1)
     prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                   const __grid_constant__ CUtensorMap v_map) {
+                   const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap y_map) {
   using S = PfShape<D>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* sQ = smem;
   unsigned char* sK = sQ + NQ * S::TILE;
   unsigned char* sV = sK + STAGES * S::TILE;
+  unsigned char* sO = sV + STAGES * S::TILE;
   __shared__ Bars bars;
   __shared__ Piece s_items[RING];
   __shared__ Batch s_batch[32];  // the load warp's lanes' (registers are short there)
@@ -699,6 +708,39 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       const int64_t slot = (int64_t)q.item * q.cut * NQ + i;  // piece k of this tile at slot + k * NQ
       float4* part = p.partial + slot * (D / 4) * BM + rr;  // [D / 4][BM] of a slot
       const float inv = q.cut > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+      // A warp whose 32 rows are whole tokens, all of them live, sends them out by TMA, 64 values of each at a time (32 / group
+      // tokens x the group's heads): a store of a row per lane touches 32 lines, and 16 of them per warp took 4300
+      // clocks of a piece.
+      if (q.cut == 1 && q.steps > 0 && 32 % p.group == 0 && __all_sync(FULL, live)) {
+        unsigned char* stage = sO + warp * S::OUT;
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the stage has been read
+          __syncwarp();
+#pragma unroll 1
+          for (int e = 0; e < 2; ++e) {
+            uint32_t o[32];
+            tmem_ld32(o_at + c * 64 + e * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (int h = 0; h < 4; ++h)
+                w[h] = Elem<T>::pack(__uint_as_float(o[8 * k + 2 * h]) * inv, __uint_as_float(o[8 * k + 2 * h + 1]) * inv);
+              if (l == 0.0f) w[0] = w[1] = w[2] = w[3] = 0;  // nothing seen: zeros
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * e + k) ^ (lane & 7)) << 4)) =
+                  make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+          proxy_fence();
+          __syncwarp();
+          if (lane == 0)
+            tma_store_3d(&y_map, stage, c * 64, q.kvh * p.group, q.row0 + first + quad * (32 / p.group));
+        }
+        if (p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
+        continue;
+      }
 #pragma unroll 1
       for (int c = 0; c < D / 16; ++c) {
         uint32_t o[16];
@@ -772,6 +814,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
     }
     if (!ok && lane == 0) s_abort = 1;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // the rows on their way out are out
   }
   __syncthreads();
   if (tid == 0) {
@@ -840,8 +883,14 @@ moe_status launch_prefill(const moe_attn& a, const PrefillParams& p, cudaStream_
   const cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)tq};
   CUtensorMap q_map;
   MOE_TRY(encode_tmap_sw128(&q_map, map_type(a.d.dtype), 3, p.q, dims, strides, box));
+  // y: a softmax warp's whole tokens (the kernel stores by rows where a warp's rows are not)
+  const cuuint64_t y_strides[2] = {(cuuint64_t)a.d.head_dim * 2, (cuuint64_t)p.heads * a.d.head_dim * 2};
+  const bool whole = 32 % p.group == 0;
+  const cuuint32_t y_box[3] = {64, whole ? (cuuint32_t)p.group : 1, whole ? 32u / p.group : 1};
+  CUtensorMap y_map;
+  MOE_TRY(encode_tmap_sw128(&y_map, map_type(a.d.dtype), 3, p.y, dims, y_strides, y_box));
   return with_kernel(a, [&](auto kernel, int smem) -> moe_status {
-    MOE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(PF_THREADS), smem, st, p, q_map, a.k_map, a.v_map));
+    MOE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(PF_THREADS), smem, st, p, q_map, a.k_map, a.v_map, y_map));
     return MOE_OK;
   });
 }
