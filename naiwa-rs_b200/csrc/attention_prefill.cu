@@ -361,6 +361,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     s_abort = 0;
     s_k_issued = s_v_issued = s_q_issued = 0;
   }
+  if (tid == PF_THREADS - 1) {  // the maps' own latency passes behind the set-up
+    for (const CUtensorMap* map : {&q_map, &k_map, &v_map})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   // rows of a tile that no box fills (a group that does not divide 128) stay zero
   if (tq * p.group < BM)
     for (int e = tid; e < NQ * S::TILE / 16; e += PF_THREADS) reinterpret_cast<uint4*>(sQ)[e] = make_uint4(0, 0, 0, 0);
@@ -717,11 +721,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         for (int c = 0; c < D / 64; ++c) {
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the stage has been read
           __syncwarp();
-#pragma unroll 1
+          uint32_t o2[2][32];
+          tmem_ld32(o_at + c * 64, o2[0]);
+          tmem_ld32(o_at + c * 64 + 32, o2[1]);
+          tmem_wait_ld();
+#pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint32_t o[32];
-            tmem_ld32(o_at + c * 64 + e * 32, o);
-            tmem_wait_ld();
+            uint32_t(&o)[32] = o2[e];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint32_t w[4];
