@@ -238,7 +238,7 @@ __device__ __forceinline__ int tokens_of(const PrefillParams& p, int b) {
   return max(0, min(__ldg(p.cu_q + b + 1), p.T) - max(0, __ldg(p.cu_q + b)));
 }
 
-__device__ __forceinline__ Batch read_batch(const PrefillParams& p, int span, int lane, int ctas) {
+__device__ __forceinline__ Batch read_batch(const PrefillParams& p, int span, int lane, int ctas, int join_cost) {
   Batch s;
   s.per = (p.B + 31) / 32;
   s.mine = 0;
@@ -260,14 +260,15 @@ __device__ __forceinline__ Batch read_batch(const PrefillParams& p, int span, in
   s.before = incl - s.mine;
   s.items = __shfl_sync(FULL, incl, 31) * p.kv_heads;
   most = __reduce_max_sync(FULL, most);
-  // the cut that takes the fewest steps in the longest CTA, pieces taken in equal rounds
+  // The cut that costs the longest CTA least, in half steps: its rounds of pieces, and the join, one CTA's work, that reads
+  // every piece's rows.
   s.cut = 1;
   if (s.items > 0) {
     int best = 0x7fffffff;
     const int cut = lane + 1;
     if (cut <= MAX_CUT && (cut == 1 || (int64_t)s.items * cut <= 2 * ctas)) {
       const int rounds = (s.items * cut + ctas - 1) / ctas;
-      best = rounds * ((most + cut - 1) / cut + PIECE_COST);
+      best = 2 * rounds * ((most + cut - 1) / cut + PIECE_COST) + (cut > 1 ? cut * join_cost : 0);
     }
     const int least = __reduce_min_sync(FULL, best);
     s.cut = __ffs(__ballot_sync(FULL, best == least));  // the smallest such cut
@@ -315,6 +316,14 @@ __device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s
   q.steps = all * (q.k + 1) / q.cut - a;
   return q;
 }
+
+// Half steps that a piece more costs its join (256 rows of D f32 values against a step's products and, capped, three
+// exponential-unit results per score). Measured, costs 0 / 1 / 3: 64 rows behind 4096 tokens, D 128: 36 / 34 / 34 us; 200
+// rows 20 / 13 / 13; 128 behind 512: 27 / 24 / 18; short capped chunks with D 64: 23 / 23 / 37.
+template <int D, bool CAP>
+struct JoinCost {
+  static constexpr int value = D == 64 ? 1 : CAP ? 2 : 3;
+};
 
 template <class T, int D, bool CAP>
 __global__ void __launch_bounds__(PF_THREADS, 1)
@@ -408,7 +417,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       uint64_t* full = is_v ? bars.v_full : bars.k_full;
       uint64_t* free_ = is_v ? bars.v_free : bars.k_free;
       const CUtensorMap* map = is_v ? &v_map : &k_map;
-      if (!is_v) s_batch[lane] = read_batch(p, span, lane, gridDim.x);
+      if (!is_v) s_batch[lane] = read_batch(p, span, lane, gridDim.x, JoinCost<D, CAP>::value);
       __syncwarp();
       int g = 0, used = 0, w = blockIdx.x;
       bool ok = true;
@@ -798,23 +807,33 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           L += v.y * ex2(v.x - at);
         }
         const float il = L == 0.0f ? 0.0f : 1.0f / L;
+        // 32 values at a time, two pieces' loads in flight together: the join is behind everything else, and its time is its
+        // trips to L2
 #pragma unroll 1
-        for (int c = 0; c < D / 8; ++c) {
-          float4 o[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
-#pragma unroll 4
+        for (int c = 0; c < D / 32; ++c) {
+          float4 o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = make_float4(0, 0, 0, 0);
+#pragma unroll 2
           for (int k = 0; k < q.cut; ++k) {
+            float4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __ldcg(part + ((int64_t)k * NQ * (D / 4) + c * 8 + e) * BM);
             const float f = ex2(__ldcg(ml + k * MLS).x - at);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float4 v = __ldcg(part + ((int64_t)k * NQ * (D / 4) + c * 2 + e) * BM);
-              o[e].x = fmaf(v.x, f, o[e].x), o[e].y = fmaf(v.y, f, o[e].y);
-              o[e].z = fmaf(v.z, f, o[e].z), o[e].w = fmaf(v.w, f, o[e].w);
+            for (int e = 0; e < 8; ++e) {
+              o[e].x = fmaf(v[e].x, f, o[e].x), o[e].y = fmaf(v[e].y, f, o[e].y);
+              o[e].z = fmaf(v[e].z, f, o[e].z), o[e].w = fmaf(v[e].w, f, o[e].w);
             }
           }
-          if (live)
-            *reinterpret_cast<uint4*>(dst + c * 8) =
-                make_uint4(Elem<T>::pack(o[0].x * il, o[0].y * il), Elem<T>::pack(o[0].z * il, o[0].w * il),
-                           Elem<T>::pack(o[1].x * il, o[1].y * il), Elem<T>::pack(o[1].z * il, o[1].w * il));
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              *reinterpret_cast<uint4*>(dst + c * 32 + e * 8) = make_uint4(
+                  Elem<T>::pack(o[2 * e].x * il, o[2 * e].y * il), Elem<T>::pack(o[2 * e].z * il, o[2 * e].w * il),
+                  Elem<T>::pack(o[2 * e + 1].x * il, o[2 * e + 1].y * il),
+                  Elem<T>::pack(o[2 * e + 1].z * il, o[2 * e + 1].w * il));
+          }
         }
         if (live && p.lse) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
       }
