@@ -20,6 +20,10 @@
 // the B operand of O^T = V^T P^T by a register transpose (movmatrix). P is rounded to 16 bits in two parts,
 // hi + lo, each with its own MMA: the weights keep 16 or more bits and the kernel, bound by loads, does
 // not notice the extra MMAs.
+//
+// Measured on a B200, whole calls, bf16, 32 + 4 heads of 128: 128 sequences of 1 to 8191 tokens 177 us (6.1 TB/s, 94% of a
+// measured copy), one of 131071 53 us (5.1 TB/s), 32 of 128 to 2304 24 us, one of 129 8 us (5.4 on the device).
+// Four warps and two CTAs per SM against eight and one: 170 against 183 us for the batch (one CTA's joins leave its SM idle).
 #include <algorithm>
 
 #include "attention_internal.cuh"
