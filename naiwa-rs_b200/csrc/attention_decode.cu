@@ -90,7 +90,7 @@ struct Seq {
 __device__ __forceinline__ Seq seq_of(const DecodeParams& p, int b, int pad) {
   Seq s;
   const int cap = p.max_pages << p.pools.page_shift;
-  s.len = max(0, min(__ldg(p.seq_lens + b), cap));
+  s.len = max(0, min(p.seq_lens[b], cap));
   s.lo = p.window > 0 ? max(0, s.len - p.window) : 0;
   s.first = s.lo / BLK;
   s.nb = (s.len + BLK - 1) / BLK - s.first;
@@ -184,8 +184,8 @@ __device__ __forceinline__ void join(const DecodeParams& p, const Split& sp, int
           v[c][i] = make_float4(0, 0, 0, 0);
           if (k + i < n && row < sp.rows) {
             const int64_t at = (int64_t)part_slot(sp.c0, k0 + (k + i) * step) * ROWS + row;
-            s[c][i] = __ldcg(ml + at);
-            v[c][i] = __ldcg(reinterpret_cast<const float4*>(p.partial + at * D + d));
+            s[c][i] = ld_l2(ml + at);
+            v[c][i] = ld_l2(reinterpret_cast<const float4*>(p.partial + at * D + d));
           }
         }
       }
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
     mine += nb;
     most = max(most, nb);
     some += nb > 0;
-    if (blockIdx.x == 0 && __ldg(p.seq_lens + b) > (p.max_pages << p.pools.page_shift)) latch(p.err, MOE_ERR_BAD_IDS);
+    if (blockIdx.x == 0 && p.seq_lens[b] > (p.max_pages << p.pools.page_shift)) latch(p.err, MOE_ERR_BAD_IDS);
   }
   most = __reduce_max_sync(FULL, most);
   // Short sequences are not split: each counts as many blocks as the longest, and slices hold whole (sequence, head)s.
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
         advance(p, c, lane * WARPS, vheads, pad);
         const int tok = (c.s.first + c.j) * BLK;
         if (tok < c.s.len) {  // not a padding block
-          const int page = __ldg(p.page_table + (int64_t)c.b * p.max_pages + (tok >> p.pools.page_shift));
+          const int page = p.page_table[(int64_t)c.b * p.max_pages + (tok >> p.pools.page_shift)];
           if ((unsigned)page < (unsigned)p.pools.num_pages) {
             my_rows = max(0, c.s.lo - tok) | min(BLK, c.s.len - tok) << 16;
             my_at = (int64_t)page * p.pools.page_stride +
@@ -376,8 +376,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
                      (int64_t)(kvh * p.group + row0 + (n < live_rows ? n : 0)) * p.q_head_stride + 2 * t4;
 #pragma unroll
       for (int kt = 0; kt < D / 16; ++kt) {
-        qf[kt][nt][0] = n < live_rows ? __ldg(reinterpret_cast<const uint32_t*>(src + kt * 16)) : 0u;
-        qf[kt][nt][1] = n < live_rows ? __ldg(reinterpret_cast<const uint32_t*>(src + kt * 16 + 8)) : 0u;
+        qf[kt][nt][0] = n < live_rows ? *reinterpret_cast<const uint32_t*>(src + kt * 16) : 0u;
+        qf[kt][nt][1] = n < live_rows ? *reinterpret_cast<const uint32_t*>(src + kt * 16 + 8) : 0u;
       }
     }
     float acc[D / 16][NT][4];

@@ -239,7 +239,7 @@ struct Batch {
 };
 
 __device__ __forceinline__ int tokens_of(const PrefillParams& p, int b) {
-  return max(0, min(__ldg(p.cu_q + b + 1), p.T) - max(0, __ldg(p.cu_q + b)));
+  return max(0, min(p.cu_q[b + 1], p.T) - max(0, p.cu_q[b]));
 }
 
 __device__ __forceinline__ Batch read_batch(const PrefillParams& p, int span, int lane, int ctas, int join_cost) {
@@ -252,7 +252,7 @@ __device__ __forceinline__ Batch read_batch(const PrefillParams& p, int span, in
     const int n = tokens_of(p, b);
     if (n == 0) continue;
     s.mine += (n + span - 1) / span;
-    const int len = min(__ldg(p.seq_lens + b), p.max_pages << p.page_shift);
+    const int len = min(p.seq_lens[b], p.max_pages << p.page_shift);
     most = max(most, (p.window > 0 ? min(len, p.window + span + BN) : len) / BN + 1);
   }
   int incl = s.mine;
@@ -305,8 +305,8 @@ __device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s
   const int src = __ffs(__ballot_sync(FULL, here)) - 1;
   q.b = __shfl_sync(FULL, b, src);
   tile = __shfl_sync(FULL, tile, src);
-  q.row0 = max(0, __ldg(p.cu_q + q.b));
-  const int news = tokens_of(p, q.b), asked = __ldg(p.seq_lens + q.b);
+  q.row0 = max(0, p.cu_q[q.b]);
+  const int news = tokens_of(p, q.b), asked = p.seq_lens[q.b];
   q.len = max(0, min(asked, p.max_pages << p.page_shift));
   q.past = q.len - news;  // negative: rows before position 0 see nothing
   if (lane == 0 && (asked != q.len || q.past < 0)) latch(p.err, MOE_ERR_BAD_IDS);
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           const int base = (q.j0 + j) * BN, st = g % STAGES;
           const int live = min(pages, (q.len - base + box_rows - 1) >> p.page_shift);  // pages that hold tokens
           const bool on = my < live;
-          int page = on ? __ldg(table + (base >> p.page_shift)) : 0;
+          int page = on ? table[base >> p.page_shift] : 0;
           if ((unsigned)page >= (unsigned)p.num_pages) {
             latch(p.err, MOE_ERR_BAD_IDS);
             page = p.num_pages;  // out of the map: the box reads as zeros
@@ -803,11 +803,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         __threadfence();
         float M = -INFINITY, L = 0.0f;
 #pragma unroll 4
-        for (int k = 0; k < q.cut; ++k) M = fmaxf(M, __ldcg(ml + k * MLS).x);
+        for (int k = 0; k < q.cut; ++k) M = fmaxf(M, ld_l2(ml + k * MLS).x);
         const float at = M == -INFINITY ? 0.0f : M;
 #pragma unroll 4
         for (int k = 0; k < q.cut; ++k) {
-          const float2 v = __ldcg(ml + k * MLS);
+          const float2 v = ld_l2(ml + k * MLS);
           L += v.y * ex2(v.x - at);
         }
         const float il = L == 0.0f ? 0.0f : 1.0f / L;
@@ -822,8 +822,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           for (int k = 0; k < q.cut; ++k) {
             float4 v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = __ldcg(part + ((int64_t)k * NQ * (D / 4) + c * 8 + e) * BM);
-            const float f = ex2(__ldcg(ml + k * MLS).x - at);
+            for (int e = 0; e < 8; ++e) v[e] = ld_l2(part + ((int64_t)k * NQ * (D / 4) + c * 8 + e) * BM);
+            const float f = ex2(ld_l2(ml + k * MLS).x - at);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               o[e].x = fmaf(v[e].x, f, o[e].x), o[e].y = fmaf(v[e].y, f, o[e].y);

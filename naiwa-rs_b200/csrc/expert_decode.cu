@@ -48,18 +48,18 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) expert_gemv_kernel(Exp
   }
   int e, es, base, count;  // es: the expert's weight slot
   if (p.act_rec) {  // one 16-byte load of the plan's record for this active index
-    const int4 r = __ldcg(p.act_rec + a_idx);
+    const int4 r = ld_l2(p.act_rec + a_idx);
     if (r.x < 0) return;
     e = r.x;
     es = r.y;
     base = r.z;
     count = r.w;
   } else {
-    if (a_idx >= __ldcg(p.n_active)) return;
-    e = __ldcg(p.active + a_idx);
-    es = p.slot_of ? __ldcg(p.slot_of + e) : e;
-    base = __ldcg(p.offsets + e);
-    count = __ldcg(p.offsets + e + 1) - base;
+    if (a_idx >= ld_l2(p.n_active)) return;
+    e = ld_l2(p.active + a_idx);
+    es = p.slot_of ? ld_l2(p.slot_of + e) : e;
+    base = ld_l2(p.offsets + e);
+    count = ld_l2(p.offsets + e + 1) - base;
   }
   (void)e;
   // a record that names a slot or a pair range outside the buffers latches an error and is skipped
@@ -214,8 +214,8 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) expert_gemv_kernel(Exp
 }
 
 // y[t][c] = sum_j ypair[t*width + j][c] (j in order) -> bf16; pairs with a bad id are skipped.
-__global__ void combine_kernel(const float* __restrict__ ypair, const uint32_t* __restrict__ ids, int T, int width,
-                               int H, int E, __nv_bfloat16* __restrict__ y, const int32_t* __restrict__ slot_of) {
+__global__ void combine_kernel(const float* ypair, const uint32_t* ids, int T, int width, int H, int E, __nv_bfloat16* y,
+                               const int32_t* slot_of) {
   pdl_wait();  // ypair from the down projection
   pdl_trigger();
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;  // one float4 per thread

@@ -199,7 +199,7 @@ struct WBF16 {
 template <bool F16>
 __device__ __forceinline__ void load_chunk(const ExpertParams& p, int src_row, int c, float (&v)[8]) {
   if (p.phase == 0) {
-    uint4 raw = ldg_nc(p.x + (int64_t)src_row * p.K + c * 8);
+    uint4 raw = ld_row(p.x + (int64_t)src_row * p.K + c * 8);
     const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -426,11 +426,11 @@ __device__ __forceinline__ Item decode_item(const GemmParams& p, int w) {
   Item it;
   const int ti = w / p.tiles;
   it.tile = w % p.tiles;
-  const int entry = __ldg(p.tile_list + ti);
-  it.e = __ldg(p.active + (entry >> 16));
-  it.es = p.slot_of ? __ldg(p.slot_of + it.e) : it.e;
-  it.base = __ldg(p.offsets + it.e);
-  const int count = __ldg(p.offsets + it.e + 1) - it.base;
+  const int entry = p.tile_list[ti];
+  it.e = p.active[entry >> 16];
+  it.es = p.slot_of ? p.slot_of[it.e] : it.e;
+  it.base = p.offsets[it.e];
+  const int count = p.offsets[it.e + 1] - it.base;
   it.n0 = (entry & 0xffff) * BN;
   it.nval = min(BN, count - it.n0);
   it.nmma = (it.nval + 15) & ~15;  // M = 128 needs N % 16 == 0
@@ -454,10 +454,10 @@ __device__ __forceinline__ void epilogue_blocks(const GemmParams& p, const Item&
     cpr[t] = 0;
     if (n < it.nval) {
       const int idx = it.base + it.n0 + n;
-      csc[t] = __ldg(p.tscale + idx);
+      csc[t] = ld_l2(p.tscale + idx);
       if (p.phase == 1) {
-        cpr[t] = __ldg(p.perm + idx);
-        csc[t] *= __ldg(p.route_w + cpr[t]);
+        cpr[t] = ld_l2(p.perm + idx);
+        csc[t] *= ld_l2(p.route_w + cpr[t]);
       }
     }
   }
@@ -832,10 +832,9 @@ constexpr int TL_THREADS = 256;
 // (a_idx << 16 | token tile) entries of the active experts, in active order. One CTA: each pass of
 // TL_THREADS active experts computes its tile counts, scans them across the block and writes its
 // entries; loads are independent per thread (a serial walk costs two dependent loads per expert).
-__global__ void __launch_bounds__(TL_THREADS) tile_list_kernel(const int32_t* __restrict__ counts,
-                                                               const int32_t* __restrict__ active,
-                                                               const int32_t* __restrict__ n_active, int bn,
-                                                               int32_t* __restrict__ list, int32_t* __restrict__ n_list) {
+__global__ void __launch_bounds__(TL_THREADS) tile_list_kernel(const int32_t* counts, const int32_t* active,
+                                                               const int32_t* n_active, int bn, int32_t* list,
+                                                               int32_t* n_list) {
   __shared__ int s_warp[TL_THREADS / 32];
   __shared__ int s_base;
   pdl_wait();  // the plan's counts and active list
@@ -846,7 +845,7 @@ __global__ void __launch_bounds__(TL_THREADS) tile_list_kernel(const int32_t* __
   __syncthreads();
   for (int a0 = 0; a0 < na; a0 += TL_THREADS) {
     const int a = a0 + threadIdx.x;
-    const int nt = a < na ? (__ldg(counts + __ldg(active + a)) + bn - 1) / bn : 0;
+    const int nt = a < na ? (counts[active[a]] + bn - 1) / bn : 0;
     int incl = nt;  // inclusive scan within the warp, then across warps
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -874,9 +873,8 @@ __global__ void __launch_bounds__(TL_THREADS) tile_list_kernel(const int32_t* __
 // its max magnitude lies in [2^13, 2^14) (exact for bf16 inputs), the scale kept per row. Only the
 // first *n_valid sorted positions exist (the plan drops empty MOE_ID_NONE slots and bad ids), so
 // warps past it return; a perm entry outside [0, n_pairs) is skipped as well.
-__global__ void gather_rows_kernel(const __nv_bfloat16* __restrict__ x, const float* __restrict__ xf, int K, int width,
-                                   const int32_t* __restrict__ perm, int n_pairs, const int32_t* __restrict__ n_valid,
-                                   __half* __restrict__ out, float* __restrict__ scale) {
+__global__ void gather_rows_kernel(const __nv_bfloat16* x, const float* xf, int K, int width, const int32_t* perm,
+                                   int n_pairs, const int32_t* n_valid, __half* out, float* scale) {
   const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, lane = threadIdx.x & 31;
   pdl_wait();  // perm and the rows to gather come from earlier kernels
   pdl_trigger();
@@ -887,7 +885,7 @@ __global__ void gather_rows_kernel(const __nv_bfloat16* __restrict__ x, const fl
   float m = 0.0f;
   for (int c = lane; c < K / 8; c += 32) {
     if (x) {
-      uint4 raw = ldg_nc(x + (int64_t)src * K + c * 8);
+      uint4 raw = ld_row(x + (int64_t)src * K + c * 8);
       const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -914,7 +912,7 @@ __global__ void gather_rows_kernel(const __nv_bfloat16* __restrict__ x, const fl
   for (int c = lane; c < K / 8; c += 32) {
     float v[8];
     if (x) {
-      uint4 raw = ldg_nc(x + (int64_t)src * K + c * 8);
+      uint4 raw = ld_row(x + (int64_t)src * K + c * 8);
       const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) expert_stream_kernel(ExpertPara
   }
   const int units_k = p.K / 128;  // units along K of one 128-row unit row
   const int chunks = p.N / 128;   // unit rows per expert
-  const int n_items = __ldcg(p.n_active) * chunks;
+  const int n_items = ld_l2(p.n_active) * chunks;
   // a contiguous, expert-major range of items per CTA: consecutive items share their expert's tokens
   const int it_begin = (int)((int64_t)n_items * blockIdx.x / gridDim.x);
   const int it_end = (int)((int64_t)n_items * (blockIdx.x + 1) / gridDim.x);
@@ -113,9 +113,9 @@ __global__ void __launch_bounds__(ST_THREADS, 1) expert_stream_kernel(ExpertPara
       bool ok = true;
       for (int it = it_begin; it < it_end && ok; ++it) {
         const int a = it / chunks, c = it - a * chunks;
-        const int e = __ldcg(p.active + a);
-        const int es = p.slot_of ? __ldcg(p.slot_of + e) : e;
-        const int count = __ldcg(p.offsets + e + 1) - __ldcg(p.offsets + e);
+        const int e = ld_l2(p.active + a);
+        const int es = p.slot_of ? ld_l2(p.slot_of + e) : e;
+        const int count = ld_l2(p.offsets + e + 1) - ld_l2(p.offsets + e);
         const int passes = (count + TPP - 1) / TPP;
         const uint8_t* src = p.wq + (int64_t)es * p.q_stride + (int64_t)c * units_k * Q8_UNIT_BYTES;
         for (int ps = 0; ps < passes && ok; ++ps)
@@ -150,9 +150,9 @@ __global__ void __launch_bounds__(ST_THREADS, 1) expert_stream_kernel(ExpertPara
   int staged_e = -1, staged_p0 = -1;  // whose tokens xs holds
   for (int it = it_begin; it < it_end && ok; ++it) {
     const int a = it / chunks, c = it - a * chunks;
-    const int e = __ldcg(p.active + a);
-    const int base = __ldcg(p.offsets + e);
-    const int count = __ldcg(p.offsets + e + 1) - base;
+    const int e = ld_l2(p.active + a);
+    const int base = ld_l2(p.offsets + e);
+    const int count = ld_l2(p.offsets + e + 1) - base;
     const int tile = c * 8 + warp;
     for (int p0 = 0; p0 < count && ok; p0 += TPP) {
       const int ntok = min(TPP, count - p0);

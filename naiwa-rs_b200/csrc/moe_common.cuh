@@ -200,6 +200,39 @@ __device__ __forceinline__ uint4 ldg_nc(const void* p) {
   return v;
 }
 
+// Loads of what another kernel of the chain, or another CTA, has written: through L2 and in program order. (__ldg, the two
+// loads above and const __restrict__ parameters promise that nothing writes the data while the kernel is in flight. A kernel
+// launched by launch_pdl is in flight before the kernel ahead of it has written its output, and neither these nor __ldcg are
+// ordered against pdl_wait(): they are for weights, tables and norms. Plain accesses and these loads stay behind it.)
+__device__ __forceinline__ int32_t ld_l2(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ld_l2(const float* p) {
+  float v;
+  asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_l2(const float2* p) {
+  float2 v;
+  asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_l2(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ int4 ld_l2(const int4* p) {
+  int4 v;
+  asm volatile("ld.global.cg.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
+// 16 bytes of token rows, which the kernel before may have written: a plain access, ordered behind pdl_wait().
+__device__ __forceinline__ uint4 ld_row(const void* p) { return *static_cast<const uint4*>(p); }
+
 // 16-byte shared load as a plain C++ access, so the compiler keeps it ordered against barriers.
 __device__ __forceinline__ uint4 lds128(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 

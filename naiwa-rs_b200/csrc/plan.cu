@@ -24,9 +24,9 @@ constexpr int PLAN_SINGLE_MAX = 8 * PLAN_CHUNK;
 // Ranks the pairs of one chunk [c0, c0 + 1024) stably and scatters them to perm.
 // base[e]: first free position of expert e before this chunk (advanced by the chunk's counts).
 // whist: [PLAN_WARPS][E] shared scratch.
-__device__ __forceinline__ void rank_chunk(const uint32_t* __restrict__ ids, int n_pairs, int E, int c0,
-                                           int* base, int* whist, int32_t* __restrict__ perm,
-                                           const int32_t* __restrict__ slot_of) {
+__device__ __forceinline__ void rank_chunk(const uint32_t* ids, int n_pairs, int E, int c0,
+                                           int* base, int* whist, int32_t* perm,
+                                           const int32_t* slot_of) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int i = threadIdx.x; i < PLAN_WARPS * E; i += PLAN_THREADS) whist[i] = 0;
   __syncthreads();
@@ -74,7 +74,7 @@ __device__ void prep_row(const TokenPrep& q, int t, int lane) {
 #pragma unroll
     for (int i = 0; i < MAXC; ++i) {
       const int c = c0 + lane + 32 * i;
-      if (c < chunks) raw[i] = ldg_nc(row + c * 8);
+      if (c < chunks) raw[i] = ld_row(row + c * 8);
     }
 #pragma unroll
     for (int i = 0; i < MAXC; ++i) {
@@ -102,7 +102,7 @@ __device__ void prep_row(const TokenPrep& q, int t, int lane) {
 #pragma unroll
       for (int i = 0; i < MAXC; ++i) {
         const int c = c0 + lane + 32 * i;
-        if (c < chunks) raw[i] = ldg_nc(row + c * 8);
+        if (c < chunks) raw[i] = ld_row(row + c * 8);
       }
     }
 #pragma unroll
@@ -129,7 +129,7 @@ __device__ __forceinline__ void write_act_rec(const PlanOut& o, int e, int a, in
 
 // Whole plan in one CTA (n_pairs <= PLAN_SINGLE_MAX); CTAs 1.. convert the token rows of `prep`
 // (one warp per row) when it is given.
-__global__ void __launch_bounds__(PLAN_THREADS) plan_single_kernel(const uint32_t* __restrict__ ids, int n_pairs,
+__global__ void __launch_bounds__(PLAN_THREADS) plan_single_kernel(const uint32_t* ids, int n_pairs,
                                                                     int E, PlanOut o, TokenPrep prep) {
   pdl_wait();  // ids and x (and, for the later passes, the earlier passes' output)
   pdl_trigger();
@@ -172,9 +172,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_single_kernel(const uint32_
 }
 
 // Large plans: per-chunk histograms -> scan -> per-chunk stable scatter.
-__global__ void __launch_bounds__(PLAN_THREADS) plan_hist_kernel(const uint32_t* __restrict__ ids, int n_pairs, int E,
-                                                                  int32_t* __restrict__ chunk_counts, int32_t* err,
-                                                                  const int32_t* __restrict__ slot_of) {
+__global__ void __launch_bounds__(PLAN_THREADS) plan_hist_kernel(const uint32_t* ids, int n_pairs, int E,
+                                                                  int32_t* chunk_counts, int32_t* err,
+                                                                  const int32_t* slot_of) {
   pdl_wait();  // ids (and, for the later passes, the earlier passes' output)
   pdl_trigger();
   extern __shared__ int psm[];
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_hist_kernel(const uint32_t*
   for (int e = threadIdx.x; e < E; e += PLAN_THREADS) chunk_counts[(size_t)blockIdx.x * E + e] = psm[e];
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) plan_scan_kernel(int n_chunks, int E, int32_t* __restrict__ chunk_counts,
+__global__ void __launch_bounds__(PLAN_THREADS) plan_scan_kernel(int n_chunks, int E, int32_t* chunk_counts,
                                                                   PlanOut o) {
   pdl_wait();  // ids (and, for the later passes, the earlier passes' output)
   pdl_trigger();
@@ -218,10 +218,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_scan_kernel(int n_chunks, i
   if (e == 0) *o.n_active = total;
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) plan_scatter_kernel(const uint32_t* __restrict__ ids, int n_pairs, int E,
-                                                                     const int32_t* __restrict__ chunk_base,
-                                                                     int32_t* __restrict__ perm,
-                                                                     const int32_t* __restrict__ slot_of) {
+__global__ void __launch_bounds__(PLAN_THREADS) plan_scatter_kernel(const uint32_t* ids, int n_pairs, int E,
+                                                                     const int32_t* chunk_base,
+                                                                     int32_t* perm,
+                                                                     const int32_t* slot_of) {
   pdl_wait();  // ids (and, for the later passes, the earlier passes' output)
   pdl_trigger();
   extern __shared__ int psm[];

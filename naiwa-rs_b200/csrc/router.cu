@@ -157,8 +157,8 @@ __device__ void select_token(const RouteParams& p, float* l, float* a, uint32_t*
 // conversions and shared-memory reads per multiply-add. Every logit sees the same operations in the
 // same order either way.
 template <int TB, int EW>
-__global__ void __launch_bounds__(ROUTER_THREADS) route_kernel(RouteParams p, float* __restrict__ ws_logits,
-                                                               unsigned* __restrict__ ws_count_end) {
+__global__ void __launch_bounds__(ROUTER_THREADS) route_kernel(RouteParams p, float* ws_logits,
+                                                               unsigned* ws_count_end) {
   constexpr int EB = ROUTER_EB * EW;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ int s_last;
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(ROUTER_THREADS) route_kernel(RouteParams p, fl
 
   for (int i = threadIdx.x; i < TB * chunks; i += ROUTER_THREADS) {
     const int t = i / chunks, c = i - t * chunks;
-    const uint4 v = t < nt ? ldg_nc(p.x + (size_t)(t0 + t) * H + c * 8) : make_uint4(0, 0, 0, 0);
+    const uint4 v = t < nt ? ld_row(p.x + (size_t)(t0 + t) * H + c * 8) : make_uint4(0, 0, 0, 0);
     if constexpr (EW == 1) {
       xs[i] = v;
     } else {
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(ROUTER_THREADS) route_kernel(RouteParams p, fl
   float* aux = lg + (size_t)TB * E;            // [TB][max(E, 64)]
   const int auxw = E > 64 ? E : 64;
   uint32_t* taken = reinterpret_cast<uint32_t*>(aux + (size_t)TB * auxw);
-  for (int i = threadIdx.x; i < nt * E; i += ROUTER_THREADS) lg[i] = __ldcg(ws_logits + (size_t)t0 * E + i);
+  for (int i = threadIdx.x; i < nt * E; i += ROUTER_THREADS) lg[i] = ld_l2(ws_logits + (size_t)t0 * E + i);
   __syncthreads();
   for (int t = warp; t < nt; t += ROUTER_WARPS)
     select_token(p, lg + t * E, aux + t * auxw, taken + t * ((E + 31) / 32), t0 + t, lane);

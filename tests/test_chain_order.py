@@ -1,0 +1,68 @@
+"""Kernels of an overlapped chain (launch_pdl) start before the kernel ahead of them has written its output. Checked in the
+sources, without a GPU: what another kernel wrote is read by accesses that stay behind pdl_wait(). Loads that promise data nothing
+writes during the launch (__ldg, ld.global.nc, const __restrict__ parameters) or that carry no order (__ldcg) are for
+weights, tables and norms."""
+import glob
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "naiwa-rs_b200", "csrc")
+
+
+def text_of(path):
+    text = re.sub(r"/\*.*?\*/", "", open(path).read(), flags=re.S)
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def chain_files():
+    names = [p for p in glob.glob(os.path.join(CSRC, "*.cu")) if "pdl_wait()" in text_of(p)]
+    headers = [os.path.join(CSRC, h) for h in ("expert_frag.cuh", "attention_internal.cuh", "layer_internal.cuh")]
+    return sorted(names) + headers
+
+
+def kernels(text):
+    """(name, parameters, body) of every __global__ function that waits for the kernel ahead of it."""
+    found = []
+    for m in re.finditer(r"__global__\s+void\s+(?:__launch_bounds__\((?:[^()]|\([^()]*\))*\)\s*)?(\w+)\(", text):
+        depth, i = 1, m.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(text[i], 0)
+            i += 1
+        params, start = text[m.end():i - 1], text.index("{", i)
+        depth, j = 1, start + 1
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[j], 0)
+            j += 1
+        if "pdl_wait()" in text[start:j]:
+            found.append((m.group(1), params, text[start:j]))
+    return found
+
+
+def test_every_chain_file_is_seen():
+    names = {os.path.basename(p) for p in chain_files()}
+    assert {"plan.cu", "router.cu", "expert_decode.cu", "expert_stream.cu", "expert_gemm_tc.cu", "attention.cu",
+            "attention_decode.cu", "attention_prefill.cu", "expert_frag.cuh"} <= names
+    assert sum(len(kernels(text_of(p))) for p in chain_files()) >= 14
+
+
+# What never changes while a kernel runs: expert weights and their scales, router weights, rotary table, norm weights.
+CONSTANT = re.compile(r"\s*(qb\b|sb\b|p\.wq\b|p\.wscale\b|wa\b|wb\b|wr\b|row \+ i\)|"
+                      r"reinterpret_cast<const \w+\*>\((nw|p\.rope_table)\b)")
+
+
+@pytest.mark.parametrize("path", chain_files(), ids=os.path.basename)
+def test_unordered_loads_read_constants_only(path):
+    text = text_of(path)
+    for m in re.finditer(r"\b(__ldg|__ldcg|__ldca|__ldcs|ldg_nc|ldg_stream)\(", text):
+        line = text[m.start():text.index("\n", m.start())]
+        assert m.group(1) != "__ldcg" and CONSTANT.match(text, m.end()), line
+    nc = [line for line in text.splitlines() if "ld.global.nc" in line]
+    assert len(nc) == (1 if path.endswith("expert_frag.cuh") else 0), nc  # the 8-byte scales of one weight format
+
+
+@pytest.mark.parametrize("path", chain_files(), ids=os.path.basename)
+def test_parameters_of_chain_kernels_are_not_promised_constant(path):
+    for name, params, _ in kernels(text_of(path)):
+        assert "__restrict__" not in params, name
