@@ -46,25 +46,28 @@ __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS) expert_gemv_kernel(Exp
     pdl_wait();
     pdl_trigger();
   }
-  int e, es, base, count;  // es: the expert's weight slot
-  if (p.act_rec) {  // one 16-byte load of the plan's record for this active index
-    const int4 r = ld_l2(p.act_rec + a_idx);
-    if (r.x < 0) return;
-    e = r.x;
-    es = r.y;
-    base = r.z;
-    count = r.w;
-  } else {
-    if (a_idx >= ld_l2(p.n_active)) return;
-    e = ld_l2(p.active + a_idx);
-    es = p.slot_of ? ld_l2(p.slot_of + e) : e;
-    base = ld_l2(p.offsets + e);
-    count = ld_l2(p.offsets + e + 1) - base;
+  // One thread reads the plan's record for this active index {expert, weight slot, first pair, pairs}: the checks below and
+  // all that follows see one copy, whatever happens to the plan meanwhile.
+  __shared__ int4 s_rec;
+  if (threadIdx.x == 0) {
+    int4 r = make_int4(-1, 0, 0, 0);
+    if (p.act_rec) {
+      r = ld_l2(p.act_rec + a_idx);
+    } else if (a_idx < ld_l2(p.n_active)) {
+      r.x = ld_l2(p.active + a_idx);
+      r.y = p.slot_of ? ld_l2(p.slot_of + r.x) : r.x;
+      r.z = ld_l2(p.offsets + r.x);
+      r.w = ld_l2(p.offsets + r.x + 1) - r.z;
+    }
+    s_rec = r;
   }
-  (void)e;
+  __syncthreads();
+  const int es = s_rec.y, base = s_rec.z, count = s_rec.w;
+  const bool idle = s_rec.x < 0;
   // a record that names a slot or a pair range outside the buffers latches an error and is skipped
-  if (es < 0 || (p.n_wslots > 0 && es >= p.n_wslots) || base < 0 || count <= 0 || base + count > p.n_pairs) {
-    if (threadIdx.x == 0 && p.err) atomicExch(p.err, (int)MOE_ERR_INVALID);
+  if (idle || es < 0 || (p.n_wslots > 0 && es >= p.n_wslots) || base < 0 || count <= 0 || base + count > p.n_pairs) {
+    if (!idle && threadIdx.x == 0 && p.err) atomicExch(p.err, (int)MOE_ERR_INVALID);
+    pdl_leave();
     return;
   }
   const int ntm = NTM;
@@ -297,7 +300,7 @@ static moe_status launch1(const ExpertParams& p, int grid, size_t smem, int rowt
 }
 
 // rowt: row tiles per CTA (1, 2, 4 or 8 with 8 warps; 16 with 16 warps, one tile per warp). The
-// grid covers min(E, n_pairs) experts; CTAs past the real count of active experts exit at once.
+// grid covers min(E, n_pairs) experts; CTAs past the real count of active experts have nothing to do.
 moe_status launch_expert_gemv(int wdtype, ExpertParams p, int max_active, int rowt, cudaStream_t st) {
   if (p.tpp % 8 || p.tpp < 8 || p.tpp > MAX_TPP) return fail(MOE_ERR_INVALID, "expert kernel: bad tokens per pass");
   if (p.K > 4096) return fail(MOE_ERR_UNSUPPORTED, "decode expert kernel: K > 4096");

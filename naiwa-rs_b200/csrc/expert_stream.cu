@@ -93,16 +93,18 @@ __global__ void __launch_bounds__(ST_THREADS, 1) expert_stream_kernel(ExpertPara
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
   // Gate/up follows the plan directly; the down pass follows gate/up, so the plan (two kernels back)
-  // has completed and its expert list can be read before the wait, which only h needs.
+  // has completed and the producer reads its expert list before the wait, which only h needs.
   if (p.phase == 0) {
     pdl_wait();
     pdl_trigger();
   }
+  __shared__ int s_active;  // read by one thread: every role walks the same items
+  if (threadIdx.x == 0) s_active = ld_l2(p.n_active);
+  __syncthreads();
   const int units_k = p.K / 128;  // units along K of one 128-row unit row
   const int chunks = p.N / 128;   // unit rows per expert
-  const int n_items = ld_l2(p.n_active) * chunks;
+  const int n_items = s_active * chunks;
   // a contiguous, expert-major range of items per CTA: consecutive items share their expert's tokens
   const int it_begin = (int)((int64_t)n_items * blockIdx.x / gridDim.x);
   const int it_end = (int)((int64_t)n_items * (blockIdx.x + 1) / gridDim.x);
@@ -137,11 +139,15 @@ __global__ void __launch_bounds__(ST_THREADS, 1) expert_stream_kernel(ExpertPara
       const uint32_t first = pos > (uint32_t)stages ? pos - (uint32_t)stages : 0u;
       for (uint32_t q = first; q < pos; ++q) mbar_wait(&full[q % stages], (q / stages) & 1, nullptr);
     }
+    pdl_leave();
     return;
   }
 
   // ---- consumers ----
-  bool waited = p.phase == 0;
+  if (p.phase == 1) {  // h belongs to gate/up's grid until it completes
+    pdl_wait();
+    pdl_trigger();
+  }
   bool ok = true;
   uint32_t pos = 0;
   const int g = lane >> 2, cq = lane & 3;
@@ -157,11 +163,6 @@ __global__ void __launch_bounds__(ST_THREADS, 1) expert_stream_kernel(ExpertPara
     for (int p0 = 0; p0 < count && ok; p0 += TPP) {
       const int ntok = min(TPP, count - p0);
       const int nt_used = (ntok + 7) >> 3;
-      if (!waited) {  // h belongs to gate/up's grid until it completes
-        pdl_wait();
-        pdl_trigger();
-        waited = true;
-      }
       if (staged_e != e || staged_p0 != p0) {
         consumers_sync();  // the previous pass's reads of xs are done
         if (threadIdx.x < TPP) spair[threadIdx.x] = threadIdx.x < ntok ? p.perm[base + p0 + threadIdx.x] : -1;

@@ -119,6 +119,13 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// For a CTA that leaves without work: every CTA of a chain kernel waits before it exits, or a launch none of whose CTAs has
+// work would complete ahead of the kernel before it, and the kernel behind would no longer know that one complete.
+__device__ __forceinline__ void pdl_leave() {
+  pdl_wait();
+  pdl_trigger();
+}
+
 bool pdl_enabled();
 
 // allow = false launches plainly (the kernel's pdl_wait / pdl_trigger are then no-ops).

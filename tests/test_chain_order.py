@@ -66,3 +66,20 @@ def test_unordered_loads_read_constants_only(path):
 def test_parameters_of_chain_kernels_are_not_promised_constant(path):
     for name, params, _ in kernels(text_of(path)):
         assert "__restrict__" not in params, name
+
+
+@pytest.mark.parametrize("path", chain_files(), ids=os.path.basename)
+def test_no_cta_leaves_before_it_has_waited(path):
+    """A kernel none of whose CTAs waits would complete ahead of the kernel before it."""
+    for name, _, body in kernels(text_of(path)):
+        before = body[:body.rindex("pdl_wait()")]
+        for m in re.finditer(r"\breturn\b[^;]*;", before):
+            assert re.search(r"pdl_leave\(\);\s*$", before[:m.start()]), (name, before[m.start() - 80:m.end()])
+
+
+def test_the_decode_kernel_reads_its_record_once():
+    """Threads that saw different records would use shared memory that the others never wrote."""
+    body = dict((n, b) for n, _, b in kernels(text_of(os.path.join(CSRC, "expert_decode.cu"))))["expert_gemv_kernel"]
+    head = body[:body.index("s_rec = r;")]
+    assert "if (threadIdx.x == 0) {" in head and "act_rec" not in body[body.index("s_rec = r;"):]
+    assert not re.search(r"p\.(n_active|active|offsets|slot_of)\b", body[body.index("s_rec = r;"):])
