@@ -4,8 +4,8 @@
 cache's pages (per-head RMS norm and rotary positions applied on the way), `decode` attends with one new token
 per sequence, `prefill` with a ragged batch of prompt chunks. The reference has no counterpart (its attention
 belongs to the model it links against); the operators follow the manner of RoutedExperts: torch CUDA tensors are
-the containers, errors raise MoeError, calls run on the current stream unless one is given and do not
-synchronise. A handle's calls must not overlap on the GPU: they share its workspace.
+the containers, errors raise MoeError, calls run on the current stream unless one is given (the caller orders it
+behind what made the inputs) and do not synchronise. A handle's calls must not overlap on the GPU: they share its workspace.
 """
 from __future__ import annotations
 
@@ -14,7 +14,7 @@ from dataclasses import dataclass
 
 from . import _lib
 from ._lib import AttnDesc, MoeError, check, lib
-from .layer import _torch
+from .layer import _torch, run_on
 
 _PAIRS = {"halves": _lib.ROPE_HALVES, "adjacent": _lib.ROPE_ADJACENT}
 
@@ -203,6 +203,8 @@ class PagedAttention:
         head strides), positions [T] or [axes, T] int32 (None without rotation), slots [T] int64 (page *
         page_size + offset; -1: a padding token). Returns norm(q) rotated ([T, num_heads, head_dim], or `out`,
         which may be q)."""
+        if stream is not None:
+            return run_on(stream, self._index, self.append, q, k, v, positions, slots, out=out)
         cfg = self.config
         T = q.shape[0]
         q, qt, qh = self._rows(q, cfg.num_heads, "append: q")
@@ -227,13 +229,15 @@ class PagedAttention:
             if out is not given or out.shape[0] != T:
                 raise _invalid("append: out must be [T, num_heads, head_dim] with consecutive, 16-byte aligned heads")
         check(self._append(self._h, q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, T, where,
-                           slots.data_ptr(), out.data_ptr(), ot, oh, self._stream(stream)))
+                           slots.data_ptr(), out.data_ptr(), ot, oh, self._stream(None)))
         return out
 
     def decode(self, q, seq_lens, page_table, out=None, lse=None, return_lse=False, stream=None):
         """One new token per sequence: q [B, num_heads, head_dim] against the seq_lens[b] cached tokens (the new one
         included, int32) in the pages of page_table[b] ([B, pages] int32). Returns y [B, num_heads, head_dim],
         or (y, lse) with return_lse or an lse tensor. A sequence of length 0 gives zeros and lse = -inf."""
+        if stream is not None:
+            return run_on(stream, self._index, self.decode, q, seq_lens, page_table, out=out, lse=lse, return_lse=return_lse)
         q, qt, qh = self._rows(q, self.config.num_heads, "decode: q")
         B = q.shape[0]
         if B > self.max_seqs:
@@ -242,13 +246,16 @@ class PagedAttention:
         page_table, pages = self._table(page_table, B, "decode")
         out, lse = self._outputs(q, out, lse, return_lse, "decode")
         check(self._decode(self._h, q.data_ptr(), qt, qh, seq_lens.data_ptr(), page_table.data_ptr(), pages, B,
-                           out.data_ptr(), None if lse is None else lse.data_ptr(), self._stream(stream)))
+                           out.data_ptr(), None if lse is None else lse.data_ptr(), self._stream(None)))
         return out if lse is None else (out, lse)
 
     def prefill(self, q, cu_q, seq_lens, page_table, out=None, lse=None, return_lse=False, stream=None):
         """Causal attention of prompt chunks that append has written: q [T, num_heads, head_dim], sequence b's rows
         cu_q[b] .. cu_q[b + 1] - 1 (cu_q [B + 1] int32), the last of its seq_lens[b] cached tokens. Returns y
         [T, num_heads, head_dim], or (y, lse)."""
+        if stream is not None:
+            return run_on(stream, self._index, self.prefill, q, cu_q, seq_lens, page_table, out=out, lse=lse,
+                          return_lse=return_lse)
         q, qt, qh = self._rows(q, self.config.num_heads, "prefill: q")
         if not (qt and qh):  # an expanded tensor: the tile loads take positive strides only
             q = q.clone(memory_format=self._torch.contiguous_format)
@@ -260,5 +267,5 @@ class PagedAttention:
         out, lse = self._outputs(q, out, lse, return_lse, "prefill")
         check(self._prefill(self._h, q.data_ptr(), qt, qh, cu_q.data_ptr(), seq_lens.data_ptr(), page_table.data_ptr(),
                             pages, B, q.shape[0], out.data_ptr(), None if lse is None else lse.data_ptr(),
-                            self._stream(stream)))
+                            self._stream(None)))
         return out if lse is None else (out, lse)

@@ -40,6 +40,33 @@ def _stream(stream=None) -> int:
     return int(stream.cuda_stream)
 
 
+def run_on(stream, device, fn, *args, **kw):
+    """fn(*args, **kw) with `stream` (of `device`, a CUDA ordinal) current: the copies and allocations that the call makes belong
+    to the stream that its kernels run on. The caller orders `stream` behind what made the inputs; tensors that pass from
+    one stream to the other are not reused before both are done with them."""
+    torch = _torch()
+    if stream.device_index != device:
+        raise MoeError(_lib.MOE_ERR_INVALID, "the stream belongs to another device")
+    here = torch.cuda.current_stream(device)
+    with torch.cuda.stream(stream):
+        result = fn(*args, **kw)
+    if here != stream:
+        def tensors(value):
+            if isinstance(value, torch.Tensor):
+                return [value] if value.is_cuda else []
+            if isinstance(value, dict):
+                value = value.values()
+            elif not isinstance(value, (tuple, list)):
+                return []
+            return [t for v in value for t in tensors(v)]
+
+        for t in tensors(args) + tensors(kw):
+            t.record_stream(stream)
+        for t in tensors(result):
+            t.record_stream(here)
+    return result
+
+
 @dataclass
 class MoeConfig:
     """The fields of the reference's ctx.config the operator reads (provider.rs:316-370)."""
