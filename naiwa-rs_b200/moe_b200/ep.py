@@ -23,7 +23,7 @@ import ctypes
 from typing import Optional
 
 from ._lib import check, lib
-from .layer import _ptr, _stream, _torch
+from .layer import _ptr, _stream, _torch, run_on
 
 
 # ---- device kernels -----------------------------------------------------------------------------
@@ -32,6 +32,8 @@ def ep_dispatch(ids, weights, experts_per_rank: int, world: int, error_word=None
     """Dispatch plan of [T, k] global ids/weights (CUDA). Returns a dict of device tensors:
     rank_counts [world], n_send [1], token_rows [T, world], send_token [cap], send_ids [cap, k] (int32
     view of u32), send_w [cap, k]; cap = T * min(world, k)."""
+    if stream is not None:
+        return run_on(stream, ids.get_device(), ep_dispatch, ids, weights, experts_per_rank, world, error_word)
     torch = _torch()
     ids = ids.to(torch.int32).contiguous()
     weights = weights.to(torch.float32).contiguous()
@@ -51,31 +53,35 @@ def ep_dispatch(ids, weights, experts_per_rank: int, world: int, error_word=None
     check(lib().moe_ep_dispatch_plan(_ptr(ids), _ptr(weights), T, k, experts_per_rank, world, _ptr(out["rank_counts"]),
                                      _ptr(out["n_send"]), _ptr(out["token_rows"]), _ptr(out["send_token"]),
                                      _ptr(out["send_ids"]), _ptr(out["send_w"]), _ptr(err),
-                                     ctypes.c_void_p(_stream(stream))))
+                                     ctypes.c_void_p(_stream())))
     out["error_word"] = err
     return out
 
 
 def ep_pack_rows(x, send_token, n_send, cap: int, stream=None):
     """send_x[row] = x[send_token[row]] for row < n_send (device count). x [T, H] bf16 (CUDA)."""
+    if stream is not None:
+        return run_on(stream, x.get_device(), ep_pack_rows, x, send_token, n_send, cap)
     torch = _torch()
     x = x.contiguous()
     T, H = x.shape
     send_x = torch.empty((max(cap, 1), H), dtype=x.dtype, device=x.device)
     check(lib().moe_ep_pack_rows(_ptr(x), T, H, _ptr(send_token), _ptr(n_send), cap, _ptr(send_x),
-                                 ctypes.c_void_p(_stream(stream))))
+                                 ctypes.c_void_p(_stream())))
     return send_x
 
 
 def ep_combine(y_back, token_rows, T: int, y_add=None, stream=None):
     """y[t] = y_add[t] + sum_r y_back[token_rows[t, r]] (bf16 out, f32 accumulation)."""
+    if stream is not None:
+        return run_on(stream, y_back.get_device(), ep_combine, y_back, token_rows, T, y_add)
     torch = _torch()
     world = token_rows.shape[1]
     H = y_back.shape[1]
     y = torch.empty((T, H), dtype=torch.bfloat16, device=y_back.device)
     check(lib().moe_ep_combine(_ptr(y_back.contiguous()), _ptr(token_rows), T, world, H,
                                _ptr(y_add.contiguous() if y_add is not None else None), _ptr(y),
-                               ctypes.c_void_p(_stream(stream))))
+                               ctypes.c_void_p(_stream())))
     return y
 
 
@@ -136,11 +142,13 @@ class ExpertParallelMoE:
         self.last_counts: Optional[tuple] = None
 
     def forward(self, xs, topk_weights, topk_ids, stream=None):
+        if stream is not None:
+            return run_on(stream, xs.get_device(), self.forward, xs, topk_weights, topk_ids)
         torch = _torch()
         T, H = xs.shape
         k = topk_ids.shape[1]
-        plan = ep_dispatch(topk_ids, topk_weights, self.epr, self.world, stream=stream)
-        send_x = ep_pack_rows(xs, plan["send_token"], plan["n_send"], plan["cap"], stream=stream)
+        plan = ep_dispatch(topk_ids, topk_weights, self.epr, self.world)
+        send_x = ep_pack_rows(xs, plan["send_token"], plan["n_send"], plan["cap"])
         y_shared = None
         if self.shared is not None:
             ones = torch.ones((T, 1), dtype=torch.float32, device=xs.device)
@@ -160,7 +168,7 @@ class ExpertParallelMoE:
             y_recv = torch.empty((0, H), dtype=torch.bfloat16, device=xs.device)
         y_back = exchange_rows(y_recv, recv_counts, send_counts, self.group)
         return ep_combine(y_back if y_back.shape[0] else torch.zeros((1, H), dtype=torch.bfloat16, device=xs.device),
-                          plan["token_rows"], T, y_add=y_shared, stream=stream)
+                          plan["token_rows"], T, y_add=y_shared)
 
     __call__ = forward
 
@@ -224,11 +232,13 @@ class PeerExpertParallelMoE:
         four CUDA events recorded after the dispatch (which ends with the receive), the local forward,
         the return and the combine (per-stage timing; the shared expert, if any, runs between the
         return and the combine, while the peers' rows come back)."""
+        if stream is not None:
+            return run_on(stream, xs.get_device(), self.forward, xs, topk_weights, topk_ids, out=out, layer=layer, marks=marks)
         torch = _torch()
         T, H = xs.shape
         if T > self.cap:
             raise ValueError("PeerExpertParallelMoE.forward: T exceeds max_tokens")
-        st = ctypes.c_void_p(_stream(stream))
+        st = ctypes.c_void_p(_stream())
         xs = xs.contiguous()
         ids = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.to(torch.int32)
         ids = ids.contiguous()
@@ -240,7 +250,7 @@ class PeerExpertParallelMoE:
 
         def mark(i):
             if marks is not None:
-                marks[i].record(stream if stream is not None else torch.cuda.current_stream())
+                marks[i].record(torch.cuda.current_stream())
         check(L.moe_ep_peer_dispatch_routed(self._h, _ptr(xs), T, _ptr(ids), _ptr(w), self.epr, 0,
                                             _ptr(P["rank_counts"]), _ptr(P["token_rows"]), _ptr(P["error_word"]), st))
         mark(0)
@@ -252,7 +262,7 @@ class PeerExpertParallelMoE:
         mark(2)
         y_shared = None
         if self.shared is not None:
-            y_shared = self.shared.forward(xs, self.shared_w[:T], self.shared_ids[:T], stream=stream)
+            y_shared = self.shared.forward(xs, self.shared_w[:T], self.shared_ids[:T])
         y = out if out is not None else torch.empty((T, H), dtype=torch.bfloat16, device=xs.device)
         check(L.moe_ep_peer_combine(self._h, 0, T, _ptr(P["rank_counts"]), _ptr(P["token_rows"]),
                                     _ptr(y_shared), _ptr(y), st))

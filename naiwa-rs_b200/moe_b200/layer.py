@@ -234,6 +234,8 @@ class RoutedExperts:
     # -- the operator -------------------------------------------------------------------------------
     def route(self, xs, out_ids=None, out_weights=None, stream=None):
         """Router + top-k for xs [.., H] bf16 -> (ids [T, k] int32 view of u32, weights [T, k] f32)."""
+        if stream is not None:
+            return run_on(stream, self.device, self.route, xs, out_ids=out_ids, out_weights=out_weights)
         torch = _torch()
         x2 = xs.reshape(-1, self.hidden)
         if x2.dtype != torch.bfloat16 or not x2.is_cuda:
@@ -243,7 +245,7 @@ class RoutedExperts:
         ids = out_ids if out_ids is not None else torch.empty((T, self.top_k), dtype=torch.int32, device=x2.device)
         w = out_weights if out_weights is not None else torch.empty((T, self.top_k), dtype=torch.float32,
                                                                     device=x2.device)
-        check(lib().moe_route(self._h, _ptr(x2), T, _ptr(ids), _ptr(w), ctypes.c_void_p(_stream(stream))))
+        check(lib().moe_route(self._h, _ptr(x2), T, _ptr(ids), _ptr(w), ctypes.c_void_p(_stream())))
         return ids, w
 
     def forward_chunked(self, xs, topk_weights, topk_ids, out=None, stream=None):
@@ -253,6 +255,8 @@ class RoutedExperts:
 
     def forward(self, xs, topk_weights, topk_ids, out=None, stream=None, _entry="moe_forward"):
         """sum_j topk_weights[t, j] * expert(topk_ids[t, j])(xs[t]) for every token, in xs's shape."""
+        if stream is not None:
+            return run_on(stream, self.device, self.forward, xs, topk_weights, topk_ids, out=out, _entry=_entry)
         torch = _torch()
         shape = xs.shape
         x2 = xs.reshape(-1, self.hidden)
@@ -275,7 +279,7 @@ class RoutedExperts:
         width = ids.shape[1]
         y = out if out is not None else torch.empty_like(x2)
         check(getattr(lib(), _entry)(self._h, _ptr(x2), T, _ptr(ids), _ptr(w), width, _ptr(y),
-                                     ctypes.c_void_p(_stream(stream))))
+                                     ctypes.c_void_p(_stream())))
         return y.reshape(shape)
 
     __call__ = forward
@@ -318,17 +322,21 @@ def requantize_q2_0(stack, src_dtype: int, E: int, N: int, K: int, device: int =
     """A stacked [E, N, K] projection (GGML bytes of src_dtype: BF16, Q8_0 or Q4_K; numpy uint8 or a
     CUDA uint8 tensor) requantised to Q2_0 on the device: a CUDA uint8 tensor of E*N*K/64*18 bytes
     (moe_requantize_q2_0, the reference's quantize_q2_0 scale-ladder search)."""
+    if stream is not None:
+        return run_on(stream, device, requantize_q2_0, stack, src_dtype, E, N, K, device)
     torch = _torch()
     dev = torch.device("cuda", device)
     src = torch.from_numpy(np.ascontiguousarray(stack).reshape(-1)).to(dev) if isinstance(stack, np.ndarray) \
         else stack.reshape(-1).contiguous()
     out = torch.empty(E * N * K // 64 * 18, dtype=torch.uint8, device=dev)
-    check(lib().moe_requantize_q2_0(int(src_dtype), _ptr(src), E, N, K, _ptr(out), ctypes.c_void_p(_stream(stream))))
+    check(lib().moe_requantize_q2_0(int(src_dtype), _ptr(src), E, N, K, _ptr(out), ctypes.c_void_p(_stream())))
     return out
 
 def route_tokens(x, w_router, k: int, mode: int, bias=None, n_group: int = 1, topk_group: int = 1,
                  routed_scale: float = 1.0, stream=None):
     """Router logits + top-k without a layer: x [T, H] bf16, w_router [E, H] bf16 (CUDA)."""
+    if stream is not None:
+        return run_on(stream, x.get_device(), route_tokens, x, w_router, k, mode, bias, n_group, topk_group, routed_scale)
     torch = _torch()
     T, H = x.shape
     E = w_router.shape[0]
@@ -338,7 +346,7 @@ def route_tokens(x, w_router, k: int, mode: int, bias=None, n_group: int = 1, to
     ws = torch.zeros(ws_bytes, dtype=torch.uint8, device=x.device)
     check(lib().moe_route_tokens(_ptr(x.contiguous()), _ptr(w_router.contiguous()), _ptr(bias), T, H, E, k, mode,
                                  n_group, topk_group, float(routed_scale), _ptr(ids), _ptr(w), _ptr(ws), ws_bytes,
-                                 ctypes.c_void_p(_stream(stream))))
+                                 ctypes.c_void_p(_stream())))
     return ids, w
 
 
@@ -360,6 +368,8 @@ class Router:
         self.ws = torch.zeros(self.ws_bytes, dtype=torch.uint8, device=self.w.device)  # counters start at 0
 
     def route(self, x, out_ids=None, out_weights=None, stream=None):
+        if stream is not None:
+            return run_on(stream, x.get_device(), self.route, x, out_ids=out_ids, out_weights=out_weights)
         torch = _torch()
         T = x.shape[0]
         if T > self.max_tokens:
@@ -368,12 +378,14 @@ class Router:
         w = out_weights if out_weights is not None else torch.empty((T, self.k), dtype=torch.float32, device=x.device)
         check(lib().moe_route_tokens(_ptr(x), _ptr(self.w), _ptr(self.bias), T, self.H, self.E, self.k, self.mode,
                                      self.n_group, self.topk_group, self.scale, _ptr(ids), _ptr(w), _ptr(self.ws),
-                                     self.ws_bytes, ctypes.c_void_p(_stream(stream))))
+                                     self.ws_bytes, ctypes.c_void_p(_stream())))
         return ids, w
 
 
 def plan_pairs(ids, num_experts: int, stream=None):
     """Histogram + stable permutation of routed pairs -> (counts, offsets, perm, active, error_word)."""
+    if stream is not None:
+        return run_on(stream, ids.get_device(), plan_pairs, ids, num_experts)
     torch = _torch()
     flat = ids.reshape(-1).to(torch.int32).contiguous()
     n = flat.numel()
@@ -387,5 +399,5 @@ def plan_pairs(ids, num_experts: int, stream=None):
     ws_bytes = int(lib().moe_plan_workspace_bytes(n, num_experts))
     ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
     check(lib().moe_plan_pairs(_ptr(flat), n, num_experts, _ptr(counts), _ptr(offsets), _ptr(perm), _ptr(active),
-                               _ptr(n_active), _ptr(ws), ws_bytes, _ptr(err), ctypes.c_void_p(_stream(stream))))
+                               _ptr(n_active), _ptr(ws), ws_bytes, _ptr(err), ctypes.c_void_p(_stream())))
     return counts, offsets, perm[:n], active, n_active, err

@@ -15,7 +15,7 @@ from __future__ import annotations
 import ctypes
 
 from ._lib import check, lib
-from .layer import _ptr, _stream, _torch
+from .layer import _ptr, _stream, _torch, run_on
 
 
 class PagedOpts(ctypes.Structure):
@@ -71,6 +71,8 @@ class PagedMoE:
         check(lib().moe_paged_set_next(self._h, nxt._h if nxt is not None else None))
 
     def forward(self, xs, topk_weights, topk_ids, out=None, stream=None):
+        if stream is not None:
+            return run_on(stream, xs.get_device(), self.forward, xs, topk_weights, topk_ids, out=out)
         torch = _torch()
         T = xs.shape[0]
         ids = topk_ids if topk_ids.dtype == torch.int32 else topk_ids.to(torch.int32)
@@ -78,13 +80,15 @@ class PagedMoE:
         ids, w, xs = ids.contiguous(), w.contiguous(), xs.contiguous()
         y = out if out is not None else torch.empty_like(xs)
         check(lib().moe_paged_forward(self._h, _ptr(xs), T, _ptr(ids), _ptr(w), ids.shape[1], _ptr(y),
-                                      ctypes.c_void_p(_stream(stream))))
+                                      ctypes.c_void_p(_stream())))
         return y
 
     __call__ = forward
 
     def prefill(self, xs, topk_weights, topk_ids, out=None, stream=None):
         """A prompt through the cached layer (PrefillStream::forward, prefill_stream.rs:1362-1694)."""
+        if stream is not None:
+            return run_on(stream, xs.get_device(), self.prefill, xs, topk_weights, topk_ids, out=out)
         torch = _torch()
         T = xs.shape[0]
         ids = topk_ids.to(torch.int32).contiguous()
@@ -92,7 +96,7 @@ class PagedMoE:
         xs = xs.contiguous()
         y = out if out is not None else torch.empty_like(xs)
         check(lib().moe_paged_prefill(self._h, _ptr(xs), T, _ptr(ids), _ptr(w), ids.shape[1], _ptr(y),
-                                      ctypes.c_void_p(_stream(stream))))
+                                      ctypes.c_void_p(_stream())))
         return y
 
     def fill(self, stream=None):

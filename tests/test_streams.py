@@ -94,6 +94,51 @@ def test_a_stream_of_another_device_is_refused(ops):
         att.decode(misaligned(1, 4), torch.tensor([1], dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32), stream=side)
 
 
+class FakeLibrary:
+    def __init__(self):
+        self.streams = []
+
+    def __getattr__(self, name):
+        def entry(*args):
+            if name.endswith("_bytes"):
+                return 64
+            self.streams += [a.value for a in args[-2:] if hasattr(a, "value")][:1]
+            return 0
+        return entry
+
+
+@pytest.mark.parametrize("name", ["plan_pairs", "route_tokens", "Router", "ep_dispatch", "ep_pack_rows", "ep_combine",
+                                  "PagedMoE.forward", "PagedMoE.prefill"])
+def test_older_calls_copy_and_allocate_on_the_given_stream(ops, monkeypatch, name):
+    import moe_b200 as M
+    from moe_b200 import ep, layer, paged
+
+    fake = FakeLibrary()
+    for module in (layer, ep, paged):
+        monkeypatch.setattr(module, "lib", lambda: fake)
+    side = FakeStream()
+    x = torch.zeros((4, 64), dtype=torch.bfloat16)[:, ::2]
+    ids, w = torch.zeros((4, 2), dtype=torch.int64), torch.zeros((4, 4))[:, ::2]
+    gate = torch.zeros((8, 64), dtype=torch.bfloat16)[:, ::2]
+    rows = torch.zeros((4, 1), dtype=torch.int32)
+    router = M.Router(gate, 2, 0, max_tokens=4)
+    moe = object.__new__(paged.PagedMoE)
+    moe._h = None
+    calls = {
+        "plan_pairs": lambda: layer.plan_pairs(ids, 8, stream=side),
+        "route_tokens": lambda: layer.route_tokens(x, gate, 2, 0, stream=side),
+        "Router": lambda: router.route(x, stream=side),
+        "ep_dispatch": lambda: ep.ep_dispatch(ids, w, 4, 2, stream=side),
+        "ep_pack_rows": lambda: ep.ep_pack_rows(x, rows, rows, 4, stream=side),
+        "ep_combine": lambda: ep.ep_combine(x, rows, 4, stream=side),
+        "PagedMoE.forward": lambda: moe.forward(x, w, ids, stream=side),
+        "PagedMoE.prefill": lambda: moe.prefill(x, w, ids, stream=side),
+    }
+    del ops[:]
+    calls[name]()
+    assert fake.streams == [side.cuda_stream] and ops and all(s is side for _, s in ops), (fake.streams, ops)
+
+
 # ---- on the GPU ---------------------------------------------------------------------------------------
 
 
@@ -140,3 +185,32 @@ def test_attention_rows_that_need_a_copy_on_a_side_stream():
     torch.cuda.synchronize()
     att.check()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_expert_inputs_that_need_a_copy_on_a_side_stream():
+    import numpy as np
+
+    import moe_b200 as M
+    from oracle import oracle as O
+
+    rng = np.random.default_rng(3)
+    E, k, H, I, T = 16, 4, 256, 128, 6
+    stacks = [O.quantize(O.DT_Q8_0, rng.normal(0, 0.02, s).astype(np.float32))[0] for s in ((E, I, H), (E, I, H), (E, H, I))]
+    cfg = M.MoeConfig(num_experts=E, num_experts_per_tok=k, hidden_size=H, moe_intermediate_size=I)
+    layer = M.RoutedExpertsProvider().build(M.ExpertLoadContext(
+        layer=0, device=0, config=cfg, wdtype=O.DT_Q8_0, gate=stacks[0], up=stacks[1], down=stacks[2], max_tokens=T))
+    x = torch.randn((T, 2 * H), device="cuda").to(torch.bfloat16)[:, ::2]
+    ids = torch.from_numpy(np.stack([rng.permutation(E)[:k] for _ in range(T)])).cuda()  # int64
+    w = torch.rand((T, 2 * k), device="cuda")[:, ::2]
+    want = layer.forward(x, w, ids)
+    side = torch.cuda.Stream()
+    busy = torch.randn((8192, 8192), device="cuda").to(torch.bfloat16)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        busy = (busy @ busy).mul_(1e-3)
+    got = layer.forward(x, w, ids, stream=side)
+    side.synchronize()
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()
+    layer.check()
