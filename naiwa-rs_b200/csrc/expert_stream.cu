@@ -27,7 +27,7 @@ namespace moe {
 constexpr int ST_CONSUMERS = 8;  // consumer warps: one 16-row tile of a 128-row unit each
 constexpr int ST_THREADS = (ST_CONSUMERS + 1) * 32;
 constexpr int ST_MAX_STAGES = 8;
-constexpr int ST_HEADER = 256;   // barriers and the abort flag, ahead of the ring
+constexpr int ST_HEADER = 256;   // barriers, the abort flag and the active count, ahead of the ring
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
@@ -99,12 +99,13 @@ __global__ void __launch_bounds__(ST_THREADS, 1) expert_stream_kernel(ExpertPara
     pdl_wait();
     pdl_trigger();
   }
-  __shared__ int s_active;  // read by one thread: every role walks the same items
-  if (threadIdx.x == 0) s_active = ld_l2(p.n_active);
+  // read by one thread, so that every role walks the same items (in the header: the ring may take all of the dynamic limit)
+  volatile int* active_count = abort_flag + 1;
+  if (threadIdx.x == 0) *active_count = ld_l2(p.n_active);
   __syncthreads();
   const int units_k = p.K / 128;  // units along K of one 128-row unit row
   const int chunks = p.N / 128;   // unit rows per expert
-  const int n_items = s_active * chunks;
+  const int n_items = *active_count * chunks;
   // a contiguous, expert-major range of items per CTA: consecutive items share their expert's tokens
   const int it_begin = (int)((int64_t)n_items * blockIdx.x / gridDim.x);
   const int it_end = (int)((int64_t)n_items * (blockIdx.x + 1) / gridDim.x);
