@@ -107,7 +107,7 @@ struct WQ2 {
     const int64_t grp = (int64_t)tile * (p.kb_count >> 2) + (kb0 >> 2);
     st.q = ldg_stream(p.wq + (int64_t)e * p.q_stride + grp * 512 + lane * 16);
     const uint2* sp = reinterpret_cast<const uint2*>(p.wsc + (int64_t)e * p.s_stride + grp * 64 + (lane >> 2) * 8);
-    asm("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(st.s.x), "=r"(st.s.y) : "l"(sp));
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(st.s.x), "=r"(st.s.y) : "l"(sp));
   }
   template <int NTM>
   __device__ static __forceinline__ void compute(const Stage& st, int kb0, int kb_end, const uint32_t* xs, int ntm,

@@ -189,11 +189,14 @@ __device__ __forceinline__ uint32_t total_key_u(float f) {
   return (uint32_t)b ^ 0x80000000u;
 }
 
-// Streaming 16-byte load that does not allocate in L1 (weights are read once per launch). The
-// data is read-only for the kernel's lifetime, so the asm is not volatile and may be scheduled freely.
+// Streaming 16-byte load that does not allocate in L1 (weights are read once per launch). The data is read-only for the
+// kernel's lifetime, but the asm is volatile: without that it is to the compiler a pure function of the address, to be evaluated
+// ahead of the test that guards it. A weight load past the K range of the last expert's last tile, whose test says no, then
+// reads behind the weight bank, and faults whenever nothing is mapped there (a bank of whole 2 MB pages at the end of what
+// the process has allocated).
 __device__ __forceinline__ uint4 ldg_stream(const void* p) {
   uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;
@@ -201,7 +204,7 @@ __device__ __forceinline__ uint4 ldg_stream(const void* p) {
 
 __device__ __forceinline__ uint4 ldg_nc(const void* p) {
   uint4 v;
-  asm("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "l"(p));
   return v;

@@ -83,3 +83,10 @@ def test_the_decode_kernel_reads_its_record_once():
     head = body[:body.index("s_rec = r;")]
     assert "if (threadIdx.x == 0) {" in head and "act_rec" not in body[body.index("s_rec = r;"):]
     assert not re.search(r"p\.(n_active|active|offsets|slot_of)\b", body[body.index("s_rec = r;"):])
+
+
+@pytest.mark.parametrize("path", sorted(glob.glob(os.path.join(CSRC, "*.cu*"))), ids=os.path.basename)
+def test_loads_in_assembly_are_volatile(path):
+    """A load in a plain asm is a pure function to the compiler, which may evaluate it ahead of the test that guards it."""
+    for m in re.finditer(r"\basm\s*(volatile\s*)?\(\s*\"([^;]*);", text_of(path)):
+        assert m.group(1) or not re.search(r"\b(ld|ldu|ldmatrix|cp|tcgen05|atom|red|st)\b", m.group(2)), m.group(0)
