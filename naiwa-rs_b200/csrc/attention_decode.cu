@@ -19,7 +19,8 @@
 // = K Q^T with m16n8k16, so the 8 heads of a group fill the N side and nothing is padded; P^T returns to
 // the B operand of O^T = V^T P^T by a register transpose (movmatrix). P is rounded to 16 bits in two parts,
 // hi + lo, each with its own MMA: the weights keep 16 or more bits and the kernel, bound by loads, does
-// not notice the extra MMAs.
+// not notice the extra MMAs. In f16 they are scaled by 2^14 first, so that a weight's parts stay above the type's
+// smallest value down to 2^-39 of the largest weight; sums are scaled alike and the quotient is the same.
 //
 // Measured on a B200, whole calls, bf16, 32 + 4 heads of 128: 128 sequences of 1 to 8191 tokens 177 us (6.1 TB/s, 94% of a
 // measured copy), one of 131071 53 us (5.1 TB/s), 32 of 128 to 2304 24 us, one of 129 8 us (5.4 on the device).
@@ -119,13 +120,17 @@ __device__ __forceinline__ void advance(const DecodeParams& p, Cursor& c, int n,
   }
 }
 
-// Four values of an output row from the joined sums (maximum M in units of log2, sum of weights L), and its lse.
+// log2 of what the weights of a type are scaled by.
+template <class T>
+constexpr float DECODE_SCALE = Elem<T>::kWeightBits ? Elem<T>::kWeightBits - 1.0f : 0.0f;
+
+// Four values of an output row from the joined sums (maximum M in units of log2, sum of scaled weights L), and its lse.
 template <class T, int D>
 __device__ __forceinline__ void store_row(const DecodeParams& p, int64_t row, int d, const float4& o, float M, float L) {
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
   *reinterpret_cast<uint2*>(static_cast<T*>(p.y) + row * D + d) =
       make_uint2(Elem<T>::pack(o.x * inv, o.y * inv), Elem<T>::pack(o.z * inv, o.w * inv));
-  if (p.lse && d == 0) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
+  if (p.lse && d == 0) p.lse[row] = L == 0.0f ? -INFINITY : (M - DECODE_SCALE<T>) * LN2 + logf(L);
 }
 
 // Workspace slot of part k of a (sequence, head) whose first CTA is c0: a CTA's part that began in an earlier
@@ -438,8 +443,8 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
           const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet: exp2(-inf - 0) = 0, no NaN
           corr[i] = ex2(m[nt][i] - ref);
           m[nt][i] = mn;
-          s[nt][i] = ex2(s[nt][i] - ref);
-          s[nt][i + 2] = ex2(s[nt][i + 2] - ref);
+          s[nt][i] = ex2(s[nt][i] - (ref - DECODE_SCALE<T>));
+          s[nt][i + 2] = ex2(s[nt][i + 2] - (ref - DECODE_SCALE<T>));
           l[nt][i] = l[nt][i] * corr[i] + (s[nt][i] + s[nt][i + 2]);
         }
 #pragma unroll

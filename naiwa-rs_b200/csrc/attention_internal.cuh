@@ -98,8 +98,12 @@ moe_status make_page_tmap(CUtensorMap* map, int dtype, const void* pool, int hea
 
 template <class T>
 struct Elem;
+// The weights of the second product are rounded to the values' type. kWeightBits: powers of two that they may be scaled up by
+// and stay finite when the largest is 1. In f16 an unscaled weight below 2^-25 would be lost from the values but not from the
+// f32 sum (all of the output where a first key with no value scores 17.5 above the rest); bf16 has f32's exponents.
 template <>
 struct Elem<__nv_bfloat16> {
+  static constexpr int kWeightBits = 0;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static __device__ __forceinline__ float2 unpack(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
@@ -110,6 +114,7 @@ struct Elem<__nv_bfloat16> {
 };
 template <>
 struct Elem<__half> {
+  static constexpr int kWeightBits = 15;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
   static __device__ __forceinline__ float2 unpack(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));

@@ -17,7 +17,8 @@
 //   * four warps per tile hold one row per thread: maximum, exponentials and sum in f32, P rounded to the
 //     values' type (what the tensor cores take; the sum is of the unrounded weights) and written over S in tensor
 //     memory, from where the second product reads it. O is rescaled only when a row's maximum grows by more than
-//     2^RESCALE (rare after the first steps), which leaves P below 2^RESCALE: the quotient does not change.
+//     2^RESCALE (rare after the first steps), which leaves P below 2^RESCALE: the quotient does not change. f16 weights
+//     take the rest of the type's range, another 2^11, so that only those below 2^-36 of the reference vanish.
 // Bound by the tensor cores (1024 clocks of MMA per 128 x 128 step) and as much by the exponentials (16 per clock and SM).
 // Measured on a B200: a step of two tiles takes about 3050 clocks of the 2062 that its MMAs need; the rest is the chain from
 // scores to weights and back. A 4096-token prompt of 32 + 4 heads of 128: 123 us alone (1.12 PFLOP/s, 66% of the measured
@@ -53,7 +54,9 @@ constexpr int MOST = BN / 32;        // products of P V (of BN / 16) that start 
 constexpr int TMEM_COLS = 512;
 constexpr int S_COL = 0;            // S_i / P_i at columns BN * i
 constexpr int O_COL = NQ * BN;      // O_i at columns O_COL + D * i
-constexpr float RESCALE = 8.0f;     // log2 of how far a row's reference may lag behind its maximum
+// log2 of how far a row's reference may lag behind its maximum; f16 weights need the rest of the type's range
+template <class T>
+constexpr float RESCALE = Elem<T>::kWeightBits ? 4.0f : 8.0f;
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
                                             uint64_t* bar) {
@@ -120,6 +123,10 @@ __device__ __forceinline__ bool wait_poll(uint64_t* bar, uint32_t parity, volati
   }
   return true;
 }
+
+// log2 of what the weights of a type are scaled by: with the reference up to RESCALE behind they reach 2^15 in f16.
+template <class T>
+constexpr float PREFILL_SCALE = Elem<T>::kWeightBits ? Elem<T>::kWeightBits - RESCALE<T> : 0.0f;
 
 // Low word of a SWIZZLE_128B shared-memory matrix descriptor, slabs of 64 values x n rows of 128 bytes, 8-row groups 1024
 // bytes apart; the high word is the same for all. Q and K: K-major (the leading offset is not used). V: MN-major, the next
@@ -657,7 +664,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           for (int a = 0; a < 4; ++a)
             mx[a] = fmaxf(fmaxf(mx[a], __uint_as_float(r[k + 2 * a])), __uint_as_float(r[k + 2 * a + 1]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c_log2;  // scale > 0
-        const bool grow = top > m + RESCALE;  // also the first finite maximum
+        const bool grow = top > m + RESCALE<T>;  // also the first finite maximum
         if (__builtin_expect(__any_sync(FULL, grow), 0)) {
           const float mn = grow ? top : m;
           const float f = grow ? ex2(m - mn) : 1.0f;
@@ -675,7 +682,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             }
           }
         }
-        const float ref = m == -INFINITY ? 0.0f : m;
+        const float ref = (m == -INFINITY ? 0.0f : m) - PREFILL_SCALE<T>;
         // The weights, 32 columns at a time. The exponential unit sets the pace (a pair per 16 clocks): its instructions are
         // kept in program order, and the packing and summing of a pair follow AHEAD pairs behind, so that no chunk waits for
         // the unit's latency.
@@ -757,7 +764,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           if (lane == 0)
             tma_store_3d(&y_map, stage, c * 64, q.kvh * p.group, q.row0 + first + quad * (32 / p.group));
         }
-        if (p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
+        if (p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m - PREFILL_SCALE<T>) * LN2 + logf(l);
         continue;
       }
 #pragma unroll 1
@@ -784,7 +791,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         }
       }
       if (q.cut == 1) {
-        if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : m * LN2 + logf(l);
+        if (live && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (m - PREFILL_SCALE<T>) * LN2 + logf(l);
         continue;
       }
       // ---- the last of the item's pieces to arrive joins them in order, each warp its own rows ----
@@ -839,7 +846,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
                   Elem<T>::pack(o[2 * e + 1].z * il, o[2 * e + 1].w * il));
           }
         }
-        if (live && p.lse) p.lse[row] = L == 0.0f ? -INFINITY : M * LN2 + logf(L);
+        if (live && p.lse) p.lse[row] = L == 0.0f ? -INFINITY : (M - PREFILL_SCALE<T>) * LN2 + logf(L);
       }
     }
     if (!ok && lane == 0) s_abort = 1;
