@@ -564,9 +564,10 @@ moe_status moe_attn_decode(moe_attn* attn, const void* q, int64_t q_token_stride
                            const int32_t* seq_lens, const int32_t* page_table, int max_pages, int B, void* y,
                            float* lse, void* stream);
 /* Causal attention of a ragged batch of prompt chunks already appended: sequence b's query rows are
- * cu_q[b] .. cu_q[b + 1] - 1 (cu_q [B + 1] int32, ascending from 0 to T), the last of its seq_lens[b]
+ * cu_q[b] .. cu_q[b + 1] - 1 (cu_q [B + 1] int32, ascending from 0 to at most T), the last of its seq_lens[b]
  * cached positions; row i sees positions up to its own. y [T, num_heads, head_dim] contiguous; lse
- * [T, num_heads] f32 or NULL. Cached values are read in tiles: an infinite or NaN value at a position below
+ * [T, num_heads] f32 or NULL. Rows that no sequence holds (from cu_q[B] on: padding; every row with B = 0) give y = 0
+ * and lse = -inf. A cu_q that starts elsewhere, descends or passes T is latched as MOE_ERR_BAD_IDS. Cached values are read in tiles: an infinite or NaN value at a position below
  * seq_lens[b] may reach rows of that sequence that do not see the position. A chunk longer than its seq_lens
  * is latched as MOE_ERR_BAD_IDS; its rows that have no position give y = 0 and lse = -inf. */
 moe_status moe_attn_prefill(moe_attn* attn, const void* q, int64_t q_token_stride, int64_t q_head_stride,

@@ -422,8 +422,9 @@ extern "C" moe_status moe_attn_prefill(moe_attn* a, const void* q, int64_t q_tok
     const char* me = "moe_attn_prefill";
     if (!a) return bad(me, "null handle");
     if (B < 0 || T < 0) return bad(me, "B and T must not be negative");
-    if (B == 0 || T == 0) return MOE_OK;
-    if (!q || !cu_q || !seq_lens || !page_table || !y || max_pages <= 0) return bad(me, "null pointer or no pages");
+    if (T == 0) return MOE_OK;
+    if (!q || !y || (B > 0 && (!cu_q || !seq_lens || !page_table || max_pages <= 0)))
+      return bad(me, "null pointer or no pages");
     if (!rows_ok(q, q_token_stride, q_head_stride) || ((uintptr_t)y & 15))
       return bad(me, "rows must be 16-byte aligned with strides that are multiples of 8");
     if ((int64_t)max_pages * a->d.page_size > 0x7fffffffll) return bad(me, "max_pages * page_size above 2^31 - 1");

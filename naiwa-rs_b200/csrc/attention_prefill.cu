@@ -43,7 +43,7 @@ constexpr int SOFTMAX_WARPS = 4 * NQ;
 constexpr int MMA_WARP = SOFTMAX_WARPS;
 constexpr int LOAD_WARP = SOFTMAX_WARPS + 1;
 constexpr int V_WARP = SOFTMAX_WARPS + 2;
-constexpr int PF_THREADS = (SOFTMAX_WARPS + 4) * 32;  // the last warp only gives up its registers
+constexpr int PF_THREADS = (SOFTMAX_WARPS + 4) * 32;  // the last warp writes the rows that no sequence holds
 // registers per thread: 168 at launch (384 threads), shared out anew: 2 x 216 + 72 = 3 x 168
 constexpr int SOFTMAX_REGS = 216, OTHER_REGS = 72;
 constexpr int RING = 4;              // pieces handed out ahead
@@ -590,6 +590,22 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         (void)mbar_wait(&bars.drained, 0, nullptr);
         __syncwarp();
       }
+    } else {
+      // ---------------- rows before cu_q[0] and from cu_q[B] on: padding, zeros and -inf ----------------
+      const int first = p.B > 0 ? min(max(p.cu_q[0], 0), p.T) : 0;
+      const int end = p.B > 0 ? min(max(p.cu_q[p.B], first), p.T) : 0;
+      for (int r = blockIdx.x; r < p.T - (end - first); r += gridDim.x) {
+        const int64_t row = (int64_t)(r < first ? r : r - first + end) * p.heads;
+        for (int e = lane; e < p.heads * (D / 8); e += 32)
+          reinterpret_cast<uint4*>(static_cast<T*>(p.y) + row * D)[e] = make_uint4(0, 0, 0, 0);
+        if (p.lse)
+          for (int e = lane; e < p.heads; e += 32) p.lse[row + e] = -INFINITY;
+      }
+      if (blockIdx.x == 0 && p.B > 0) {
+        bool bad = p.cu_q[0] != 0 || p.cu_q[p.B] > p.T;
+        for (int b = lane; b < p.B; b += 32) bad |= p.cu_q[b + 1] < p.cu_q[b];
+        if (bad) latch(p.err, MOE_ERR_BAD_IDS);
+      }
     }
   } else {
     // ---------------- softmax: one row per thread ----------------
@@ -908,7 +924,7 @@ moe_status launch_prefill(const moe_attn& a, const PrefillParams& p, cudaStream_
   // every sequence wastes less than one item
   const int64_t items = ((int64_t)p.T / span + std::min(p.B, p.T)) * p.kv_heads;
   if (items > 0x3fffffff) return fail(MOE_ERR_INVALID, "moe_attn_prefill: too many rows");
-  const int grid = (int)std::min<int64_t>(a.sms, items * MAX_CUT);
+  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(a.sms, items * MAX_CUT));
   // strides of dimensions of size 1 are never used and may be anything
   const int64_t ts = p.T > 1 ? p.q_token_stride : (int64_t)p.heads * a.d.head_dim;
   const int64_t hs = p.heads > 1 ? p.q_head_stride : a.d.head_dim;

@@ -252,7 +252,7 @@ class PagedAttention:
     def prefill(self, q, cu_q, seq_lens, page_table, out=None, lse=None, return_lse=False, stream=None):
         """Causal attention of prompt chunks that append has written: q [T, num_heads, head_dim], sequence b's rows
         cu_q[b] .. cu_q[b + 1] - 1 (cu_q [B + 1] int32), the last of its seq_lens[b] cached tokens. Returns y
-        [T, num_heads, head_dim], or (y, lse)."""
+        [T, num_heads, head_dim], or (y, lse). Rows from cu_q[B] on are padding: zeros and lse = -inf."""
         if stream is not None:
             return run_on(stream, self._index, self.prefill, q, cu_q, seq_lens, page_table, out=out, lse=lse,
                           return_lse=return_lse)

@@ -58,3 +58,86 @@ def test_a_long_flat_tail_behind_a_score_without_a_value(M, dtype, D, op):
     off = (y.double() * (1 + t) / t - 1).abs().max()
     assert off <= U[dtype] + weights + 2 * adds, off
     assert (lse.double() - (17.5 + math.log1p(t))).abs().max() <= adds + 2.0 ** -18
+
+
+# ---- rows that no sequence holds ----------------------------------------------------------------------
+
+
+def prompt(M, lens, heads=4, kv=2, D=64, dtype=BF16, page=16):
+    """A handle over random pools, the query rows and the arguments of a prefill of whole prompts."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    pages = [-(-n // page) for n in lens]
+    shape = (sum(pages) + 1, kv, page, D)
+    k, v = (torch.randn(shape, generator=g, device="cuda").to(dtype) for _ in range(2))
+    table = torch.zeros((len(lens), max(pages, default=1) or 1), dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(pages):
+        table[b, :n] = torch.arange(at, at + n)
+        at += n
+    q = torch.randn((sum(lens), heads, D), generator=g, device="cuda").to(dtype)
+    cu = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    return M.PagedAttention(M.AttentionConfig(heads, kv, D), k, v, max_seqs=8), q, cu, table.cuda()
+
+
+def refused(M, att):
+    with pytest.raises(M.MoeError) as e:
+        att.check()
+    assert e.value.status == 5, e.value
+
+
+def filled(q, rows):
+    """Outputs of `rows` rows that hold something else before the call."""
+    return (torch.full((rows,) + q.shape[1:], 7.0, dtype=q.dtype, device="cuda"),
+            torch.full((rows, q.shape[1]), 7.0, device="cuda"))
+
+
+@pytest.mark.parametrize("D,pad", [(64, 1), (128, 37), (64, 700)])
+def test_prefill_padding_rows_are_zero(M, D, pad):
+    lens = [5, 0, 70, 129]
+    att, q, cu, table = prompt(M, lens, D=D)
+    want, wl = att.prefill(q, i32(cu), i32(lens), table, return_lse=True)
+    wide = torch.cat([q, torch.full((pad,) + q.shape[1:], float("nan"), dtype=q.dtype, device="cuda")])
+    y, lse = filled(q, len(wide))
+    att.prefill(wide, i32(cu), i32(lens), table, out=y, lse=lse)
+    att.check()
+    n = len(q)
+    assert torch.equal(y[:n], want) and torch.equal(lse[:n], wl)
+    assert not y[n:].any() and torch.isneginf(lse[n:]).all()
+
+
+def test_prefill_graph_of_the_largest_batch_serves_smaller_ones(M):
+    lens = [40, 90, 17]
+    att, q, cu, table = prompt(M, lens)
+    want = att.prefill(q, i32(cu), i32(lens), table)
+    c, n = i32(cu), i32(lens)
+    y, lse = filled(q, len(q))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        att.prefill(q, c, n, table, out=y, lse=lse)
+    for live in (3, 1, 0, 2):
+        y.fill_(7.0), lse.fill_(7.0)
+        c.copy_(i32([cu[min(i, live)] for i in range(4)])), n.copy_(i32(lens[:live] + [0] * (3 - live)))
+        graph.replay()
+        att.check()
+        rows = cu[live]
+        assert torch.equal(y[:rows], want[:rows]) and not y[rows:].any()
+        assert torch.isfinite(lse[:rows]).all() and torch.isneginf(lse[rows:]).all()
+
+
+def test_prefill_without_a_sequence(M):
+    att, q, _, table = prompt(M, [33])
+    y, lse = filled(q, len(q))
+    att.prefill(q, i32([0]), i32([]), table[:0], out=y, lse=lse)
+    att.check()
+    assert not y.any() and torch.isneginf(lse).all()
+
+
+@pytest.mark.parametrize("cu", [[2, 5, 20], [0, 25, 20], [0, 8, 21], [-1, 8, 20], [0, 30, 20]])
+def test_prefill_reports_row_offsets_that_do_not_fit(M, cu):
+    att, q, _, table = prompt(M, [12, 8])
+    y, lse = filled(q, len(q))
+    att.prefill(q, i32(cu), i32([64, 64]), table.repeat(1, 4), out=y, lse=lse)
+    refused(M, att)
+    first = max(cu[0], 0)
+    assert not y[:first].any() and torch.isneginf(lse[:first]).all() and torch.isfinite(lse[first:]).all()
+    att.check()
