@@ -57,9 +57,18 @@ def kv_pools(num_pages: int, num_kv_heads: int, page_size: int, head_dim: int, d
 
 
 def page_slots(page_table, seqs, positions, page_size: int):
-    """The cache slots ([T] int64) of tokens at `positions` of sequences `seqs` (CUDA int tensors), for append."""
-    pos = positions.long()
-    return page_table[seqs.long(), pos // page_size].long() * page_size + pos % page_size
+    """The cache slots ([T] int64) of tokens at `positions` of sequences `seqs` (CUDA int tensors), for append. A token
+    without a page (an entry below 0, a position or sequence outside the table) gets -2, which append reports; -1 would
+    pass for padding."""
+    torch = _torch()
+    pos, seq = positions.long(), seqs.long()
+    rows, width = page_table.shape
+    if not rows or not width:
+        return torch.full_like(pos, -2)
+    col = pos.div(page_size, rounding_mode="floor")
+    page = page_table[seq.clamp(0, rows - 1), col.clamp(0, width - 1)].long()
+    here = (page >= 0) & (pos >= 0) & (col < width) & (seq >= 0) & (seq < rows)
+    return torch.where(here, page * page_size + pos % page_size, -2)
 
 
 def _invalid(msg: str):
