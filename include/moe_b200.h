@@ -573,6 +573,10 @@ moe_status moe_attn_decode(moe_attn* attn, const void* q, int64_t q_token_stride
 moe_status moe_attn_prefill(moe_attn* attn, const void* q, int64_t q_token_stride, int64_t q_head_stride,
                             const int32_t* cu_q, const int32_t* seq_lens, const int32_t* page_table, int max_pages,
                             int B, int T, void* y, float* lse, void* stream);
+/* How long a device-side wait of moe_attn_prefill between its own warps lasts, in SM clocks (1 .. 400000000, the default:
+ * about 200 ms). One that runs out is latched as MOE_ERR_TIMEOUT; the call's output is then not valid, and further calls of
+ * moe_attn_prefill on the handle do nothing until moe_attn_check. */
+moe_status moe_attn_set_wait_limit(moe_attn* attn, int64_t sm_clocks);
 /* Synchronises `stream`, then reads and clears the handle's error word: MOE_OK, MOE_ERR_BAD_IDS or
  * MOE_ERR_TIMEOUT. */
 moe_status moe_attn_check(moe_attn* attn, void* stream);

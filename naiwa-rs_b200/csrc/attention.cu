@@ -290,6 +290,7 @@ extern "C" moe_status moe_attn_create(const moe_attn_desc* desc, moe_attn** out)
     if (!a) return fail(MOE_ERR_OOM, "moe_attn_create: host allocation failed");
     a->d = *desc;
     a->group = desc->num_heads / desc->num_kv_heads;
+    a->wait_limit = (uint32_t)WAIT_CYCLES;
     a->scale = desc->scale > 0.0f ? desc->scale : 1.0f / std::sqrt((float)desc->head_dim);
     a->page_stride =
         desc->page_stride ? desc->page_stride : (int64_t)desc->num_kv_heads * desc->page_size * desc->head_dim;
@@ -438,8 +439,19 @@ extern "C" moe_status moe_attn_prefill(moe_attn* a, const void* q, int64_t q_tok
     p.y = y, p.lse = lse, p.err = a->err;
     p.partial = a->pf_partial, p.partial_ml = a->pf_ml, p.counters = a->pf_counters;
     p.work = a->pf_counters + prefill_counters(*a);
+    p.wait_limit = a->wait_limit;
     DeviceGuard guard(a->d.device);
     return launch_prefill(*a, p, static_cast<cudaStream_t>(stream));
+  });
+}
+
+extern "C" moe_status moe_attn_set_wait_limit(moe_attn* a, int64_t sm_clocks) {
+  return guarded([&]() -> moe_status {
+    const char* me = "moe_attn_set_wait_limit";
+    if (!a) return bad(me, "null handle");
+    if (sm_clocks < 1 || sm_clocks > WAIT_CYCLES) return bad(me, "the limit must be in 1 .. 400000000 SM clocks");
+    a->wait_limit = (uint32_t)sm_clocks;
+    return MOE_OK;
   });
 }
 

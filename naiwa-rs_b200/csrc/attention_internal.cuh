@@ -24,6 +24,7 @@ struct moe_attn {
   float4* pf_partial = nullptr;    // pieces of cut items
   float2* pf_ml = nullptr;
   int32_t* err = nullptr;
+  uint32_t wait_limit;  // SM clocks
   CUtensorMap k_map, v_map;  // prefill's page boxes
 };
 
@@ -75,6 +76,7 @@ struct PrefillParams {
   int32_t* counters;   // arrivals per (item, tile, warp)
   int32_t* work;       // [0] pieces taken, [1] CTAs that have left
   int32_t* err;
+  uint32_t wait_limit;  // SM clocks
 };
 
 // Rows of query heads that one decode work unit holds, and the sizes that follow from them.

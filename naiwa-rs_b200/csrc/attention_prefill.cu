@@ -25,8 +25,8 @@
 // burst peak), 144 under sustained load. Not taken: two threads a row (197 us against 157), an MMA warp per tile (137 against
 // 129), three stages of K or V (129 against 127), exponentials by polynomials (125 to 131 against 126).
 //
-// Every wait is bounded: one that runs out sets MOE_ERR_TIMEOUT, the CTA stops issuing work, waits for its
-// own MMAs and copies, frees its tensor memory and returns.
+// Every wait is bounded (moe_attn_set_wait_limit): one that runs out sets MOE_ERR_TIMEOUT, the CTA stops issuing work, waits for
+// its own MMAs and copies, frees its tensor memory and returns.
 #include <algorithm>
 #include <type_traits>
 
@@ -111,15 +111,42 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-// mbar_wait without the suspend-time hint and in few instructions.
-__device__ __forceinline__ bool wait_poll(uint64_t* bar, uint32_t parity, volatile int* abort) {
+// The bound of this launch's waits: SM clocks, the suspend hint that goes with them, and the flag of a role that gave up.
+struct Waits {
+  uint32_t limit, suspend;
+  volatile int* abort;
+};
+
+// Bounded parity wait that sleeps; false once the limit has passed or another role gave up.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, const Waits& w) {
+  const uint32_t a = smem_u32(bar);
+  uint32_t done;
+  asm volatile(
+      "{.reg .pred p;\n"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;}"
+      : "=r"(done)
+      : "r"(a), "r"(parity)
+      : "memory");
+  if (done) return true;
+  const long long t0 = clock64();
+#pragma unroll 1
+  for (uint32_t i = 0; i < WAIT_POLLS; ++i) {
+    if (*w.abort || clock64() - t0 > w.limit) return false;
+    if (mbar_try_sleep(a, parity, w.suspend)) return true;
+  }
+  return false;
+}
+
+// The same without the suspend-time hint and in few instructions.
+__device__ __forceinline__ bool wait_poll(uint64_t* bar, uint32_t parity, const Waits& w) {
   const uint32_t a = smem_u32(bar);
   uint32_t t0 = 0;
 #pragma unroll 1
   while (!mbar_try(a, parity)) {
     const uint32_t t = (uint32_t)clock() | 1u;
     if (t0 == 0) t0 = t;
-    if (*abort || t - t0 > (uint32_t)WAIT_CYCLES) return false;
+    if (*w.abort || t - t0 > w.limit) return false;
   }
   return true;
 }
@@ -354,7 +381,15 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   __shared__ volatile int s_abort;
   __shared__ int s_k_issued, s_v_issued, s_q_issued;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  volatile int* abort = &s_abort;
+  const Waits waits = {p.wait_limit, min(p.wait_limit, SUSPEND_NS), &s_abort};
+  // The last CTA to leave puts the counter of pieces back for the next call; a CTA that has nothing to do counts as well.
+  auto leave = [&]() {
+    __threadfence();
+    if (atomicAdd(p.work + 1, 1) == (int)gridDim.x - 1) {
+      p.work[0] = 0;
+      p.work[1] = 0;
+    }
+  };
   const int tq = BM / p.group, span = NQ * tq;  // tokens of a tile, of an item
 
   if (tid == 0) {
@@ -378,7 +413,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     mbar_init(&bars.q_free, 1);
     mbar_init(&bars.drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_abort = 0;
     s_k_issued = s_v_issued = s_q_issued = 0;
   }
   if (tid == PF_THREADS - 1) {  // the maps' own latency passes behind the set-up
@@ -391,7 +425,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   proxy_fence();
   pdl_wait();
   pdl_trigger();
-  if (*reinterpret_cast<volatile int32_t*>(p.err) == (int32_t)MOE_ERR_TIMEOUT) return;
+  // after a wait that gave up nothing runs until moe_attn_check; one thread looks, since other CTAs may be setting the word
+  if (tid == 0) s_abort = *reinterpret_cast<volatile int32_t*>(p.err) == (int32_t)MOE_ERR_TIMEOUT;
+  __syncthreads();
+  if (s_abort) {
+    if (tid == 0) leave();
+    return;
+  }
   if (warp == MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(TMEM_COLS));
@@ -405,7 +445,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
   // The n-th piece for a consuming warp; false once a wait gave up. Lane 0 releases the slot.
   auto take = [&](int n, Piece* q) -> bool {
     const int slot = n % RING;
-    const bool ok = __all_sync(FULL, mbar_wait(&bars.item_full[slot], (n / RING) & 1, abort));
+    const bool ok = __all_sync(FULL, wait_for(&bars.item_full[slot], (n / RING) & 1, waits));
     if (!ok) return false;
     *q = s_items[slot];
     __syncwarp();
@@ -441,7 +481,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         } else {
           q = piece_of(p, s_batch[lane], w, span, lane);
           const int slot = n % RING;
-          ok = __all_sync(FULL, n < RING || mbar_wait(&bars.item_free[slot], ((n / RING) - 1) & 1, abort));
+          ok = __all_sync(FULL, n < RING || wait_for(&bars.item_free[slot], ((n / RING) - 1) & 1, waits));
           if (!ok) break;
           if (lane == 0) {
             s_items[slot] = q;
@@ -462,13 +502,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
             latch(p.err, MOE_ERR_BAD_IDS);
             page = p.num_pages;  // out of the map: the box reads as zeros
           }
-          ok = __all_sync(FULL, mbar_wait(&free_[st], ((g / STAGES) & 1) ^ 1, abort));
+          ok = __all_sync(FULL, wait_for(&free_[st], ((g / STAGES) & 1) ^ 1, waits));
           if (!ok) break;
           if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)(live * box_bytes));
           __syncwarp();
           if (on) tma_load_4d(dst + st * S::TILE, map, half * 64, 0, q.kvh, page, &full[st]);
           if (j == 0 && !is_v) {  // Q behind the first K tile: its place is the last to come free
-            ok = __all_sync(FULL, mbar_wait(&bars.q_free, (used & 1) ^ 1, abort));
+            ok = __all_sync(FULL, wait_for(&bars.q_free, (used & 1) ^ 1, waits));
             if (!ok) {
               ++g;
               break;
@@ -493,8 +533,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       }
       // the releases of the last stages have landed before the CTA ends
 #pragma unroll 1
-      for (int c = max(0, g - STAGES); c < g && ok; ++c) ok = mbar_wait(&free_[c % STAGES], (c / STAGES) & 1, abort);
-      if (ok && used > 0) ok = mbar_wait(&bars.q_free, (used - 1) & 1, abort);
+      for (int c = max(0, g - STAGES); c < g && ok; ++c) ok = wait_for(&free_[c % STAGES], (c / STAGES) & 1, waits);
+      if (ok && used > 0) ok = wait_for(&bars.q_free, (used - 1) & 1, waits);
       if (!ok && lane == 0) s_abort = 1;
       __syncwarp();
     } else if (warp == MMA_WARP) {
@@ -506,6 +546,8 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       bool ok = true;
       int g = 0, used = 0;
       uint32_t phase = 0;  // bit i: parity of tile i's next P
+      // bits 2 i, 2 i + 1: tile i has committed scores, their last parity; bits 4 + 2 i, 5 + 2 i: outputs
+      uint32_t committed = 0xaa;
 #pragma unroll 1
       for (int n = 0; ok; ++n) {
         Piece q;
@@ -513,7 +555,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (!ok || uniform(q.b) < 0) break;
         const int steps = uniform(q.steps);
         if (steps == 0) continue;
-        ok = __all_sync(FULL, mbar_wait(&bars.q_full, used & 1, abort));
+        ok = __all_sync(FULL, wait_for(&bars.q_full, used & 1, waits));
         if (!ok) break;
         ++used;
         tc_after();
@@ -523,9 +565,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           // step j of this piece is the CTA's step g + j
           const int sv = (g + j + STAGES) % STAGES, sk = (g + j + 1) % STAGES;
           const bool more = j + 1 < steps;
-          if (more) ok = mbar_wait(&bars.k_full[sk], ((g + j + 1) / STAGES) & 1, abort);
+          if (more) ok = wait_for(&bars.k_full[sk], ((g + j + 1) / STAGES) & 1, waits);
           if (j >= 0) {
-            ok = ok && mbar_wait(&bars.v_full[sv], ((g + j) / STAGES) & 1, abort);
+            ok = ok && wait_for(&bars.v_full[sv], ((g + j) / STAGES) & 1, waits);
             // values past the sequence's length (the rest of its last page, pages not loaded) may be anything, and
             // 0 * NaN is NaN: clear them
             const int valid = q.len - (q.j0 + j) * BN;
@@ -551,7 +593,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
               // the product starts on the first keys' weights while the last ones are being computed
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                ok = __all_sync(FULL, mbar_wait(e ? &bars.p_full[i] : &bars.p_most[i], (phase >> i) & 1, abort));
+                ok = __all_sync(FULL, wait_for(e ? &bars.p_full[i] : &bars.p_most[i], (phase >> i) & 1, waits));
                 if (!ok) break;
                 tc_after();
                 if (elect()) {
@@ -580,16 +622,24 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
               }
             }
             __syncwarp();
+            const int bit = 2 * i + (more ? 0 : 4);
+            committed = (committed | 1u << bit) ^ 2u << bit;
           }
         }
         g += steps;
       }
-      if (!ok) {
-        if (lane == 0) s_abort = 1;
-        if (elect()) commit(&bars.drained);  // every MMA issued so far lands before the CTA goes on
+      if (!ok && lane == 0) s_abort = 1;
+      // Every MMA issued and every arrival of a commit lands before the CTA goes on, whichever role gave up (a softmax warp
+      // may while the last product runs). A CTA that issued none has none to wait for.
+      if (committed & 0x55) {
+        if (elect()) commit(&bars.drained);
         (void)mbar_wait(&bars.drained, 0, nullptr);
-        __syncwarp();
+        for (int i = 0; i < NQ; ++i) {
+          if (committed >> (2 * i) & 1) (void)mbar_wait(&bars.s_full[i], committed >> (2 * i + 1) & 1, nullptr);
+          if (committed >> (4 + 2 * i) & 1) (void)mbar_wait(&bars.o_full[i], committed >> (5 + 2 * i) & 1, nullptr);
+        }
       }
+      __syncwarp();
     } else {
       // ---------------- rows before cu_q[0] and from cu_q[B] on: padding, zeros and -inf ----------------
       const int first = p.B > 0 ? min(max(p.cu_q[0], 0), p.T) : 0;
@@ -640,7 +690,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
       float m = -INFINITY, l = 0.0f;  // reference in units of log2, sum of weights
 #pragma unroll 1
       for (int j = 0; j < q.steps; ++j, ++seen) {
-        ok = wait_poll(&bars.s_full[i], seen & 1, abort);
+        ok = wait_poll(&bars.s_full[i], seen & 1, waits);
         ok = __all_sync(FULL, ok);
         if (!ok) break;
         // S complete means that every product issued before it is: the previous step's with P (O may be rescaled), and
@@ -735,7 +785,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         if (lane == 0) mbar_arrive(&bars.p_full[i]);
       }
       if (ok && q.steps > 0) {
-        ok = __all_sync(FULL, wait_poll(&bars.o_full[i], pieces & 1, abort));
+        ok = __all_sync(FULL, wait_poll(&bars.o_full[i], pieces & 1, waits));
         ++pieces;
         if (ok && frees) mbar_arrive(&bars.v_free[(g + q.steps - 1) % STAGES]);
       }
@@ -881,12 +931,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
         (void)mbar_wait(&bars.v_full[j % STAGES], (j / STAGES) & 1, nullptr);
       atomicExch(p.err, (int)MOE_ERR_TIMEOUT);
     }
-    // the last CTA to leave puts the counter of pieces back for the next call
-    __threadfence();
-    if (atomicAdd(p.work + 1, 1) == (int)gridDim.x - 1) {
-      p.work[0] = 0;
-      p.work[1] = 0;
-    }
+    leave();
   }
   tc_before();
   __syncthreads();

@@ -72,14 +72,14 @@ __device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
 // completes (or about SUSPEND_NS pass) instead of spinning, so waiting roles leave the issue slots
 // to the dequantising warps.
 constexpr uint32_t SUSPEND_NS = 1u << 20;
-__device__ __forceinline__ bool mbar_try_sleep(uint32_t a, uint32_t parity) {
+__device__ __forceinline__ bool mbar_try_sleep(uint32_t a, uint32_t parity, uint32_t suspend_ns = SUSPEND_NS) {
   uint32_t done;
   asm volatile(
       "{.reg .pred p;\n"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
       "selp.u32 %0, 1, 0, p;}"
       : "=r"(done)
-      : "r"(a), "r"(parity), "r"(SUSPEND_NS)
+      : "r"(a), "r"(parity), "r"(suspend_ns)
       : "memory");
   return done != 0;
 }

@@ -197,6 +197,7 @@ def lib():
             "moe_attn_append": (i, [P, P, L64, L64, P, L64, L64, P, L64, L64, i, P, P, P, L64, L64, P]),
             "moe_attn_decode": (i, [P, P, L64, L64, P, P, i, i, P, P, P]),
             "moe_attn_prefill": (i, [P, P, L64, L64, P, P, P, i, i, i, P, P, P]),
+            "moe_attn_set_wait_limit": (i, [P, L64]),
             "moe_attn_check": (i, [P, P]),
             "moe_version": (ctypes.c_char_p, []),
         }

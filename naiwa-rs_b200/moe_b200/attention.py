@@ -158,6 +158,11 @@ class PagedAttention:
         range)."""
         check(lib().moe_attn_check(self._h, self._stream(stream)))
 
+    def set_wait_limit(self, sm_clocks: int):
+        """How long prefill's device-side waits last, in SM clocks (default 400 million, about 200 ms). One that runs out is
+        reported by check() as MOE_ERR_TIMEOUT; until then further prefill calls do nothing."""
+        check(lib().moe_attn_set_wait_limit(self._h, int(sm_clocks)))
+
     # -- argument checks (a small call is a few microseconds on the device: each of these counts) --------------
     def _rows(self, x, heads: int, what: str):
         """(x, token stride, head stride) as rows the kernels take: one head's values consecutive, 16-byte aligned

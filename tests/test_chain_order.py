@@ -90,3 +90,20 @@ def test_loads_in_assembly_are_volatile(path):
     """A load in a plain asm is a pure function to the compiler, which may evaluate it ahead of the test that guards it."""
     for m in re.finditer(r"\basm\s*(volatile\s*)?\(\s*\"([^;]*);", text_of(path)):
         assert m.group(1) or not re.search(r"\b(ld|ldu|ldmatrix|cp|tcgen05|atom|red|st)\b", m.group(2)), m.group(0)
+
+
+def test_prefill_reads_its_error_word_once():
+    """Threads of a CTA that saw different words would part before its barriers and its collective allocation."""
+    body = dict((n, b) for n, _, b in kernels(text_of(os.path.join(CSRC, "attention_prefill.cu"))))["prefill_kernel"]
+    reads = [m.start() for m in re.finditer(r"p\.err\)\s*==", body)]
+    assert len(reads) == 1 and re.search(r"if \(tid == 0\) s_abort = [^;]*$", body[:reads[0]].rstrip("*"))
+    assert body.index("__syncthreads();", reads[0]) < body.index("tcgen05.alloc")
+    stop = body[reads[0]:body.index("tcgen05.alloc")]
+    assert "leave();" in stop, "a CTA that leaves early counts itself"
+
+
+def test_a_commit_follows_an_mma():
+    """No commit in a CTA that has issued no MMA, and none whose arrival nothing waits for."""
+    body = dict((n, b) for n, _, b in kernels(text_of(os.path.join(CSRC, "attention_prefill.cu"))))["prefill_kernel"]
+    at = body.index("commit(&bars.drained)")
+    assert "if (committed & 0x55)" in body[at - 120:at]

@@ -141,3 +141,54 @@ def test_prefill_reports_row_offsets_that_do_not_fit(M, cu):
     first = max(cu[0], 0)
     assert not y[:first].any() and torch.isneginf(lse[:first]).all() and torch.isfinite(lse[first:]).all()
     att.check()
+
+
+# ---- waits that run out -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens,heads,kv,D", [([700, 300], 8, 2, 128), ([3, 1500], 4, 4, 64), ([4000], 2, 2, 128)])
+def test_prefill_waits_that_run_out_are_reported(M, lens, heads, kv, D):
+    """Limits from one clock (the first wait gives up) to about a call's length (some role in the middle of its work does): the
+    call ends, says so, leaves the handle usable, and the next call gives the bits that it always gives."""
+    from moe_b200 import _lib
+
+    att, q, cu, table = prompt(M, lens, heads=heads, kv=kv, D=D)
+    c, n = i32(cu), i32(lens)
+    want = att.prefill(q, c, n, table)
+    gave_up = []
+    for limit in (1, 300, 1000, 2000, 4000, 6000, 8000, 10000, 14000, 20000, 40000):
+        att.set_wait_limit(limit)
+        y = att.prefill(q, c, n, table)
+        still, _ = filled(q, len(q))
+        att.prefill(q, c, n, table, out=still)  # behind a wait that ran out: nothing
+        try:
+            att.check()
+        except M.MoeError as e:
+            assert e.status == _lib.MOE_ERR_TIMEOUT
+            gave_up.append(limit)
+        else:
+            assert torch.equal(y, want) and torch.equal(still, want)
+        att.set_wait_limit(400_000_000)
+        assert torch.equal(att.prefill(q, c, n, table), want)
+        att.check()
+    assert 1 in gave_up
+
+
+def test_prefill_does_nothing_between_a_wait_that_ran_out_and_the_check(M):
+    from moe_b200 import _lib
+
+    att, q, cu, table = prompt(M, [200, 90])
+    c, n = i32(cu), i32([200, 90])
+    want = att.prefill(q, c, n, table)
+    att.set_wait_limit(1)
+    att.prefill(q, c, n, table)
+    att.set_wait_limit(400_000_000)
+    for _ in range(3):
+        y, _ = filled(q, len(q))
+        att.prefill(q, c, n, table, out=y)
+        assert (y == 7.0).all()
+    with pytest.raises(M.MoeError) as e:
+        att.check()
+    assert e.value.status == _lib.MOE_ERR_TIMEOUT
+    assert torch.equal(att.prefill(q, c, n, table), want)
+    att.check()
