@@ -551,8 +551,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM)
 
   pdl_wait();  // the tile list, the gathered tokens and the error word come from earlier kernels
   pdl_trigger();
-  // after any CTA gave up on a wait, the rest of the launch does no work
-  if (p.err && *reinterpret_cast<volatile int32_t*>(p.err) == (int32_t)MOE_ERR_TIMEOUT) return;
+  // after any CTA gave up on a wait, the rest of the launch does no work; one thread looks, since a CTA may be setting the word
+  if (threadIdx.x == 0) s_abort = p.err && *reinterpret_cast<volatile int32_t*>(p.err) == (int32_t)MOE_ERR_TIMEOUT;
+  __syncthreads();
+  if (s_abort) return;
   const int n_items = *p.n_tiles * p.tiles;
   if ((int)blockIdx.x >= n_items) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -581,7 +583,6 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS_PER_SM)
       mbar_init(&item_free[s], item_consumers<C>());
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_abort = 0;
     s_units_issued = 0;
     s_tiles_issued = 0;
   }

@@ -107,3 +107,12 @@ def test_a_commit_follows_an_mma():
     body = dict((n, b) for n, _, b in kernels(text_of(os.path.join(CSRC, "attention_prefill.cu"))))["prefill_kernel"]
     at = body.index("commit(&bars.drained)")
     assert "if (committed & 0x55)" in body[at - 120:at]
+
+
+def test_the_grouped_gemm_reads_its_error_word_once():
+    """As above: before the CTA's first barrier, by one thread."""
+    body = dict((n, b) for n, _, b in kernels(text_of(os.path.join(CSRC, "expert_gemm_tc.cu"))))["expert_gemm_kernel"]
+    assert not re.search(r"MOE_ERR_TIMEOUT\)\s*return", body)
+    read = body.index("p.err) ==")
+    assert "if (threadIdx.x == 0) s_abort = " in body[read - 90:read]
+    assert "__syncthreads();" in body[read:body.index("if (s_abort) return;")] and body.count("s_abort = 0") == 0
