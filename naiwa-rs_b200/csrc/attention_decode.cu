@@ -456,10 +456,15 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t hi = Elem<T>::pack(s[nt][2 * i], s[nt][2 * i + 1]);
+          // Both parts above zero, so that an infinite value stays one (0 * inf and inf - inf are NaN): hi is rounded down, and
+          // each part is at least the type's smallest value, 2^-38 of the largest weight in f16. Values of tokens that are
+          // not seen are zeros in shared memory.
+          constexpr float LEAST = Elem<T>::kLeast;
+          const float a = fmaxf(s[nt][2 * i], LEAST), b = fmaxf(s[nt][2 * i + 1], LEAST);
+          const uint32_t hi = Elem<T>::pack_down(a, b);
           const float2 back = Elem<T>::unpack(hi);
           ph[nt][i] = movmatrix_t(hi);
-          pl[nt][i] = movmatrix_t(Elem<T>::pack(s[nt][2 * i] - back.x, s[nt][2 * i + 1] - back.y));
+          pl[nt][i] = movmatrix_t(Elem<T>::pack(fmaxf(a - back.x, LEAST), fmaxf(b - back.y, LEAST)));
         }
       }
       {

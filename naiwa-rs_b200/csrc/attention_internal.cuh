@@ -106,6 +106,12 @@ struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
   static constexpr int kWeightBits = 0;
+  static constexpr float kLeast = 1.17549435e-38f;  // smallest normal value
+  static __device__ __forceinline__ uint32_t pack_down(float lo, float hi) {  // towards zero
+    uint32_t v;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+    return v;
+  }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static __device__ __forceinline__ float2 unpack(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
@@ -117,6 +123,12 @@ struct Elem<__nv_bfloat16> {
 template <>
 struct Elem<__half> {
   static constexpr int kWeightBits = 15;
+  static constexpr float kLeast = 5.9604645e-08f;  // smallest value
+  static __device__ __forceinline__ uint32_t pack_down(float lo, float hi) {
+    uint32_t v;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+    return v;
+  }
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
   static __device__ __forceinline__ float2 unpack(uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));

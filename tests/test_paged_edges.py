@@ -192,3 +192,91 @@ def test_prefill_does_nothing_between_a_wait_that_ran_out_and_the_check(M):
     assert e.value.status == _lib.MOE_ERR_TIMEOUT
     assert torch.equal(att.prefill(q, c, n, table), want)
     att.check()
+
+
+# ---- infinities and NaN among the values ---------------------------------------------------------------
+
+
+def plain_row(q, k, v, scale):
+    """One query row of one head over the keys it sees, in 64 bits."""
+    p = torch.softmax((k.double() @ q.double()) * scale, 0)
+    return p @ v.double()
+
+
+def same_kind(got, want, bound):
+    """NaN where the definition gives NaN, the same infinities, and finite values within the bound."""
+    got, want = got.double().cpu(), want.cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), (got, want)
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf]) and torch.isfinite(got[~inf & ~torch.isnan(want)]).all()
+    ok = torch.isfinite(want)
+    assert ((got - want)[ok].abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,D,n", [(2, 64, 1), (8, 128, 37), (24, 64, 300), (3, 128, 5000)])
+def test_decode_infinite_and_nan_values_reach_what_sees_them(M, dtype, heads, D, n):
+    """An infinite value gives an infinite output in its column and no other, a NaN value a NaN there; a NaN key makes the whole row NaN;
+    values outside the window or past the length reach nothing. Scores within +-2, so every weight counts. Bound: u of
+    the largest value and twice u of the weights (the definition's own scale), with |v| below 8."""
+    inf, nan = math.inf, math.nan
+    window = 200
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for what in ("inf", "-inf", "both", "nan value", "nan key", "nan row", "outside"):
+        k, v, table = one_sequence(n + 30, 1, D, 16, dtype)
+        k.copy_(torch.randn(k.shape, generator=g, device="cuda") * 0.1), v.copy_(torch.randn(v.shape, generator=g, device="cuda"))
+        v.clamp_(-7, 7)
+        q = torch.randn((1, heads, D), generator=g, device="cuda").clamp_(-3, 3).to(dtype)
+        at = n - 1 - min(n, window) // 3
+        if what in ("inf", "both"):
+            v[at // 16, 0, at % 16, 3] = inf
+        if what == "-inf":
+            v[at // 16, 0, at % 16, 3] = -inf
+        if what == "both" and n > 1:
+            v[(n - 1) // 16, 0, (n - 1) % 16, 3] = -inf
+        if what == "nan value":
+            v[at // 16, 0, at % 16, 5] = nan
+        if what == "nan key":
+            k[at // 16, 0, at % 16, 5] = nan
+        if what == "nan row":
+            q[0, 1, 7] = nan
+        for past in range(n, n + 30):
+            k[past // 16, 0, past % 16], v[past // 16, 0, past % 16] = (nan, inf) if past % 2 else (inf, nan)
+        if what == "outside" and n > window:
+            v[0, 0, 0], k[0, 0, 0] = nan, nan
+        att = M.PagedAttention(M.AttentionConfig(heads, 1, D, window=window), k, v, max_seqs=1)
+        y = att.decode(q, i32([n]), table)
+        att.check()
+        rows = slice(max(0, n - window), n)
+        ks, vs = (p.transpose(1, 2).reshape(-1, D)[rows] for p in (k, v))
+        for h in range(heads):
+            same_kind(y[0, h], plain_row(q[0, h], ks, vs, D ** -0.5), 8 * 3 * U[dtype])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_prefill_infinite_and_nan_values_reach_the_rows_that_see_them(M, dtype):
+    """Rows from the value's position on: as decode. Other columns, other heads' values and other sequences: untouched."""
+    lens, D = [150, 90], 128
+    att, q, cu, table = prompt(M, lens, heads=4, kv=2, D=D, dtype=dtype)
+    c, n = i32(cu), i32(lens)
+    clean = att.prefill(q, c, n, table)
+    k, v = att._keep[0], att._keep[1]
+    at, page = 70, int(table[0, 70 // 16])
+    for bad in (math.inf, -math.inf, math.nan):
+        keep = v[page, 1, at % 16, 9].clone()
+        v[page, 1, at % 16, 9] = bad
+        y = att.prefill(q, c, n, table)
+        att.check()
+        v[page, 1, at % 16, 9] = keep
+        seen = y[at:150, 2:, 9].float()  # the heads of key/value head 1
+        assert torch.isnan(seen).all() if math.isnan(bad) else (seen == bad).all()
+        y[:150, 2:, 9] = clean[:150, 2:, 9]
+        assert torch.equal(y, clean)
+    keep = k[page, 1, at % 16, 9].clone()
+    k[page, 1, at % 16, 9] = math.nan
+    y = att.prefill(q, c, n, table)
+    k[page, 1, at % 16, 9] = keep
+    assert torch.isnan(y[at:150, 2:]).all()
+    y[at:150, 2:] = clean[at:150, 2:]
+    assert torch.equal(y, clean)
+    att.check()
