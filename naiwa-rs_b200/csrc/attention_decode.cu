@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
 
   const float c_log2 = p.scale * LOG2E;
   const bool capped = p.softcap > 0.0f;
-  const float cap_in = capped ? 2.0f * c_log2 / p.softcap : 0.0f, cap_out = p.softcap * LOG2E;
+  const Cap cap = make_cap(p.scale, capped ? p.softcap : 1.0f);
   const int g8 = lane >> 2, t4 = lane & 3;
   int use = 0;
   int idx = start;  // first block of the piece
@@ -429,8 +429,7 @@ __global__ void __launch_bounds__(THREADS, CTAS_PER_SM) decode_kernel(DecodePara
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v = s[nt][i] + s2[nt][i];
-          // capped: tanh(x) = 1 - 2 / (e^2x + 1), absolute error about 1e-7 of the cap
-          v = capped ? cap_out - __fdividef(2.0f * cap_out, ex2(v * cap_in) + 1.0f) : v * c_log2;
+          v = !capped ? v * c_log2 : cap.wide ? wide_capped_score(cap, v) : capped_score(cap, v);
           s[nt][i] = (i < 2 ? in0 : in1) ? v : -INFINITY;  // in units of log2
         }
         float corr[2];

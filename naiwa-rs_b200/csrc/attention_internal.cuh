@@ -151,6 +151,29 @@ __device__ __forceinline__ float ex2_ordered(float x) {
   return y;
 }
 
+// softcap * tanh(x / softcap) in units of log2, of scores v before their scale. softcap * (1 - 2 / (e^2t + 1)), t = x / softcap,
+// is off by about 2^-23 of the cap, however small the score is; caps above WIDE_CAP, of which that would be
+// more than a weight can take, use tanh's series t - t^3 / 3 + 2 t^5 / 15 - 17 t^7 / 315 + 62 t^9 / 2835 (2^-26 relative) for |t| < 1/4.
+struct Cap {
+  float in, out, slope, gain;  // 2 / ln 2 * scale / softcap, softcap / ln 2, scale / softcap, scale / ln 2
+  bool wide;
+};
+constexpr float WIDE_CAP = 64.0f;
+
+__device__ __forceinline__ Cap make_cap(float scale, float softcap) {
+  return {fminf(2.0f * LOG2E * scale / softcap, 3.0e38f), softcap * LOG2E, scale / softcap, scale * LOG2E, softcap > WIDE_CAP};
+}
+
+__device__ __forceinline__ float capped_score(const Cap& c, float v) {
+  return c.out - __fdividef(2.0f * c.out, ex2(v * c.in) + 1.0f);
+}
+
+__device__ __forceinline__ float wide_capped_score(const Cap& c, float v) {
+  const float t = v * c.slope, t2 = t * t;
+  const float r = fmaf(t2, fmaf(t2, fmaf(t2, fmaf(t2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+  return fabsf(t) < 0.25f ? v * c.gain * r : capped_score(c, v);
+}
+
 __device__ __forceinline__ void latch(int32_t* err, moe_status st) { atomicCAS(err, 0, (int32_t)st); }
 
 }  // namespace attn

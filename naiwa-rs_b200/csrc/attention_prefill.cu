@@ -667,7 +667,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t s_at = lane_base + S_COL + i * BN, o_at = lane_base + O_COL + i * D;
     const float c_log2 = CAP ? 1.0f : p.scale * LOG2E;
-    const float cap_in = CAP ? 2.0f * LOG2E * p.scale / p.softcap : 0.0f, cap_out = p.softcap * LOG2E;
+    const Cap cap = make_cap(p.scale, CAP ? p.softcap : 1.0f);
     bool ok = true;
     int seen = 0;           // this tile's steps so far
     int g = 0, pieces = 0;  // the CTA's steps so far, this tile's pieces
@@ -707,10 +707,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           tmem_ld32(s_at + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
         tmem_wait_ld();
         if (CAP) {
-          // softcap * tanh(x) = softcap * (1 - 2 / (e^2x + 1)), absolute error about 1e-7 of the cap
+          if (cap.wide) {
 #pragma unroll
-          for (int k = 0; k < BN; ++k)
-            r[k] = __float_as_uint(cap_out - __fdividef(2.0f * cap_out, ex2(__uint_as_float(r[k]) * cap_in) + 1.0f));
+            for (int k = 0; k < BN; ++k) r[k] = __float_as_uint(wide_capped_score(cap, __uint_as_float(r[k])));
+          } else {
+#pragma unroll
+            for (int k = 0; k < BN; ++k) r[k] = __float_as_uint(capped_score(cap, __uint_as_float(r[k])));
+          }
         }
         const int base = (q.j0 + j) * BN;
         // keys that every live row of the tile sees need no mask

@@ -280,3 +280,36 @@ def test_prefill_infinite_and_nan_values_reach_the_rows_that_see_them(M, dtype):
     y[at:150, 2:] = clean[at:150, 2:]
     assert torch.equal(y, clean)
     att.check()
+
+
+# ---- large caps ----------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("softcap", [60.0, 70.0, 1000.0, 1e5, 1e30, 3e38])
+@pytest.mark.parametrize("size", [1.5, 60.0])
+def test_large_caps(M, dtype, softcap, size):
+    """A cap far above the scores leaves them as they are, and one near them bends them exactly, however large it is: the bound
+    is that of uncapped scores (tests/attention_oracle.py), plus the formula's 2^-21 of the cap up to 64 and 2^-21 of the score
+    above, twice per weight."""
+    import attention_oracle as AO
+
+    lens, heads, kv, D = [130, 77], 4, 2, 64
+    att, q, cu, table = prompt(M, lens, heads=heads, kv=kv, D=D, dtype=dtype)
+    k, v = att._keep[0], att._keep[1]
+    q = (q * size).to(dtype)
+    att = M.PagedAttention(M.AttentionConfig(heads, kv, D, softcap=softcap), k, v, max_seqs=2)
+    y, lse = att.prefill(q, i32(cu), i32(lens), table, return_lse=True)
+    last = torch.tensor([c - 1 for c in cu[1:]], device="cuda")
+    z, zl = att.decode(q[last].contiguous(), i32(lens), table, return_lse=True)
+    att.check()
+    # a cap whose f64 tanh is its argument to the last bit: the oracle's softcap * tanh(x / softcap) is exact enough at 1e30
+    want = AO.run(q, k, v, table, lens, cu, 1 / math.sqrt(D), softcap, 0, AO.U[dtype])
+    loose = AO.run(q, k, v, table, lens, cu, 1 / math.sqrt(D), 0.0, 0, AO.U[dtype])
+    extra = 2.0 ** -21 * min(softcap, 64.0) if softcap <= 64 else 0.0
+    vmax = v.double().abs().max().item()
+    yb, lb = loose[1] + 4 * extra * vmax + 2 * AO.U[dtype] * vmax, loose[3] + 2 * extra
+    AO.assert_within(y, want[0], yb, "prefill")
+    AO.assert_within(lse, want[2], lb, "prefill lse")
+    AO.assert_within(z, want[0][last.cpu()], yb[last.cpu()], "decode")
+    AO.assert_within(zl, want[2][last.cpu()], lb[last.cpu()], "decode lse")
