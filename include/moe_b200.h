@@ -500,7 +500,8 @@ moe_status moe_requantize_q2_0(int src_dtype, const void* src, int E, int N, int
  * aligned and strides are multiples of 8. Query head h reads key/value head
  * h / (num_heads / num_kv_heads). Sums, softmax statistics and norms are held in f32.
  *
- * Slots past a sequence's length and pages past its last are never used and may hold anything. Device-
+ * Slots past a sequence's length and pages past its last are never used and may hold anything; with a window so may
+ * pages wholly behind the first position that a row sees (their table entries too). Device-
  * side errors (a slot, page or position out of range, a length past the page table) never read or write
  * out of bounds; they are latched and reported by moe_attn_check. One moe_attn's calls must not overlap
  * on the GPU (one stream, or streams ordered by events): they share its workspace. Every call enqueues

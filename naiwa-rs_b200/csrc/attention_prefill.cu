@@ -262,9 +262,9 @@ struct Bars {
 };
 
 // A piece of work: steps [j0, j0 + steps) over the keys of one item. row0: the sequence's first row; past: the position
-// of that row; [t0, t1): the item's tokens. b < 0: no more work.
+// of that row; [t0, t1): the item's tokens; lo: the first key that one of them sees. b < 0: no more work.
 struct Piece {
-  int b, kvh, row0, past, t0, t1, len, j0, steps, cut, k, item;
+  int b, kvh, row0, past, t0, t1, len, lo, j0, steps, cut, k, item;
 };
 
 // The batch as the load warp sees it: each lane holds the tiles of its sequences and their prefix.
@@ -347,8 +347,8 @@ __device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s
   q.t0 = tile * span;
   q.t1 = min(news, q.t0 + span);
   const int hi = max(0, q.past + q.t1);  // keys [lo, hi)
-  const int lo = p.window > 0 ? max(0, q.past + q.t0 - p.window + 1) : 0;
-  const int first = lo / BN, all = hi > lo ? (hi + BN - 1) / BN - first : 0;
+  q.lo = p.window > 0 ? max(0, q.past + q.t0 - p.window + 1) : 0;
+  const int first = q.lo / BN, all = hi > q.lo ? (hi + BN - 1) / BN - first : 0;
   const int a = all * q.k / q.cut;  // all < 2^24, cut <= MAX_CUT
   q.j0 = first + a;
   q.steps = all * (q.k + 1) / q.cut - a;
@@ -495,8 +495,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 #pragma unroll 1
         for (int j = 0; j < q.steps; ++j, ++g) {
           const int base = (q.j0 + j) * BN, st = g % STAGES;
-          const int live = min(pages, (q.len - base + box_rows - 1) >> p.page_shift);  // pages that hold tokens
-          const bool on = my < live;
+          // pages that hold tokens which a row sees: not those past the length, nor those wholly behind the window
+          const int end = min(pages, (q.len - base + box_rows - 1) >> p.page_shift);
+          const int begin = max(0, q.lo - base) >> p.page_shift;
+          const bool on = my >= begin && my < end;
           int page = on ? table[base >> p.page_shift] : 0;
           if ((unsigned)page >= (unsigned)p.num_pages) {
             latch(p.err, MOE_ERR_BAD_IDS);
@@ -504,7 +506,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           }
           ok = __all_sync(FULL, wait_for(&free_[st], ((g / STAGES) & 1) ^ 1, waits));
           if (!ok) break;
-          if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)(live * box_bytes));
+          if (lane == 0) mbar_expect_tx(&full[st], (uint32_t)((end - begin) * box_bytes));
           __syncwarp();
           if (on) tma_load_4d(dst + st * S::TILE, map, half * 64, 0, q.kvh, page, &full[st]);
           if (j == 0 && !is_v) {  // Q behind the first K tile: its place is the last to come free
@@ -568,13 +570,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
           if (more) ok = wait_for(&bars.k_full[sk], ((g + j + 1) / STAGES) & 1, waits);
           if (j >= 0) {
             ok = ok && wait_for(&bars.v_full[sv], ((g + j) / STAGES) & 1, waits);
-            // values past the sequence's length (the rest of its last page, pages not loaded) may be anything, and
-            // 0 * NaN is NaN: clear them
-            const int valid = q.len - (q.j0 + j) * BN;
-            if (valid < BN && __all_sync(FULL, ok)) {
+            // values past the sequence's length (the rest of its last page, pages not loaded) and behind the window may be
+            // anything, and 0 * NaN is NaN: clear them, rows [0, head) and [valid, BN)
+            const int valid = min(BN, q.len - (q.j0 + j) * BN), head = max(0, q.lo - (q.j0 + j) * BN);
+            if ((valid < BN || head > 0) && __all_sync(FULL, ok)) {
 #pragma unroll 1
-              for (int e = lane; e < (BN - valid) * (D / 8); e += 32) {
-                const int r = valid + e / (D / 8), c = e % (D / 8);
+              for (int e = lane; e < (BN - valid + head) * (D / 8); e += 32) {
+                const int at = e / (D / 8), r = at < head ? at : valid + at - head, c = e % (D / 8);
                 *reinterpret_cast<uint4*>(sV + sv * S::TILE + (c / 8) * S::SLAB + r * 128 + ((c & 7) << 4)) =
                     make_uint4(0, 0, 0, 0);
               }

@@ -313,3 +313,38 @@ def test_large_caps(M, dtype, softcap, size):
     AO.assert_within(lse, want[2], lb, "prefill lse")
     AO.assert_within(z, want[0][last.cpu()], yb[last.cpu()], "decode")
     AO.assert_within(zl, want[2][last.cpu()], lb[last.cpu()], "decode lse")
+
+
+# ---- pages behind the window ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("D,page,window", [(64, 16, 40), (128, 16, 1), (128, 32, 200), (64, 64, 130), (128, 128, 300)])
+@pytest.mark.parametrize("entry", ["none", "reused"])
+def test_pages_behind_the_window_are_not_read(M, D, page, window, entry):
+    """A cache that frees pages behind the window: their table entries name nothing, or pages that hold something else (NaN and
+    infinities here). The rows' outputs are those of the full cache, bit for bit."""
+    heads, kv, rows, lens = 4, 2, [70, 3, 200], [900, 513, 640]
+    g = torch.Generator(device="cuda").manual_seed(8)
+    need = [-(-n // page) for n in lens]
+    shape = (sum(need) + 1, kv, page, D)
+    k, v = (torch.randn(shape, generator=g, device="cuda").to(BF16) for _ in range(2))
+    k[-1], v[-1] = math.inf, math.nan
+    table = torch.zeros((3, max(need)), dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(need):
+        table[b, :n] = torch.arange(at, at + n)
+        at += n
+    cut = table.clone()
+    for b in range(3):
+        first = max(0, lens[b] - rows[b] - window + 1)  # of the chunk's first row
+        cut[b, :first // page] = -1 if entry == "none" else shape[0] - 1
+    cu = [0, 70, 73, 273]
+    q = torch.randn((273, heads, D), generator=g, device="cuda").to(BF16)
+    att = M.PagedAttention(M.AttentionConfig(heads, kv, D, window=window), k, v, max_seqs=3)
+    want = att.prefill(q, i32(cu), i32(lens), table.cuda(), return_lse=True)
+    got = att.prefill(q, i32(cu), i32(lens), cut.cuda(), return_lse=True)
+    att.check()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    last = q[torch.tensor([69, 72, 272], device="cuda")].contiguous()
+    assert torch.equal(att.decode(last, i32(lens), cut.cuda()), att.decode(last, i32(lens), table.cuda()))
+    att.check()
