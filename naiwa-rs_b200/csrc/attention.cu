@@ -397,7 +397,7 @@ extern "C" moe_status moe_attn_decode(moe_attn* a, const void* q, int64_t q_toke
     if (!a) return bad(me, "null handle");
     if (B < 0 || B > a->d.max_seqs) return bad(me, "B must be in 0 .. max_seqs");
     if (B == 0) return MOE_OK;
-    if (!q || !seq_lens || !page_table || !y || max_pages <= 0) return bad(me, "null pointer or no pages");
+    if (!q || !seq_lens || !y || max_pages < 0 || (max_pages && !page_table)) return bad(me, "null pointer or no pages");
     if (!rows_ok(q, q_token_stride, q_head_stride) || ((uintptr_t)y & 15))
       return bad(me, "rows must be 16-byte aligned with strides that are multiples of 8");
     if ((int64_t)max_pages * a->d.page_size > 0x7fffffffll) return bad(me, "max_pages * page_size above 2^31 - 1");
@@ -424,7 +424,7 @@ extern "C" moe_status moe_attn_prefill(moe_attn* a, const void* q, int64_t q_tok
     if (!a) return bad(me, "null handle");
     if (B < 0 || T < 0) return bad(me, "B and T must not be negative");
     if (T == 0) return MOE_OK;
-    if (!q || !y || (B > 0 && (!cu_q || !seq_lens || !page_table || max_pages <= 0)))
+    if (!q || !y || max_pages < 0 || (B > 0 && (!cu_q || !seq_lens || (max_pages && !page_table))))
       return bad(me, "null pointer or no pages");
     if (!rows_ok(q, q_token_stride, q_head_stride) || ((uintptr_t)y & 15))
       return bad(me, "rows must be 16-byte aligned with strides that are multiples of 8");

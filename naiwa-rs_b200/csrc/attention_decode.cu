@@ -595,7 +595,7 @@ moe_status launch_decode(const moe_attn& a, const DecodeParams& p, cudaStream_t 
   const int64_t bound = (widest * p.B * p.kv_heads * p.row_blocks + MIN_SLICE - 1) / MIN_SLICE;
   if (widest * p.B * p.kv_heads * p.row_blocks > 0x3fffffffll)
     return fail(MOE_ERR_INVALID, "moe_attn_decode: B * num_kv_heads * max_pages * page_size / 16 must be below 2^30");
-  const int grid = (int)std::min<int64_t>(decode_max_ctas(a.sms), bound);
+  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(decode_max_ctas(a.sms), bound));
   return with_kernel(a, [&](auto kernel, int smem) -> moe_status {
     MOE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(THREADS), smem, st, p));
     return MOE_OK;

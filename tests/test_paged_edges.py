@@ -348,3 +348,25 @@ def test_pages_behind_the_window_are_not_read(M, D, page, window, entry):
     last = q[torch.tensor([69, 72, 272], device="cuda")].contiguous()
     assert torch.equal(att.decode(last, i32(lens), cut.cuda()), att.decode(last, i32(lens), table.cuda()))
     att.check()
+
+
+# ---- the smallest table, the largest window --------------------------------------------------------------
+
+
+def test_an_empty_page_table_serves_empty_sequences(M):
+    """No sequence has a page yet: zeros and -inf, as for a sequence of length 0 in a larger table; a length that the table does
+    not hold is reported."""
+    att, q, _, table = prompt(M, [5])
+    none = table.new_empty((3, 0))
+    y, lse = filled(q, 3)
+    att.decode(q[:3], i32([0, 0, 0]), none, out=y, lse=lse)
+    att.check()
+    assert not y.any() and torch.isneginf(lse).all()
+    y, lse = filled(q, len(q))
+    att.prefill(q, i32([0, 0, 0, 0]), i32([0, 0, 0]), none, out=y, lse=lse)
+    att.check()
+    assert not y.any() and torch.isneginf(lse).all()
+    y, _ = filled(q, 3)
+    att.decode(q[:3], i32([0, 1, 0]), none, out=y)
+    refused(M, att)
+    assert not y.any()
