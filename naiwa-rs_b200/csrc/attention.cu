@@ -23,6 +23,8 @@ namespace attn {
 //   out_a = inv (a (w_a c) - b (w_b s)),  out_b = inv (b (w_b c) + a (w_a s)),  inv = 1 / sqrt(mean(x^2) + eps).
 // Blocks are (lanes of a row, lane groups, tokens), so a thread finds its work without a division.
 constexpr int APPEND_THREADS = 256;
+// A window above this (2,080,374,784 positions) is none: position arithmetic beside it would leave 32 bits.
+constexpr int MAX_WINDOW = 0x7c000000;
 // Rows per lane group, measured at 4096 tokens of 32 + 2 x 4 heads of 128: 2 rows 33.8 us, 4: 20.2 (4.3 TB/s), 8: 21.2.
 constexpr int ROWS = 4;
 
@@ -289,6 +291,7 @@ extern "C" moe_status moe_attn_create(const moe_attn_desc* desc, moe_attn** out)
     moe_attn* a = new (std::nothrow) moe_attn();
     if (!a) return fail(MOE_ERR_OOM, "moe_attn_create: host allocation failed");
     a->d = *desc;
+    if (a->d.window > MAX_WINDOW) a->d.window = 0;
     a->group = desc->num_heads / desc->num_kv_heads;
     a->wait_limit = (uint32_t)WAIT_CYCLES;
     a->scale = desc->scale > 0.0f ? desc->scale : 1.0f / std::sqrt((float)desc->head_dim);

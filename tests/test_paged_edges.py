@@ -370,3 +370,16 @@ def test_an_empty_page_table_serves_empty_sequences(M):
     att.decode(q[:3], i32([0, 1, 0]), none, out=y)
     refused(M, att)
     assert not y.any()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 200, 2 ** 30])
+def test_a_window_longer_than_any_sequence_is_none(M, window):
+    """Bit for bit: few long items are cut along their keys, and the cut follows from the window."""
+    lens = [4000, 129]
+    att, q, cu, table = prompt(M, lens, D=128)
+    other = M.PagedAttention(M.AttentionConfig(4, 2, 128, window=window), att._keep[0], att._keep[1], max_seqs=2)
+    args = (i32(cu), i32(lens), table)
+    assert torch.equal(other.prefill(q, *args), att.prefill(q, *args))
+    last = q[[c - 1 for c in cu[1:]]].contiguous()
+    assert torch.equal(other.decode(last, *args[1:]), att.decode(last, *args[1:]))
+    other.check()
