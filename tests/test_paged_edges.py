@@ -383,3 +383,63 @@ def test_a_window_longer_than_any_sequence_is_none(M, window):
     last = q[[c - 1 for c in cu[1:]]].contiguous()
     assert torch.equal(other.decode(last, *args[1:]), att.decode(last, *args[1:]))
     other.check()
+
+
+# ---- further forms against the definition ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("scale", [0.02, 0.5])
+@pytest.mark.parametrize("softcap,window", [(0.0, 0), (20.0, 77)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_prefill_with_a_scale_of_its_own(M, scale, softcap, window, dtype):
+    import attention_oracle as AO
+
+    lens, D = [150, 301], 64
+    att, q, cu, table = prompt(M, lens, heads=6, kv=2, D=D, dtype=dtype)
+    k, v = att._keep[0], att._keep[1]
+    att = M.PagedAttention(M.AttentionConfig(6, 2, D, scale=scale, softcap=softcap, window=window), k, v, max_seqs=2)
+    y, lse = att.prefill(q, i32(cu), i32(lens), table, return_lse=True)
+    att.check()
+    want = AO.run(q, k, v, table, lens, cu, scale, softcap, window, AO.U[dtype])
+    AO.assert_within(y, want[0], want[1], "y")
+    AO.assert_within(lse, want[2], want[3], "lse")
+
+
+@pytest.mark.parametrize("T,heads,kv,D,rope_dim,sections", [(31, 6, 2, 128, 64, (8, 12, 12)), (5, 3, 3, 64, 32, (1, 0, 15)),
+                                                          (17, 5, 1, 128, 16, (3, 3, 2)), (9, 9, 3, 64, 48, ())])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_adjacent_pairs_of_part_of_a_head(M, T, heads, kv, D, rope_dim, sections, dtype):
+    import test_paged_attention as A
+
+    A.test_append_matches_definition(M, T, heads, kv, D, 16, dtype, rope_dim, "adjacent", sections, True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_and_attention_each_within_its_bound(M, dtype):
+    """A prompt in two chunks and a token: what append stores and returns against the definition, and the attention of those
+    stored values (no rounding in between) against the definition."""
+    import attention_oracle as AO
+
+    heads, kv, D, page, n = 8, 2, 128, 16, 75
+    g = torch.Generator(device="cuda").manual_seed(4)
+    k_pool, v_pool = M.kv_pools(8, kv, page, D, dtype=dtype)
+    k_pool.fill_(math.nan), v_pool.fill_(math.nan)
+    table = i32([[6, 1, 3, 0, 7]])
+    rope = M.rope_table(D, 100)
+    norm = (1 + torch.randn(D, generator=g, device="cuda") * 0.1).to(dtype)
+    att = M.PagedAttention(M.AttentionConfig(heads, kv, D, rope_dim=D), k_pool, v_pool, rope_table=rope, q_norm=norm, k_norm=norm)
+    q, k, v = (torch.randn((n, h, D), generator=g, device="cuda").to(dtype) for h in (heads, kv, kv))
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    slots = M.page_slots(table, torch.zeros_like(pos), pos, page)
+    outs, turned = [], []
+    for a, z in ((0, 50), (50, 74), (74, 75)):
+        turned.append(att.append(q[a:z], k[a:z], v[a:z], pos[a:z], slots[a:z]))
+        outs.append(att.prefill(turned[-1], i32([0, z - a]), i32([z]), table) if z - a > 1 else
+                    att.decode(turned[-1], i32([z]), table))
+    att.check()
+    turned = torch.cat(turned)
+    for got, x in ((turned, q), (k_pool[slots // page, :, slots % page], k)):
+        want, bound = AO.append(x, norm, 1e-6, rope, pos[None], (D // 2,), D, False)
+        AO.assert_within(got, want, bound + AO.rounding(want, dtype), "append")
+    want = AO.run(turned, k_pool.nan_to_num(0.0), v_pool.nan_to_num(0.0), table, [n], [0, n], 1 / math.sqrt(D), 0.0, 0, AO.U[dtype])
+    AO.assert_within(torch.cat(outs), want[0], want[1], "attention")
