@@ -116,3 +116,9 @@ def test_the_grouped_gemm_reads_its_error_word_once():
     read = body.index("p.err) ==")
     assert "if (threadIdx.x == 0) s_abort = " in body[read - 90:read]
     assert "__syncthreads();" in body[read:body.index("if (s_abort) return;")] and body.count("s_abort = 0") == 0
+
+
+def test_no_device_wide_limit_is_changed():
+    """A limit of the context is its other users' too (a stack reserve of 16 KB per thread held 5 GB of the device)."""
+    for path in glob.glob(os.path.join(CSRC, "*.c*")):
+        assert "DeviceSetLimit" not in text_of(path) and "CtxSetLimit" not in text_of(path), path
