@@ -991,13 +991,8 @@ moe_status launch_prefill(const moe_attn& a, const PrefillParams& p, cudaStream_
   const cuuint32_t y_box[3] = {64, whole ? (cuuint32_t)p.group : 1, whole ? 32u / p.group : 1};
   CUtensorMap y_map;
   MOE_TRY(encode_tmap_sw128(&y_map, map_type(a.d.dtype), 3, p.y, dims, y_strides, y_box));
-  // head_dim 64: the kernel keeps one word in local memory. Chains of overlapped launches with kernels that use local memory
-  // have ended in illegal accesses whose cause is not settled, so this one starts after the kernel before it has ended
-  // (short chunks 24.6 us against 23.0 with the overlap).
-  const bool overlap = a.d.head_dim != 64;
   return with_kernel(a, [&](auto kernel, int smem) -> moe_status {
-    MOE_CUDA_TRY(
-        launch_pdl_if(overlap, kernel, dim3(grid), dim3(PF_THREADS), smem, st, p, q_map, a.k_map, a.v_map, y_map));
+    MOE_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(PF_THREADS), smem, st, p, q_map, a.k_map, a.v_map, y_map));
     return MOE_OK;
   });
 }
