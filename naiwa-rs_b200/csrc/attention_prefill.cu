@@ -356,11 +356,13 @@ __device__ __forceinline__ Piece piece_of(const PrefillParams& p, const Batch& s
 }
 
 // Half steps that a piece more costs its join (256 rows of D f32 values against a step's products and, capped, three
-// exponential-unit results per score). Measured, costs 0 / 1 / 3: 64 rows behind 4096 tokens, D 128: 36 / 34 / 34 us; 200
-// rows 20 / 13 / 13; 128 behind 512: 27 / 24 / 18; short capped chunks with D 64: 23 / 23 / 37.
+// exponential-unit results per score). Measured (captured calls, 32 + 4 heads, bf16), costs 0 / 1 / 2 / 3: heads of 128, 64 rows behind
+// 4096 tokens 34.2 / 34.1 / 33.8 / 33.8 us, 200 rows 19.3 / 12.2 / 12.1 / 12.1, 128 behind 512 25.8 / 22.4 / 22.3 / 16.9; the same
+// capped 40.2 / 44.8 / 49.2 / 49.2, 22.0 / 16.8 / 16.8 / 16.7, 28.6 / 27.2 / 29.8 / 28.5; heads of 64, 64 behind 4096
+// 23.2 / 24.0 / 25.4 / 25.4, capped 40 behind 700 19.7 / 21.0 / 24.5 / 30.6.
 template <int D, bool CAP>
 struct JoinCost {
-  static constexpr int value = D == 64 ? 1 : CAP ? 2 : 3;
+  static constexpr int value = D == 64 || CAP ? 1 : 3;
 };
 
 template <class T, int D, bool CAP>
