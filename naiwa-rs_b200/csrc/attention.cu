@@ -25,7 +25,8 @@ namespace attn {
 constexpr int APPEND_THREADS = 256;
 // A window above this (2,080,374,784 positions) is none: position arithmetic beside it would leave 32 bits.
 constexpr int MAX_WINDOW = 0x7c000000;
-// Rows per lane group, measured at 4096 tokens of 32 + 2 x 4 heads of 128: 2 rows 33.8 us, 4: 20.2 (4.3 TB/s), 8: 21.2.
+// Rows per lane group, measured at 4096 tokens of 32 + 2 x 4 heads of 128: 2 rows 33.8 us, 4: 20.2, 8: 21.2 (4 in a whole call:
+// 21.6, 4.0 TB/s).
 constexpr int ROWS = 4;
 
 struct AppendParams {

@@ -22,8 +22,11 @@
 // not notice the extra MMAs. In f16 they are scaled by 2^14 first, so that a weight's parts stay above the type's
 // smallest value down to 2^-39 of the largest weight; sums are scaled alike and the quotient is the same.
 //
-// Measured on a B200, whole calls, bf16, 32 + 4 heads of 128: 128 sequences of 1 to 8191 tokens 177 us (6.1 TB/s, 94% of a
-// measured copy), one of 131071 53 us (5.1 TB/s), 32 of 128 to 2304 24 us, one of 129 8 us (5.4 on the device).
+// "Each byte once" holds for groups of up to 16 query heads; a larger group's heads are taken 16 at a time, and each 16 read the
+// cache again (through L2 where it still holds it).
+//
+// Measured on a B200, whole calls, bf16, 32 + 4 heads of 128: 128 sequences of 1 to 8191 tokens 176 us (6.1 TB/s, 95% of a
+// measured copy), one of 131071 53 us (5.1 TB/s), 32 of 128 to 2304 23 us, one of 129 8 us (5.4 on the device).
 // Four warps and two CTAs per SM against eight and one: 170 against 183 us for the batch (one CTA's joins leave its SM idle).
 #include <algorithm>
 

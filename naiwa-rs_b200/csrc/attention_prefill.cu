@@ -21,8 +21,10 @@
 //     take the rest of the type's range, another 2^11, so that only those below 2^-36 of the reference vanish.
 // Bound by the tensor cores (1024 clocks of MMA per 128 x 128 step) and as much by the exponentials (16 per clock and SM).
 // Measured on a B200: a step of two tiles takes about 3050 clocks of the 2062 that its MMAs need; the rest is the chain from
-// scores to weights and back. A 4096-token prompt of 32 + 4 heads of 128: 123 us alone (1.12 PFLOP/s, 66% of the measured
-// burst peak), 144 under sustained load. Not taken: two threads a row (197 us against 157), an MMA warp per tile (137 against
+// scores to weights and back. A 4096-token prompt of 32 + 4 heads of 128: 142 us (0.97 PFLOP/s, 58% of the measured burst
+// peak, 69% of the sustained one). The weights' rounding (8 bits in bf16, 11 in f16) is what tcgen05.mma takes: errors
+// against 64 bits are 2.0e-3 to 2.3e-3 in bf16 where f32 weights give 1.6e-3, 2.6e-4 against 2.1e-4 in f16. Not taken
+// (times of the steps they were weighed in, on a rested GPU): two threads a row (197 us against 157), an MMA warp per tile (137 against
 // 129), three stages of K or V (129 against 127), exponentials by polynomials (125 to 131 against 126).
 //
 // Every wait is bounded (moe_attn_set_wait_limit): one that runs out sets MOE_ERR_TIMEOUT, the CTA stops issuing work, waits for
