@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(P2P_THREADS) peer_receive_kernel(PeerPtrs peer
     const size_t row = i / k;
     const int s = (int)(row / cap), pos = (int)(row % cap);
     if (pos < cnt[s]) {  // peer-written: L2-coherent loads, no stale L1 line from an earlier epoch
-      ids[i] = __ldcg(rid + i);
-      w[i] = __ldcg(rw + i);
+      ids[i] = ld_l2(rid + i);
+      w[i] = ld_l2(rw + i);
     } else {
       ids[i] = MOE_ID_NONE;
       w[i] = 0.0f;
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(P2P_THREADS) peer_combine_kernel(PeerPtrs peer
     for (int r = 0; r < W && ok; ++r) {
       const int row = token_rows[(size_t)t * W + r];
       if (row < 0 || row - start[r] >= cap) continue;  // rows past the region were never sent
-      const uint4 v = __ldcg(ret + ((size_t)r * cap + (row - start[r])) * H8 + c);  // peer-written
+      const uint4 v = ld_l2(ret + ((size_t)r * cap + (row - start[r])) * H8 + c);  // peer-written
       const __nv_bfloat162* b = reinterpret_cast<const __nv_bfloat162*>(&v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {

@@ -219,6 +219,7 @@ __device__ __forceinline__ int32_t ld_l2(const int32_t* p) {
   asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
+__device__ __forceinline__ uint32_t ld_l2(const uint32_t* p) { return (uint32_t)ld_l2(reinterpret_cast<const int32_t*>(p)); }
 __device__ __forceinline__ float ld_l2(const float* p) {
   float v;
   asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
@@ -238,6 +239,10 @@ __device__ __forceinline__ int4 ld_l2(const int4* p) {
   int4 v;
   asm volatile("ld.global.cg.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
+}
+__device__ __forceinline__ uint4 ld_l2(const uint4* p) {
+  const int4 v = ld_l2(reinterpret_cast<const int4*>(p));
+  return make_uint4(v.x, v.y, v.z, v.w);
 }
 
 // 16 bytes of token rows, which the kernel before may have written: a plain access, ordered behind pdl_wait().

@@ -122,3 +122,10 @@ def test_no_device_wide_limit_is_changed():
     """A limit of the context is its other users' too (a stack reserve of 16 KB per thread held 5 GB of the device)."""
     for path in glob.glob(os.path.join(CSRC, "*.c*")):
         assert "DeviceSetLimit" not in text_of(path) and "CtxSetLimit" not in text_of(path), path
+
+
+@pytest.mark.parametrize("path", sorted(glob.glob(os.path.join(CSRC, "*.cu*"))), ids=os.path.basename)
+def test_loads_of_what_others_write_are_ordered(path):
+    """__ldcg carries no order against a wait, nor against the test that guards it: what a peer or another CTA wrote is read by
+    ld_l2."""
+    assert "__ldcg(" not in text_of(path)
