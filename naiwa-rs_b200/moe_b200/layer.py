@@ -371,6 +371,9 @@ class Router:
         if stream is not None:
             return run_on(stream, x.get_device(), self.route, x, out_ids=out_ids, out_weights=out_weights)
         torch = _torch()
+        if x.dim() != 2 or x.shape[1] != self.H or x.dtype != torch.bfloat16 or x.get_device() != self.w.get_device():
+            raise MoeError(_lib.MOE_ERR_INVALID, "Router.route: x must be [T, hidden] bf16 on the gate's device")
+        x = x.contiguous()
         T = x.shape[0]
         if T > self.max_tokens:
             raise MoeError(_lib.MOE_ERR_INVALID, "Router.route: T exceeds max_tokens")
